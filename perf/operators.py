@@ -202,15 +202,16 @@ def _quantize(x):
     """A row's scale is its largest magnitude / 127."""
     x = x.float()
     most = x.abs().amax(1)
-    inv = torch.where(most > 0, 127 / most, torch.zeros_like(most))
-    return torch.round(x * inv[:, None]).to(torch.int8), most / 127
+    top = torch.full_like(most, 127)  # (a tensor: by a number, torch multiplies by its rounded reciprocal)
+    inv = torch.where(most > 0, top / most, torch.zeros_like(most))
+    return torch.round(x * inv[:, None]).to(torch.int8), most / top
 
 
 def _to_4_bits(x):
     """bf16 [..., HEAD] -> codes (fp32 whole numbers), step and low (bf16 [...])."""
     x = x.float()
     low, high = x.amin(-1), x.amax(-1)
-    step = ((high - low) / 15).bfloat16()
+    step = ((high - low) / torch.full_like(low, 15)).bfloat16()
     by = torch.where(step > 0, step.float(), torch.full_like(low, math.inf))  # one value alone: code 0
     code = torch.round((x - low[..., None]) / by[..., None]).clamp(0, 15)
     return code, step, low.bfloat16()
