@@ -136,6 +136,16 @@ const char* fdllm_error_string(int code) {
   }
 }
 
+int fdllm_stream_capture_id(cudaStream_t stream, uint64_t* id) {
+  if (id == nullptr) return FDLLM_ERR_ARG;
+  *id = 0;
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  unsigned long long cid = 0;
+  if (cudaStreamGetCaptureInfo(stream, &st, &cid) != cudaSuccess) return FDLLM_ERR_CUDA;
+  if (st == cudaStreamCaptureStatusActive) *id = cid;
+  return FDLLM_OK;
+}
+
 int fdllm_status_read(int32_t out[4], cudaStream_t stream) {
   int32_t* d = fdllm::status_ptr();
   if (d == nullptr || out == nullptr) return FDLLM_ERR_CUDA;

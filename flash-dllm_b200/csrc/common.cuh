@@ -197,6 +197,27 @@ __device__ __forceinline__ void umma_bf16(uint32_t d_tmem, uint64_t a_desc, uint
       : "memory");
 }
 
+// D[tmem] (+)= A[smem] * B[smem]^T, signed 8-bit inputs, exact 32-bit integer
+// accumulate, one CTA.  An instruction takes 32 K: the same 32 bytes of every
+// operand row as a bf16 one.
+__device__ __forceinline__ void umma_s8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+template <bool I8>
+__device__ __forceinline__ void umma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                     uint32_t accumulate) {
+  if (I8)
+    umma_s8(d_tmem, a_desc, b_desc, idesc, accumulate);
+  else
+    umma_bf16(d_tmem, a_desc, b_desc, idesc, accumulate);
+}
+
 // Arrive on ``bar`` once all previously issued tcgen05.mma of this thread
 // have completed (their smem operands may then be overwritten).
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
@@ -329,6 +350,16 @@ __host__ __device__ constexpr uint32_t umma_idesc_bf16(int M, int N) {
          | (static_cast<uint32_t>(M >> 4) << 24);    // M / 16
 }
 
+// Instruction descriptor: kind::i8, A = B = signed 8-bit, D = int32, both
+// K-major (D format 2 = S32, A / B format 1 = S8; no saturation).
+__host__ __device__ constexpr uint32_t umma_idesc_s8(int M, int N) {
+  return (2u << 4)                                   // D format int32
+         | (1u << 7)                                 // A format signed 8-bit
+         | (1u << 10)                                // B format signed 8-bit
+         | (static_cast<uint32_t>(N >> 3) << 17)     // N / 8
+         | (static_cast<uint32_t>(M >> 4) << 24);    // M / 16
+}
+
 // Instruction-descriptor bit that marks the B operand MN-major.
 constexpr uint32_t kUmmaBMajorMN = 1u << 16;
 
@@ -397,6 +428,23 @@ __device__ __forceinline__ void umma_bf16_pair(uint32_t d_tmem, uint64_t a_desc,
       "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+__device__ __forceinline__ void umma_s8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                             uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+template <bool I8>
+__device__ __forceinline__ void umma_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t accumulate) {
+  if (I8)
+    umma_s8_pair(d_tmem, a_desc, b_desc, idesc, accumulate);
+  else
+    umma_bf16_pair(d_tmem, a_desc, b_desc, idesc, accumulate);
 }
 // arrive on the mbarrier at `bar_cluster_addr` (either CTA of the pair) once
 // all earlier pair MMAs issued by this thread have completed

@@ -13,6 +13,17 @@
 //              bf16(bf16(silu(bf16(gate_j))) * bf16(up_j)), so the gate / up
 //              activations never reach HBM (ref :628-633).
 //
+// With I8 the operands are 8-bit integers (kind::i8, exact 32-bit integer
+// accumulators) and the epilogue's value is
+//   float(sum_k a[r, k] w[c, k]) * sa[r] * sw[c],
+// a scale per token (row of A) and per output channel (row of B).  A stage's
+// 128-byte operand rows then hold 128 K instead of 64, and a UMMA consumes
+// the same 32 bytes of every row as a bf16 one, so every size below that
+// counts "64-K boxes" counts 128-byte boxes: the tensor maps are the bf16
+// ones over K / 2 columns, and the tiles, ring, schedule and descriptors are
+// shared.  Stream-K partials are the 32-bit integers themselves: a sum split
+// over CTAs is exact whatever the split.
+//
 // Work decomposition.  A tile is 128 rows x BN columns (BN = 128 or 256
 // UMMA columns).  The CTAs form one group per 128-row m-tile; each group
 // covers the (column tile, k-block) space of its m-tile, one contiguous range
@@ -59,6 +70,9 @@ constexpr int kGRingBytes = 160 * 1024;
 constexpr size_t kGFlagBytes = 4096;  // one int32 flag per CTA (grid <= 1024)
 constexpr int kGStageBytes = 8 * 32 * 64 * 4;  // epilogue staging: 8 warps x 32 rows x 64 fp32
 
+// int8 products of at most 128 * 128: 131,071 of them stay below 2^31
+constexpr int kGMaxKInt8 = 131056;  // (a multiple of 16)
+
 enum GemmEpi { kEpiQkv = 0, kEpiStore = 1, kEpiSwiglu = 2 };
 
 template <int BN, int XROWS, int KSUB>
@@ -99,6 +113,8 @@ struct GemmParams {
   const int64_t* pos;
   const float* sin;
   const float* cos;
+  const float* sa;   // I8: scale of each A row
+  const float* sw;   // I8: scale of each output channel (swiglu: gate channels, then up channels)
   float* partials;   // [grid][BN / 4][128][4] fp32
   int32_t* flags;    // [grid]
   int32_t* status;
@@ -156,7 +172,13 @@ __device__ __forceinline__ bool g_more(const GIter& it, const GemmParams& p) {
 // all partial loads are in flight together (one L2 latency per pair).
 // Contributors [q0, q0 + n_smem) were copied (in order) into shared memory
 // at `spart`; the others are read from the workspace.
-template <int BN, int PR>
+// sum of two accumulator words: fp32, or int32 held in a float's bits (I8)
+template <bool I8>
+__device__ __forceinline__ float g_add(float a, float b) {
+  return I8 ? __int_as_float(__float_as_int(a) + __float_as_int(b)) : a + b;
+}
+
+template <int BN, int PR, bool I8>
 __device__ __forceinline__ void g_chunk2(uint32_t t_row, int ca, int cb, const GemmParams& p, int q0, int q1, int qmul,
                                          int qadd, const float4* spart, int n_smem, int r_tile, float (&va)[32],
                                          float (&vb)[32]) {
@@ -175,14 +197,14 @@ __device__ __forceinline__ void g_chunk2(uint32_t t_row, int ca, int cb, const G
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      va[4 * j] += xa[j].x;
-      va[4 * j + 1] += xa[j].y;
-      va[4 * j + 2] += xa[j].z;
-      va[4 * j + 3] += xa[j].w;
-      vb[4 * j] += xb[j].x;
-      vb[4 * j + 1] += xb[j].y;
-      vb[4 * j + 2] += xb[j].z;
-      vb[4 * j + 3] += xb[j].w;
+      va[4 * j] = g_add<I8>(va[4 * j], xa[j].x);
+      va[4 * j + 1] = g_add<I8>(va[4 * j + 1], xa[j].y);
+      va[4 * j + 2] = g_add<I8>(va[4 * j + 2], xa[j].z);
+      va[4 * j + 3] = g_add<I8>(va[4 * j + 3], xa[j].w);
+      vb[4 * j] = g_add<I8>(vb[4 * j], xb[j].x);
+      vb[4 * j + 1] = g_add<I8>(vb[4 * j + 1], xb[j].y);
+      vb[4 * j + 2] = g_add<I8>(vb[4 * j + 2], xb[j].z);
+      vb[4 * j + 3] = g_add<I8>(vb[4 * j + 3], xb[j].w);
     }
   }
 }
@@ -260,6 +282,23 @@ __device__ __forceinline__ void g_stage_get8(const float4* stage, int r, int u, 
   v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
 }
 
+// I8: the scales of channels col .. col + 7 (16-byte loads: `sw` is 16-byte
+// aligned and col a multiple of 8; channels at or past n are not read), and
+// the accumulators as scaled fp32.  The product of the integer with the
+// token's scale is formed first: it is the size of an activation, so neither
+// order of large and small scales can overflow on the way.
+__device__ __forceinline__ void g_load_scales(const float* sw, int col, int n, float (&w)[8]) {
+  const bool in = col < n;  // n is a multiple of 8
+  const float4 a = in ? __ldg(reinterpret_cast<const float4*>(sw + col)) : make_float4(0.f, 0.f, 0.f, 0.f);
+  const float4 b = in ? __ldg(reinterpret_cast<const float4*>(sw + col) + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
+  w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+  w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+}
+__device__ __forceinline__ void g_apply_scales(float (&v)[8], float sa, const float (&w)[8]) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = static_cast<float>(__float_as_int(v[k])) * sa * w[k];
+}
+
 // Epilogue of one tile on this CTA's accumulator rows (global rows row0 +
 // r), by the 8 epilogue warps: warp quarter w holds rows RQ w .. RQ w + RQ - 1
 // in its TMEM lanes 0 .. RQ - 1 (RQ = 32 for M = 128 accumulators, 16 for
@@ -267,7 +306,7 @@ __device__ __forceinline__ void g_stage_get8(const float4* stage, int r, int u, 
 // `half` 0 / 1 takes the even / odd column groups.  `slot` is the QKV cache
 // slot of this thread's row (-1: not written).  Lanes past RQ read row 0 of
 // their quarter's partials and write nothing.
-template <int BN, int EPI, int PR, int RQ>
+template <int BN, int EPI, int PR, int RQ, bool I8>
 __device__ __forceinline__ void g_tile_epilogue(const GemmParams& p, uint32_t t_row, float4* stage, int quarter,
                                                 int half, int lane, int row0, int n_tile, int q0, int q1, int qmul,
                                                 int qadd, const float4* spart, int n_smem, int64_t slot,
@@ -291,7 +330,7 @@ __device__ __forceinline__ void g_tile_epilogue(const GemmParams& p, uint32_t t_
       for (int g = 0; g < group; ++g) {
         const int hh = h0 + g;
         float va[32], vb[32];
-        g_chunk2<BN, PR>(t_row, hh * 128 + half * 32, hh * 128 + 64 + half * 32, p, q0, q1, qmul, qadd, spart,
+        g_chunk2<BN, PR, I8>(t_row, hh * 128 + half * 32, hh * 128 + 64 + half * 32, p, q0, q1, qmul, qadd, spart,
                          n_smem, r_tile, va, vb);
         g_stage_put(g == 0 ? stage : stage2, lane, va, vb);
       }
@@ -366,7 +405,7 @@ __device__ __forceinline__ void g_tile_epilogue(const GemmParams& p, uint32_t t_
       const int col0 = n_tile * BN + g;
       if (col0 >= p.n_cols) break;  // uniform
       float va[32], vb[32];
-      g_chunk2<BN, PR>(t_row, g, g + 32, p, q0, q1, qmul, qadd, spart, n_smem, r_tile, va, vb);
+      g_chunk2<BN, PR, I8>(t_row, g, g + 32, p, q0, q1, qmul, qadd, spart, n_smem, r_tile, va, vb);
       g_stage_put(stage, lane, va, vb);
       __syncwarp();
       // 8 lanes per row: lane takes columns col0 + 8 sub .. + 7 of rows
@@ -374,6 +413,8 @@ __device__ __forceinline__ void g_tile_epilogue(const GemmParams& p, uint32_t t_
       // together
       const int sub = lane & 7;
       const int col = col0 + 8 * sub;
+      float wsc[8];
+      if (I8) g_load_scales(p.sw, col, p.n_cols, wsc);
       uint4 rv[8];
       if (p.res != nullptr) {
 #pragma unroll
@@ -391,6 +432,7 @@ __device__ __forceinline__ void g_tile_epilogue(const GemmParams& p, uint32_t t_
         float v[8];
         g_stage_get8(stage, rr, 2 * sub, v);
         if (row >= p.n_rows || col >= p.n_cols) continue;
+        if (I8) g_apply_scales(v, __ldg(p.sa + row), wsc);
         if (p.res != nullptr) {
           const uint32_t w[4] = {rv[it].x, rv[it].y, rv[it].z, rv[it].w};
 #pragma unroll
@@ -409,11 +451,16 @@ __device__ __forceinline__ void g_tile_epilogue(const GemmParams& p, uint32_t t_
 #pragma unroll 1
     for (int c0 = half * 32; c0 < BN / 2; c0 += 64) {
       float gv[32], uv[32];
-      g_chunk2<BN, PR>(t_row, c0, BN / 2 + c0, p, q0, q1, qmul, qadd, spart, n_smem, r_tile, gv, uv);
+      g_chunk2<BN, PR, I8>(t_row, c0, BN / 2 + c0, p, q0, q1, qmul, qadd, spart, n_smem, r_tile, gv, uv);
       g_stage_put(stage, lane, gv, uv);
       __syncwarp();
       const int sub = lane & 3;
       const int col = n_tile * (BN / 2) + c0 + 8 * sub;
+      float wsg[8], wsu[8];
+      if (I8) {
+        g_load_scales(p.sw, col, p.hidden, wsg);
+        g_load_scales(p.sw + p.hidden, col, p.hidden, wsu);
+      }
 #pragma unroll 1
       for (int it = 0; it < RQ / 8; ++it) {
         const int rr = it * 8 + (lane >> 2);
@@ -422,6 +469,11 @@ __device__ __forceinline__ void g_tile_epilogue(const GemmParams& p, uint32_t t_
         g_stage_get8(stage, rr, 2 * sub, g8);
         g_stage_get8(stage, rr, 8 + 2 * sub, u8);
         if (row >= p.n_rows) continue;
+        if (I8) {
+          const float sa = __ldg(p.sa + row);
+          g_apply_scales(g8, sa, wsg);
+          g_apply_scales(u8, sa, wsu);
+        }
         // silu with the fast exp / divide intrinsics: their few-ulp fp32 error
         // sits far below the bf16 rounding that follows, and the IEEE forms
         // serialise into ~140 cycles per element here
@@ -484,7 +536,7 @@ __device__ __forceinline__ const CUtensorMap* g_b_coord(const GemmParams& p, int
   return m0;
 }
 
-template <int BN, int XROWS, int KSUB, int EPI>
+template <int BN, int XROWS, int KSUB, int EPI, bool I8>
 __global__ void __launch_bounds__(kGThreads, 1)
     gemm_sk_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b0,
                    const __grid_constant__ CUtensorMap map_b1, const __grid_constant__ CUtensorMap map_b2,
@@ -598,7 +650,8 @@ __global__ void __launch_bounds__(kGThreads, 1)
     // -------------------------------------------------------- MMA issuer --
     if (lane == 0) {
       // M = 64 UMMAs for 64-row A tiles (no idle accumulator rows)
-      constexpr uint32_t idesc = umma_idesc_bf16(XROWS == 64 ? 64 : kGBM, BN);
+      constexpr uint32_t idesc = I8 ? umma_idesc_s8(XROWS == 64 ? 64 : kGBM, BN)
+                                    : umma_idesc_bf16(XROWS == 64 ? 64 : kGBM, BN);
       uint32_t g = 0;
       int seg = 0;
       bool ok = true;
@@ -624,7 +677,7 @@ __global__ void __launch_bounds__(kGThreads, 1)
             const uint64_t db = umma_desc_kmajor_sw128(smem_u32(a0 + C::kABytes + sub * C::kBSub));
 #pragma unroll
             for (int k = 0; k < kGBK / 16; ++k)
-              umma_bf16(d_tmem, da + 2 * k, db + 2 * k, idesc, (kb > sg.k0 || sub > 0 || k > 0) ? 1u : 0u);
+              umma<I8>(d_tmem, da + 2 * k, db + 2 * k, idesc, (kb > sg.k0 || sub > 0 || k > 0) ? 1u : 0u);
           }
           umma_commit(&empty[s]);
         }
@@ -702,7 +755,7 @@ __global__ void __launch_bounds__(kGThreads, 1)
       // contributors' partials: a second staging area for the QKV epilogue
       float4* stage2 = (!g_more<false>(it, p) && q_end == cta + 1)
                            ? reinterpret_cast<float4*>(smem) + (warp - 4) * (32 * 16) : nullptr;
-      g_tile_epilogue<BN, EPI, XROWS, kRQ>(p, t_row, stage, quarter, half, lane, row0, n_tile, cta + 1, q_end, 1, 0,
+      g_tile_epilogue<BN, EPI, XROWS, kRQ, I8>(p, t_row, stage, quarter, half, lane, row0, n_tile, cta + 1, q_end, 1, 0,
                                            reinterpret_cast<const float4*>(smem), n_smem, slot, stage2);
       // every column of this accumulator has been read
       tc_fence_before();
@@ -749,7 +802,7 @@ struct G2Cfg {
   static_assert(kSmem <= 232448, "shared memory");
 };
 
-template <int KSUB, int EPI, bool WAVES>
+template <int KSUB, int EPI, bool WAVES, bool I8>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
     gemm_sk2_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b0,
                     const __grid_constant__ CUtensorMap map_b1, const __grid_constant__ CUtensorMap map_b2,
@@ -865,7 +918,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
   } else if (warp == 1) {
     // -------------------------------------------- MMA issuer (leader only) --
     if (rank == 0 && lane == 0) {
-      constexpr uint32_t idesc = umma_idesc_bf16(2 * kGBM, BN);
+      constexpr uint32_t idesc = I8 ? umma_idesc_s8(2 * kGBM, BN) : umma_idesc_bf16(2 * kGBM, BN);
       uint32_t g = 0;
       int seg = 0;
       bool ok = true;
@@ -891,7 +944,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
             const uint64_t db = umma_desc_kmajor_sw128(smem_u32(a0 + C::kABytes + sub * C::kSub));
 #pragma unroll
             for (int k = 0; k < kGBK / 16; ++k)
-              umma_bf16_pair(d_tmem, da + 2 * k, db + 2 * k, idesc, (kb > sg.k0 || sub > 0 || k > 0) ? 1u : 0u);
+              umma_pair<I8>(d_tmem, da + 2 * k, db + 2 * k, idesc, (kb > sg.k0 || sub > 0 || k > 0) ? 1u : 0u);
           }
           umma_commit_pair(mapa_shared(&empty[s], 0));
           umma_commit_pair(mapa_shared(&empty[s], 1));
@@ -959,7 +1012,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
       // operand ring is free unless it holds contributors' partials
       float4* stage2 = (!g_more<WAVES>(it, p) && q_end == pair + 1)
                            ? reinterpret_cast<float4*>(smem) + (warp - 4) * (32 * 16) : nullptr;
-      g_tile_epilogue<BN, EPI, kGBM, 32>(p, t_row, stage, quarter, half, lane, row0, n_tile, pair + 1, q_end, 2,
+      g_tile_epilogue<BN, EPI, kGBM, 32, I8>(p, t_row, stage, quarter, half, lane, row0, n_tile, pair + 1, q_end, 2,
                                static_cast<int>(rank), reinterpret_cast<const float4*>(smem), n_smem, slot, stage2);
       tc_fence_before();
       __syncwarp();
@@ -1001,16 +1054,16 @@ GemmOverride& gemm_override() {
 
 // Resident 2-CTA clusters of a pair-kernel configuration (an SM count that
 // is odd within a GPC leaves SMs out); cached per device and configuration.
-template <int KSUB, int EPI>
+template <int KSUB, int EPI, bool I8>
 int g2_max_pairs() {
   static int cache[64] = {0};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
   if (cache[dev] == 0) {
     using C = G2Cfg<KSUB>;
-    if (cudaFuncSetAttribute(gemm_sk2_kernel<KSUB, EPI, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    if (cudaFuncSetAttribute(gemm_sk2_kernel<KSUB, EPI, false, I8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              C::kSmem) != cudaSuccess ||
-        cudaFuncSetAttribute(gemm_sk2_kernel<KSUB, EPI, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        cudaFuncSetAttribute(gemm_sk2_kernel<KSUB, EPI, true, I8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              C::kSmem) != cudaSuccess)
       return 0;
     cudaLaunchConfig_t cfg = {};
@@ -1018,17 +1071,19 @@ int g2_max_pairs() {
     cfg.blockDim = dim3(kGThreads, 1, 1);
     cfg.dynamicSmemBytes = C::kSmem;
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, gemm_sk2_kernel<KSUB, EPI, false>, &cfg) != cudaSuccess || n <= 0)
+    if (cudaOccupancyMaxActiveClusters(&n, gemm_sk2_kernel<KSUB, EPI, false, I8>, &cfg) != cudaSuccess || n <= 0)
       return 0;
     cache[dev] = n;
   }
   return cache[dev];
 }
 
+template <bool I8>
 int g2_max_pairs_for(int epi, int ksub) {
-  if (epi == kEpiQkv) return ksub == 2 ? g2_max_pairs<2, kEpiQkv>() : g2_max_pairs<1, kEpiQkv>();
-  if (epi == kEpiStore) return ksub == 2 ? g2_max_pairs<2, kEpiStore>() : g2_max_pairs<1, kEpiStore>();
-  return ksub == 2 ? g2_max_pairs<2, kEpiSwiglu>() : g2_max_pairs<1, kEpiSwiglu>();
+  if (epi == kEpiStore) return ksub == 2 ? g2_max_pairs<2, kEpiStore, I8>() : g2_max_pairs<1, kEpiStore, I8>();
+  if (epi == kEpiSwiglu) return ksub == 2 ? g2_max_pairs<2, kEpiSwiglu, I8>() : g2_max_pairs<1, kEpiSwiglu, I8>();
+  // (the QKV epilogue is bf16 only)
+  return ksub == 2 ? g2_max_pairs<2, kEpiQkv, false>() : g2_max_pairs<1, kEpiQkv, false>();
 }
 
 // Up to 128 rows: single CTAs with 128-column tiles, stream-K (the kernel
@@ -1039,7 +1094,10 @@ int g2_max_pairs_for(int epi, int ksub) {
 // one whole tile each with no fix-ups when the tiles nearly fill the grid
 // (attn_out: 4096 x 4096 at 4 x 128 rows), stream-K otherwise.  Ring stages: two 64-K boxes (256 B of every operand row per
 // request) for 64-row single CTAs, one 64-K box elsewhere.
-GemmPlan plan_gemm(int epi, int32_t n_rows, int32_t n_cols, int32_t k_dim, int32_t d_model) {
+//
+// I8: k_dim counts pairs of int8 (the 2-byte columns of the tensor maps); a
+// last box that reaches past it is zero-filled by the loads.
+GemmPlan plan_gemm(int epi, int32_t n_rows, int32_t n_cols, int32_t k_dim, int32_t d_model, bool i8 = false) {
   GemmPlan pl{};
   const GemmOverride& ov = gemm_override();
   const int out_cols = epi == kEpiSwiglu ? n_cols / 2 : n_cols;
@@ -1070,13 +1128,13 @@ GemmPlan plan_gemm(int epi, int32_t n_rows, int32_t n_cols, int32_t k_dim, int32
   if (!pl.pair && bn == 256 && pl.xrows == kGBM) ksub = 1;  // a 96 KB stage leaves one stage
   if (k_dim % (kGBK * ksub) != 0) ksub = 1;
   pl.ksub = ksub;
-  pl.kbt = k_dim / (kGBK * ksub);
+  pl.kbt = (k_dim + kGBK * ksub - 1) / (kGBK * ksub);
   pl.bn = bn;
   const int out_per_tile = epi == kEpiSwiglu ? bn / 2 : bn;
   pl.n_tiles = (out_cols + out_per_tile - 1) / out_per_tile;
   // every CTA must be resident at once (owners wait for contributors): at
   // most one CTA per SM, or the resident pairs
-  int units = pl.pair ? g2_max_pairs_for(epi, ksub) : sm_count();
+  int units = pl.pair ? (i8 ? g2_max_pairs_for<true>(epi, ksub) : g2_max_pairs_for<false>(epi, ksub)) : sm_count();
   if (units <= 0) units = pl.pair ? sm_count() / 2 : sm_count();
   if (ov.grid > 0 && ov.grid < units) units = ov.grid;
   if (units > (pl.pair ? 512 : 1024)) units = pl.pair ? 512 : 1024;
@@ -1117,7 +1175,7 @@ size_t gemm_ws_bytes(const GemmPlan& pl) {
   return kGFlagBytes + static_cast<size_t>(pl.grid) * kGBM * pl.bn * sizeof(float);
 }
 
-template <int BN, int XROWS, int KSUB, int EPI>
+template <int BN, int XROWS, int KSUB, int EPI, bool I8>
 int launch_gemm_cfg(const CUtensorMap& ma, const CUtensorMap& mb0, const CUtensorMap& mb1, const CUtensorMap& mb2,
                     const GemmParams& p, int grid, cudaStream_t stream) {
   using C = GCfg<BN, XROWS, KSUB>;
@@ -1125,57 +1183,58 @@ int launch_gemm_cfg(const CUtensorMap& ma, const CUtensorMap& mb0, const CUtenso
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return FDLLM_ERR_CUDA;
   if (!attr_set[dev]) {
-    if (cudaFuncSetAttribute(gemm_sk_kernel<BN, XROWS, KSUB, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    if (cudaFuncSetAttribute(gemm_sk_kernel<BN, XROWS, KSUB, EPI, I8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              C::kSmem) != cudaSuccess)
       return FDLLM_ERR_CUDA;
     attr_set[dev] = true;
   }
-  if (launch_ex(gemm_sk_kernel<BN, XROWS, KSUB, EPI>, dim3(grid), dim3(kGThreads), C::kSmem, stream, 1,
+  if (launch_ex(gemm_sk_kernel<BN, XROWS, KSUB, EPI, I8>, dim3(grid), dim3(kGThreads), C::kSmem, stream, 1,
                 pdl_enabled(), ma, mb0, mb1, mb2, p) != cudaSuccess)
     return FDLLM_ERR_CUDA;
   return cudaPeekAtLastError() == cudaSuccess ? FDLLM_OK : FDLLM_ERR_CUDA;
 }
 
-template <int KSUB, int EPI>
+template <int KSUB, int EPI, bool I8>
 int launch_gemm2_cfg(const CUtensorMap& ma, const CUtensorMap& mb0, const CUtensorMap& mb1, const CUtensorMap& mb2,
                      const GemmParams& p, int grid, cudaStream_t stream) {
   using C = G2Cfg<KSUB>;
-  if (g2_max_pairs<KSUB, EPI>() <= 0) return FDLLM_ERR_CUDA;  // also sets the shared-memory attribute
+  if (g2_max_pairs<KSUB, EPI, I8>() <= 0) return FDLLM_ERR_CUDA;  // also sets the shared-memory attribute
   // the kernel's __cluster_dims__ gives the pairs; no cluster attribute here
   const cudaError_t e =
       p.sk_tiles < p.tiles
-          ? launch_ex(gemm_sk2_kernel<KSUB, EPI, true>, dim3(grid), dim3(kGThreads), C::kSmem, stream, 1,
+          ? launch_ex(gemm_sk2_kernel<KSUB, EPI, true, I8>, dim3(grid), dim3(kGThreads), C::kSmem, stream, 1,
                       pdl_enabled(), ma, mb0, mb1, mb2, p)
-          : launch_ex(gemm_sk2_kernel<KSUB, EPI, false>, dim3(grid), dim3(kGThreads), C::kSmem, stream, 1,
+          : launch_ex(gemm_sk2_kernel<KSUB, EPI, false, I8>, dim3(grid), dim3(kGThreads), C::kSmem, stream, 1,
                       pdl_enabled(), ma, mb0, mb1, mb2, p);
   if (e != cudaSuccess) return FDLLM_ERR_CUDA;
   return cudaPeekAtLastError() == cudaSuccess ? FDLLM_OK : FDLLM_ERR_CUDA;
 }
 
-template <int EPI>
+template <int EPI, bool I8>
 int dispatch_gemm(const GemmPlan& pl, const CUtensorMap& ma, const CUtensorMap& mb0, const CUtensorMap& mb1,
                   const CUtensorMap& mb2, const GemmParams& p, cudaStream_t stream) {
   if (pl.pair)
-    return pl.ksub == 2 ? launch_gemm2_cfg<2, EPI>(ma, mb0, mb1, mb2, p, pl.grid, stream)
-                        : launch_gemm2_cfg<1, EPI>(ma, mb0, mb1, mb2, p, pl.grid, stream);
+    return pl.ksub == 2 ? launch_gemm2_cfg<2, EPI, I8>(ma, mb0, mb1, mb2, p, pl.grid, stream)
+                        : launch_gemm2_cfg<1, EPI, I8>(ma, mb0, mb1, mb2, p, pl.grid, stream);
   if (pl.bn == 256) {
     if (pl.xrows == 64)
-      return pl.ksub == 2 ? launch_gemm_cfg<256, 64, 2, EPI>(ma, mb0, mb1, mb2, p, pl.grid, stream)
-                          : launch_gemm_cfg<256, 64, 1, EPI>(ma, mb0, mb1, mb2, p, pl.grid, stream);
-    return launch_gemm_cfg<256, 128, 1, EPI>(ma, mb0, mb1, mb2, p, pl.grid, stream);
+      return pl.ksub == 2 ? launch_gemm_cfg<256, 64, 2, EPI, I8>(ma, mb0, mb1, mb2, p, pl.grid, stream)
+                          : launch_gemm_cfg<256, 64, 1, EPI, I8>(ma, mb0, mb1, mb2, p, pl.grid, stream);
+    return launch_gemm_cfg<256, 128, 1, EPI, I8>(ma, mb0, mb1, mb2, p, pl.grid, stream);
   }
   if (pl.xrows == 64)
-    return pl.ksub == 2 ? launch_gemm_cfg<128, 64, 2, EPI>(ma, mb0, mb1, mb2, p, pl.grid, stream)
-                        : launch_gemm_cfg<128, 64, 1, EPI>(ma, mb0, mb1, mb2, p, pl.grid, stream);
-  return pl.ksub == 2 ? launch_gemm_cfg<128, 128, 2, EPI>(ma, mb0, mb1, mb2, p, pl.grid, stream)
-                      : launch_gemm_cfg<128, 128, 1, EPI>(ma, mb0, mb1, mb2, p, pl.grid, stream);
+    return pl.ksub == 2 ? launch_gemm_cfg<128, 64, 2, EPI, I8>(ma, mb0, mb1, mb2, p, pl.grid, stream)
+                        : launch_gemm_cfg<128, 64, 1, EPI, I8>(ma, mb0, mb1, mb2, p, pl.grid, stream);
+  return pl.ksub == 2 ? launch_gemm_cfg<128, 128, 2, EPI, I8>(ma, mb0, mb1, mb2, p, pl.grid, stream)
+                      : launch_gemm_cfg<128, 128, 1, EPI, I8>(ma, mb0, mb1, mb2, p, pl.grid, stream);
 }
 
 // Shared set-up: plan, workspace split, tensor maps of A and of the weights.
+// I8: lda and k_dim count pairs of int8.
 int run_gemm(int epi, const void* a, int64_t lda, const void* const* w, int n_w, int64_t w_rows, int32_t n_rows,
              int32_t n_cols, int32_t k_dim, GemmParams& p, void* workspace, size_t workspace_bytes,
-             cudaStream_t stream) {
-  const GemmPlan pl = plan_gemm(epi, n_rows, n_cols, k_dim, p.d_model);
+             cudaStream_t stream, bool i8 = false) {
+  const GemmPlan pl = plan_gemm(epi, n_rows, n_cols, k_dim, p.d_model, i8);
   if (pl.iters < 0 || pl.tiles <= 0 || pl.grid <= 0) return FDLLM_ERR_ARG;
   if (workspace == nullptr || workspace_bytes < gemm_ws_bytes(pl) || !aligned16(workspace))
     return FDLLM_ERR_WORKSPACE;
@@ -1200,9 +1259,12 @@ int run_gemm(int epi, const void* a, int64_t lda, const void* const* w, int n_w,
   for (int i = 0; i < n_w; ++i)
     if ((rc = make_tmap_bf16_sw128(&mb[i], w[i], w_rows, k_dim, k_dim, box)) != FDLLM_OK) return rc;
   for (int i = n_w; i < 3; ++i) mb[i] = mb[0];
-  if (epi == kEpiQkv) return dispatch_gemm<kEpiQkv>(pl, ma, mb[0], mb[1], mb[2], p, stream);
-  if (epi == kEpiStore) return dispatch_gemm<kEpiStore>(pl, ma, mb[0], mb[1], mb[2], p, stream);
-  return dispatch_gemm<kEpiSwiglu>(pl, ma, mb[0], mb[1], mb[2], p, stream);
+  if (i8)
+    return epi == kEpiStore ? dispatch_gemm<kEpiStore, true>(pl, ma, mb[0], mb[1], mb[2], p, stream)
+                            : dispatch_gemm<kEpiSwiglu, true>(pl, ma, mb[0], mb[1], mb[2], p, stream);
+  if (epi == kEpiQkv) return dispatch_gemm<kEpiQkv, false>(pl, ma, mb[0], mb[1], mb[2], p, stream);
+  if (epi == kEpiStore) return dispatch_gemm<kEpiStore, false>(pl, ma, mb[0], mb[1], mb[2], p, stream);
+  return dispatch_gemm<kEpiSwiglu, false>(pl, ma, mb[0], mb[1], mb[2], p, stream);
 }
 
 }  // namespace
@@ -1278,6 +1340,59 @@ int fdllm_gemm_bf16(const void* a, const void* w, void* out, const void* residua
   p.ld_res = ld_res;
   const void* ws[1] = {w};
   return run_gemm(kEpiStore, a, k_dim, ws, 1, n_cols, n_rows, n_cols, k_dim, p, workspace, workspace_bytes, stream);
+}
+
+size_t fdllm_gemm_int8_workspace_bytes(int32_t n_rows, int32_t n_cols, int32_t k_dim, int32_t swiglu) {
+  if (n_rows <= 0 || n_cols <= 0 || k_dim <= 0) return fdllm::kGFlagBytes;
+  return fdllm::gemm_ws_bytes(
+      fdllm::plan_gemm(swiglu ? fdllm::kEpiSwiglu : fdllm::kEpiStore, n_rows, n_cols, (k_dim + 1) / 2, 0, true));
+}
+
+int fdllm_gemm_int8(const void* a, const float* a_scale, const void* w, const float* w_scale, void* out,
+                    const void* residual, int32_t n_rows, int32_t n_cols, int32_t k_dim, int64_t ld_out,
+                    int64_t ld_res, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  using namespace fdllm;
+  if (n_rows < 0 || n_cols <= 0 || k_dim <= 0 || n_cols % 8 != 0 || k_dim % 16 != 0 || k_dim > kGMaxKInt8 ||
+      ld_out < n_cols || ld_out % 8 != 0 || (residual != nullptr && (ld_res < n_cols || ld_res % 8 != 0)))
+    return FDLLM_ERR_ARG;
+  if (n_rows == 0) return FDLLM_OK;
+  const void* ptrs[] = {a, w, w_scale, out};
+  for (const void* x : ptrs)
+    if (x == nullptr || !aligned16(x)) return FDLLM_ERR_ARG;
+  if (a_scale == nullptr || (residual != nullptr && !aligned16(residual))) return FDLLM_ERR_ARG;
+  GemmParams p{};
+  p.out0 = static_cast<__nv_bfloat16*>(out);
+  p.res = static_cast<const __nv_bfloat16*>(residual);
+  p.ld_out = ld_out;
+  p.ld_res = ld_res;
+  p.sa = a_scale;
+  p.sw = w_scale;
+  const void* ws[1] = {w};
+  return run_gemm(kEpiStore, a, k_dim / 2, ws, 1, n_cols, n_rows, n_cols, k_dim / 2, p, workspace, workspace_bytes,
+                  stream, true);
+}
+
+int fdllm_gemm_swiglu_int8(const void* a, const float* a_scale, const void* w_gate_up, const float* w_scale, void* out,
+                           int32_t n_rows, int32_t hidden, int32_t k_dim, int64_t ld_out, void* workspace,
+                           size_t workspace_bytes, cudaStream_t stream) {
+  using namespace fdllm;
+  if (n_rows < 0 || hidden <= 0 || k_dim <= 0 || hidden % 128 != 0 || k_dim % 16 != 0 || k_dim > kGMaxKInt8 ||
+      ld_out < hidden || ld_out % 8 != 0)
+    return FDLLM_ERR_ARG;
+  if (n_rows == 0) return FDLLM_OK;
+  const void* ptrs[] = {a, w_gate_up, w_scale, out};
+  for (const void* x : ptrs)
+    if (x == nullptr || !aligned16(x)) return FDLLM_ERR_ARG;
+  if (a_scale == nullptr) return FDLLM_ERR_ARG;
+  GemmParams p{};
+  p.out0 = static_cast<__nv_bfloat16*>(out);
+  p.ld_out = ld_out;
+  p.hidden = hidden;
+  p.sa = a_scale;
+  p.sw = w_scale;
+  const void* ws[1] = {w_gate_up};
+  return run_gemm(kEpiSwiglu, a, k_dim / 2, ws, 1, 2 * hidden, n_rows, 2 * hidden, k_dim / 2, p, workspace,
+                  workspace_bytes, stream, true);
 }
 
 int fdllm_gemm_swiglu(const void* a, const void* w_gate_up, void* out, int32_t n_rows, int32_t hidden, int32_t k_dim,

@@ -53,6 +53,10 @@ const char* fdllm_error_string(int code);
  * No reference counterpart (the reference has no error reporting). */
 int fdllm_status_read(int32_t out[4], cudaStream_t stream);
 
+/* The id of the graph capture that `stream` takes part in, 0 outside a capture (CUDA numbers captures
+ * uniquely within a process).  A host that keeps workspaces uses it to give every captured graph its own. */
+int fdllm_stream_capture_id(cudaStream_t stream, uint64_t* id);
+
 /* RMSNorm as the reference's RMSLayerNorm: y = bf16(w * bf16(x * rsqrt(mean(x^2) + eps))),
  * x/w/y bf16, rows x dim.  ref llada/model/modeling_llada.py:389-403 (called as
  * self.attn_norm(x) at llada/flash_cache_triton.py:494). */
@@ -116,6 +120,37 @@ int fdllm_gemm_bf16(const void* a, const void* w, void* out, const void* residua
  * activations stay in TMEM.  ref llada/flash_cache_triton.py:628-633. */
 int fdllm_gemm_swiglu(const void* a, const void* w_gate_up, void* out, int32_t n_rows, int32_t hidden, int32_t k_dim,
                       int64_t ld_out, void* workspace, size_t workspace_bytes, cudaStream_t stream);
+
+/* Rows of bf16 to 8-bit integers with a scale per row: scale[r] = max_j |x[r, j]| / 127 (fp32),
+ * codes[r, j] = rint(x[r, j] * (127 / max)) in [-127, 127] (half to even).  x bf16 with row stride ld
+ * elements, codes int8 [rows, dim] contiguous; dim and ld multiples of 8.  A row whose maximum is below
+ * 2^-120 becomes zeros; a row with an infinity or NaN gets a NaN scale and zero codes.  No reference
+ * counterpart (the reference computes in bf16 only), as for the other entry points of this block. */
+int fdllm_quantize_int8(const void* x, int64_t ld, void* codes, float* scale, int32_t rows, int32_t dim,
+                        cudaStream_t stream);
+
+/* fdllm_rmsnorm followed by fdllm_quantize_int8 in one pass (the same codes and scales); dim a multiple
+ * of 8, at most 16384. */
+int fdllm_rmsnorm_int8(const void* x, const void* weight, void* codes, float* scale, int32_t rows, int32_t dim,
+                       float eps, cudaStream_t stream);
+
+/* 8-bit integer product with a scale per token and per output channel:
+ *   out[r, c] = bf16(float(sum_k a[r, k] * w[c, k]) * a_scale[r] * w_scale[c] (+ residual[r, c]))
+ * a int8 [n_rows, k_dim], w int8 [n_cols, k_dim] (both contiguous), scales fp32, out / residual bf16 with
+ * row strides ld_out / ld_res elements (residual may be NULL).  The sum is an exact 32-bit integer,
+ * rounded to fp32 once.  n_cols a multiple of 8, k_dim a multiple of 16 and at most 131056.  The
+ * stream-K tcgen05 GEMM of fdllm_gemm_bf16 with kind::i8 instructions; workspace as there, its first
+ * 4096 bytes (the flags) zero before first use. */
+size_t fdllm_gemm_int8_workspace_bytes(int32_t n_rows, int32_t n_cols, int32_t k_dim, int32_t swiglu);
+int fdllm_gemm_int8(const void* a, const float* a_scale, const void* w, const float* w_scale, void* out,
+                    const void* residual, int32_t n_rows, int32_t n_cols, int32_t k_dim, int64_t ld_out,
+                    int64_t ld_res, void* workspace, size_t workspace_bytes, cudaStream_t stream);
+
+/* fdllm_gemm_swiglu with 8-bit operands: w_gate_up int8 [2 * hidden, k_dim], w_scale fp32 [2 * hidden]; the
+ * gate and up sums are scaled as in fdllm_gemm_int8 before the rounding points of fdllm_gemm_swiglu. */
+int fdllm_gemm_swiglu_int8(const void* a, const float* a_scale, const void* w_gate_up, const float* w_scale, void* out,
+                           int32_t n_rows, int32_t hidden, int32_t k_dim, int64_t ld_out, void* workspace,
+                           size_t workspace_bytes, cudaStream_t stream);
 
 /* Workspace (bytes) fdllm_qkv_rope_cache / fdllm_verify_qkv need for n_rows query rows. */
 size_t fdllm_qkv_workspace_bytes(int32_t n_rows, int32_t d_model, int32_t n_heads);
@@ -210,6 +245,58 @@ int fdllm_attn_cache(const void* q, void* o, const void* k_cache, const void* v_
                      int32_t seqlen_max, int64_t n_slots, float softmax_scale, int32_t kv_splits,
                      const int32_t* page_table, int32_t pages_per_seq, void* workspace, size_t workspace_bytes,
                      cudaStream_t stream);
+
+/* The 4-bit paged KV cache.  k_cache and v_cache are uint8 [n_pages, n_kv_heads, 4352]: per page (64
+ * tokens) and head 64 x 64 bytes of codes, then 64 x (bf16 step, bf16 low).  A group is the 128 values of
+ * one token and head (bf16): low = min, step = bf16((max - low) / 15), code = clamp(rint((x - low) / step),
+ * 0, 15), value = low + code * step; dim 8 w + 2 i + j of a group is at bits 16 j + 4 i of its 32-bit word w.
+ * A group holding an infinity or NaN reads as NaN.  No reference counterpart (its caches are bf16). */
+
+/* Append tokens to a paged cache, with the position rotation on the way.  Row r is the token of slot
+ * slots[r] = sequence * seqlen_max + position; its page is page_table[sequence * pages_per_seq + position /
+ * 64], line position % 64 (page_table NULL: page slot / 64, seqlen_max a multiple of 64).
+ *   q, k, v   bf16, row strides ldq / ldk / ldv elements (e.g. parts of one stacked projection), n_heads /
+ *             n_kv_heads / n_kv_heads heads of 128
+ *   rope_sin, rope_cos  fp32 [>= seqlen_max, 128] by position, or both NULL: no rotation
+ *   q_out     bf16 [n_rows, n_heads * 128]: the rotated Q (NULL: q is not read); may be q itself
+ *   kv_bits   16: k_cache, v_cache bf16 [n_pages * 64, n_kv_heads * 128];  4: the 4-bit cache above
+ * Rotated K and V go to their token's line; everything else in the caches stays as it was.  A slot or
+ * page out of range is reported as FDLLM_ERR_INDEX and its row left out entirely.  Slots of one call must
+ * be distinct (of two rows with the same slot, either may be kept, value by value).  batch and
+ * pages_per_seq are page_table's sizes.  ref llada/flash_cache_triton.py:78-100 (the rotation and the
+ * cache store, into contiguous bf16 regions). */
+int fdllm_rope_append(const void* q, const void* k, const void* v, int64_t ldq, int64_t ldk, int64_t ldv,
+                      const int64_t* slots, const float* rope_sin, const float* rope_cos, void* q_out, void* k_cache,
+                      void* v_cache, int32_t kv_bits, int32_t n_rows, int32_t n_heads, int32_t n_kv_heads,
+                      int32_t seqlen_max, int64_t n_pages, const int32_t* page_table, int32_t batch,
+                      int32_t pages_per_seq, cudaStream_t stream);
+
+/* Tokens of a 4-bit cache as bf16 rows: k_out, v_out [n_rows, n_kv_heads * 128] = the values (rounded to
+ * bf16) held for slots[r].  A slot or page out of range is reported as FDLLM_ERR_INDEX and reads as 0. */
+int fdllm_read_cache_int4(const void* k_cache, const void* v_cache, const int64_t* slots, void* k_out, void* v_out,
+                          int32_t n_rows, int32_t n_kv_heads, int32_t seqlen_max, int64_t n_pages,
+                          const int32_t* page_table, int32_t batch, int32_t pages_per_seq, cudaStream_t stream);
+
+/* fdllm_attn_cache over the 4-bit cache.  q, o bf16 [n_rows, n_heads * 128]; n_heads a multiple of
+ * n_kv_heads (query head h reads kv head h / (n_heads / n_kv_heads); at most 64 per kv head); plan and
+ * max_items as for fdllm_attn_cache; page_table int32 [batch, pages_per_seq] or NULL (sequence b owns
+ * pages [b * seqlen_max / 64, ...), seqlen_max a multiple of 64); a page outside the cache is reported as
+ * FDLLM_ERR_INDEX and read as page 0.  attn_scores and score_scale as there.
+ *   rows_hint  rows of one sequence the caller expects at most (0: unknown): chooses the kernel and the
+ *              split; results are right whatever it says
+ *   kv_splits  key ranges per item (0: automatic)
+ * The sizes of the workspace (returned) and of the scratch (*scratch_bytes) depend on the arguments as
+ * passed here.  The workspace is zero before first use and every call leaves it zero (zero it again after
+ * a call whose device status reported an error); the scratch may hold anything. */
+size_t fdllm_attn_int4_workspace_bytes(int32_t n_rows, int32_t max_items, int32_t n_heads, int32_t n_kv_heads,
+                                       int32_t seqlen_max, int32_t kv_splits, int32_t rows_hint, int32_t scores,
+                                       size_t* scratch_bytes);
+int fdllm_attn_cache_int4(const void* q, void* o, const void* k_cache, const void* v_cache, const void* plan,
+                          int32_t max_items, float* attn_scores, float score_scale, int32_t n_rows, int32_t n_heads,
+                          int32_t n_kv_heads, int32_t seqlen_max, int64_t n_pages, float softmax_scale,
+                          int32_t kv_splits, int32_t rows_hint, const int32_t* page_table, int32_t batch,
+                          int32_t pages_per_seq, void* workspace, size_t workspace_bytes, void* scratch, size_t scratch_bytes,
+                          cudaStream_t stream);
 
 /* Flash-Verify attention: rows [q_s, q_e) of verify block row b = (k_s, k_e, q_s, q_e) (int32
  * [n_blocks, 4]) attend to cache rows pos_k[k_s:k_e] (gathered) and to their own block's fresh
