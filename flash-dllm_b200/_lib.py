@@ -8,6 +8,8 @@ fallback.  ``call(name, *args)`` invokes an entry point and raises
 from __future__ import annotations
 
 import ctypes as C
+import importlib.machinery
+import importlib.util
 import os
 
 import torch
@@ -91,6 +93,22 @@ def _load():
 
 
 _LIB = _load()
+
+
+def _load_torch_ops():
+    """The torch binding of the quantised operators (csrc/torch_ops.cpp)."""
+    name = "_torch_ops"
+    path = os.path.join(os.path.dirname(LIB_PATH), name + ".so")
+    if not os.path.exists(path):
+        raise ImportError(f"{path} is missing: build it with `python -m flash_dllm_b200.build`")
+    loader = importlib.machinery.ExtensionFileLoader(name, path)
+    mod = importlib.util.module_from_spec(importlib.util.spec_from_loader(name, loader))
+    loader.exec_module(mod)
+    mod.set_error_class(FdllmError)
+    return mod
+
+
+torch_ops = _load_torch_ops()
 
 
 def lib():

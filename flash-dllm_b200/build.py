@@ -5,7 +5,9 @@
 Every ``csrc/*.cu`` is compiled for sm_100a only (``-gencode
 arch=compute_100a,code=sm_100a -lineinfo -O3``) into ``_build/`` at the repo
 root and linked into ``flash-dllm_b200/libflashdllm_b200.so`` next to this
-file.  Objects are rebuilt when a source or header is newer.
+file.  ``csrc/torch_ops.cpp`` (the torch binding of the quantised operators)
+is compiled with g++ against the installed torch and linked to that library
+as ``_torch_ops.so``.  Objects are rebuilt when a source or header is newer.
 """
 from __future__ import annotations
 
@@ -15,6 +17,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -22,6 +25,8 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 BUILD = os.path.join(ROOT, "_build")
 LIB = os.path.join(PKG, "libflashdllm_b200.so")
+BINDING_SRC = os.path.join(CSRC, "torch_ops.cpp")
+BINDING = os.path.join(PKG, "_torch_ops.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr", "-I", INCLUDE,
          "-I", CSRC]
@@ -38,6 +43,18 @@ def _newest_dep() -> float:
     deps = glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(CSRC, "*.h")) + \
         glob.glob(os.path.join(INCLUDE, "*.h"))
     return max(os.path.getmtime(d) for d in deps) if deps else 0.0
+
+
+def _binding_cmd() -> list:
+    from torch.utils import cpp_extension as ext
+    inc = [*ext.include_paths("cuda"), sysconfig.get_paths()["include"], INCLUDE]
+    libs = ext.library_paths("cuda")
+    # (the system's g++: the module has to share torch's libstdc++, which a
+    # compiler that links its own statically would not)
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+            "-DTORCH_EXTENSION_NAME=_torch_ops", *[f"-I{p}" for p in inc], BINDING_SRC, "-o", BINDING,
+            *[f"-L{p}" for p in libs], "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda",
+            f"-L{PKG}", f"-l:{os.path.basename(LIB)}", "-Wl,-rpath,$ORIGIN"]
 
 
 def build(verbose: bool = False, force: bool = False) -> str:
@@ -64,6 +81,8 @@ def build(verbose: bool = False, force: bool = False) -> str:
         list(ex.map(run, jobs))
     if jobs or not os.path.exists(LIB) or any(os.path.getmtime(o) > os.path.getmtime(LIB) for o in objs):
         run([nvcc, *ARCH, "-shared", "-o", LIB, *objs, "-lcudart_static", "-lrt", "-ldl", "-lpthread"])
+    if force or not os.path.exists(BINDING) or os.path.getmtime(BINDING) < max(os.path.getmtime(BINDING_SRC), dep_t):
+        run(_binding_cmd())
     return LIB
 
 

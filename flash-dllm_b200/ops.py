@@ -8,15 +8,13 @@ their counters at zero after every call).
 """
 from __future__ import annotations
 
-import ctypes
 import functools
-import threading
 from typing import Dict, Optional, Tuple
 
 import torch
 
 from . import _lib
-from ._lib import call, ptr
+from ._lib import call, ptr, torch_ops as _T
 
 BF16 = torch.bfloat16
 
@@ -27,9 +25,8 @@ class Workspace:
     Buffers that were outgrown stay allocated (in ``_retired``): a captured
     CUDA graph may still hold their addresses."""
 
-    _bufs: Dict[tuple, torch.Tensor] = {}
+    _bufs: Dict[Tuple[int, str], torch.Tensor] = {}
     _retired: list = []
-    _captured: Dict[tuple, list] = {}
 
     @classmethod
     def get(cls, device: torch.device, nbytes: int, tag: str = "main") -> torch.Tensor:
@@ -47,40 +44,10 @@ class Workspace:
         return buf
 
     @classmethod
-    def on_stream(cls, device: torch.device, stream: int, nbytes: int, tag: str, zero_bytes: int) -> torch.Tensor:
-        """Scratch of the current stream alone, its first ``zero_bytes`` zero.
-        Eager calls keep one buffer per (device, stream, tag).  A captured
-        graph gets its own from its memory pool, cleared by a node of the
-        graph: two graphs that replay at the same time, or a graph and an eager
-        call, never share one, and nothing has to run before the capture."""
-        capture = _capture_id(stream)
-        if capture == 0:
-            key = (device.index, tag, stream)
-            buf = cls._bufs.get(key)
-            if buf is None or buf.numel() < nbytes:
-                size = max(nbytes, 1 << 16)
-                if buf is not None:
-                    size = max(size, int(buf.numel() * 1.5))
-                    cls._retired.append(buf)
-                buf = cls._bufs[key] = torch.zeros(size, dtype=torch.uint8, device=device)
-            return buf
-        key = (device.index, tag, capture)
-        held = cls._captured.get(key)
-        if held is None:
-            while len(cls._captured) >= 32:  # of captures long ended: their memory stays with their graphs' pools
-                cls._captured.pop(next(iter(cls._captured)))
-            held = cls._captured[key] = []
-        if not held or held[-1].numel() < nbytes:
-            buf = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
-            buf[:zero_bytes].zero_()
-            held.append(buf)
-        return held[-1]
-
-    @classmethod
     def clear(cls) -> None:
         cls._bufs.clear()
         cls._retired.clear()
-        cls._captured.clear()
+        _T.workspace_clear()
 
     @classmethod
     def rezero(cls) -> None:
@@ -88,6 +55,7 @@ class Workspace:
         counters or flags set); addresses are kept."""
         for buf in cls._bufs.values():
             buf.zero_()
+        _T.workspace_rezero()
 
 
 _lib.on_device_error(Workspace.rezero)
@@ -239,145 +207,38 @@ def swiglu(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
 
 
 # ------------------------------------------- 8-bit products, 4-bit cache --
+# (arguments are checked, outputs and workspaces made by csrc/torch_ops.cpp)
 
 HEAD_DIM = 128
 PAGE = 64
 INT4_BLOCK = PAGE * HEAD_DIM // 2 + PAGE * 4  # bytes of one page of one head: codes, then (step, low) pairs
-_GEMM_FLAG_BYTES = 4096
-_u64 = ctypes.c_uint64
-_capture_out = threading.local()
 
 
-def _capture_id(stream: int) -> int:
-    """Id of the graph capture ``stream`` takes part in (0: none)."""
-    out = getattr(_capture_out, "id", None)
-    if out is None:
-        out = _capture_out.id = _u64()
-    call("fdllm_stream_capture_id", stream, ctypes.addressof(out))
-    return out.value
-
-
-def _on_device(fn):
-    """Run a wrapper on the device of its first tensor (its current stream
-    there), whatever the current device is."""
-    @functools.wraps(fn)
-    def run(t, *args, **kw):
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
-            raise ValueError(f"{fn.__name__}: the tensors must be CUDA tensors (no CPU path)")
-        if t.device.index == torch._C._cuda_getDevice():
-            return fn(t, *args, **kw)
-        with torch.cuda.device(t.device):
-            return fn(t, *args, **kw)
-    return run
-
-
-def _same_device(t: torch.Tensor, **others) -> None:
-    for name, o in others.items():
-        if o is not None and o.device != t.device:
-            raise ValueError(f"{name} must be on {t.device}, got {o.device}")
-
-
-def _rows_view(t: torch.Tensor, name: str, cols: Optional[int] = None) -> int:
-    """Checks a 2-D bf16 tensor with unit column stride; returns its row stride."""
-    if t.dim() != 2 or t.dtype != BF16 or (cols is not None and t.shape[1] != cols):
-        raise ValueError(f"{name} must be a 2-D bf16 tensor" + (f" of {cols} columns" if cols is not None else "") +
-                         f", got {t.dtype} {tuple(t.shape)}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
-        raise ValueError(f"{name} must have unit column stride")
-    ld = t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
-    if ld < t.shape[1] or ld % 8 or t.data_ptr() % 16:
-        raise ValueError(f"{name}: rows must not overlap and must start on 16-byte boundaries")
-    return ld
-
-
-@_on_device
 def quantize_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """(codes int8, scale fp32 [rows]) of a bf16 [rows, dim]: scale = max|x| / 127
     of the row, codes = round(x / scale) in [-127, 127].  ``x`` may be a
     row-strided view.  A row with an infinity or NaN gets a NaN scale."""
-    ld = _rows_view(x, "x")
-    rows, dim = x.shape
-    codes = torch.empty(rows, dim, dtype=torch.int8, device=x.device)
-    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    call("fdllm_quantize_int8", ptr(x), ld, ptr(codes), ptr(scale), rows, dim, _stream())
-    return codes, scale
+    return _T.quantize_int8(x)
 
 
-@_on_device
 def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float) -> Tuple[torch.Tensor, torch.Tensor]:
     """``quantize_int8(rmsnorm(x, weight, eps))`` in one pass."""
-    _check(x, "x", BF16, 2)
-    _check(weight, "weight", BF16, 1)
-    _same_device(x, weight=weight)
-    rows, dim = x.shape
-    if weight.shape[0] != dim:
-        raise ValueError(f"weight must have {dim} values, got {weight.shape[0]}")
-    codes = torch.empty(rows, dim, dtype=torch.int8, device=x.device)
-    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    call("fdllm_rmsnorm_int8", ptr(x), ptr(weight), ptr(codes), ptr(scale), rows, dim, float(eps), _stream())
-    return codes, scale
+    return _T.rmsnorm_int8(x, weight, eps)
 
 
-def _int8_operands(a, a_scale, w, w_scale) -> Tuple[int, int, int]:
-    _check(a, "a", torch.int8, 2)
-    _check(w, "w", torch.int8, 2)
-    _check(a_scale, "a_scale", torch.float32, 1)
-    _check(w_scale, "w_scale", torch.float32, 1)
-    _same_device(a, a_scale=a_scale, w=w, w_scale=w_scale)
-    (rows, k), n = a.shape, w.shape[0]
-    if w.shape[1] != k:
-        raise ValueError(f"shapes {tuple(a.shape)} x {tuple(w.shape)}^T do not match")
-    if a_scale.shape[0] != rows or w_scale.shape[0] != n:
-        raise ValueError(f"scales must be [{rows}] and [{n}], got {tuple(a_scale.shape)} and {tuple(w_scale.shape)}")
-    return rows, n, k
-
-
-@_on_device
 def linear_int8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
                 residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """bf16((a @ w.T) * a_scale[:, None] * w_scale (+ residual)) of int8 a
     [rows, k] and w [n, k]: an exact integer sum, scaled in fp32, rounded once.
     k a multiple of 16, n of 8.  ``residual`` and ``out`` may be row-strided."""
-    rows, n, k = _int8_operands(a, a_scale, w, w_scale)
-    ld_res = 0
-    if residual is not None:
-        _same_device(a, residual=residual)
-        ld_res = _rows_view(residual, "residual", n)
-        if residual.shape[0] != rows:
-            raise ValueError(f"residual must have {rows} rows")
-    if out is None:
-        out = torch.empty(rows, n, dtype=BF16, device=a.device)
-        ld_out = n
-    else:
-        _same_device(a, out=out)
-        ld_out = _rows_view(out, "out", n)
-        if out.shape[0] != rows:
-            raise ValueError(f"out must have {rows} rows")
-    stream = _stream()
-    ws = Workspace.on_stream(a.device, stream, _int8_workspace(rows, n, k, 0), "int8", _GEMM_FLAG_BYTES)
-    call("fdllm_gemm_int8", ptr(a), ptr(a_scale), ptr(w), ptr(w_scale), ptr(out), ptr(residual), rows, n, k, ld_out,
-         ld_res, ptr(ws), ws.numel(), stream)
-    return out
+    return _T.linear_int8(a, a_scale, w, w_scale, residual, out)
 
 
-@_on_device
 def linear_swiglu_int8(a: torch.Tensor, a_scale: torch.Tensor, w_gate_up: torch.Tensor,
                        w_scale: torch.Tensor) -> torch.Tensor:
     """:func:`linear_swiglu` of 8-bit operands: ``w_gate_up`` int8 [2H, k] with
     ``w_scale`` fp32 [2H]; H a multiple of 128, k of 16."""
-    rows, n, k = _int8_operands(a, a_scale, w_gate_up, w_scale)
-    if n % 2:
-        raise ValueError("w_gate_up must be [2H, K]")
-    out = torch.empty(rows, n // 2, dtype=BF16, device=a.device)
-    stream = _stream()
-    ws = Workspace.on_stream(a.device, stream, _int8_workspace(rows, n, k, 1), "int8", _GEMM_FLAG_BYTES)
-    call("fdllm_gemm_swiglu_int8", ptr(a), ptr(a_scale), ptr(w_gate_up), ptr(w_scale), ptr(out), rows, n // 2, k,
-         n // 2, ptr(ws), ws.numel(), stream)
-    return out
-
-
-def _int8_workspace(rows: int, n: int, k: int, swiglu: int) -> int:
-    return _lib.lib().fdllm_gemm_int8_workspace_bytes(rows, n, k, swiglu)
+    return _T.linear_swiglu_int8(a, a_scale, w_gate_up, w_scale)
 
 
 def int4_cache(n_pages: int, n_kv_heads: int, device="cuda") -> Tuple[torch.Tensor, torch.Tensor]:
@@ -386,33 +247,6 @@ def int4_cache(n_pages: int, n_kv_heads: int, device="cuda") -> Tuple[torch.Tens
     return tuple(torch.zeros(n_pages, n_kv_heads, INT4_BLOCK, dtype=torch.uint8, device=device) for _ in range(2))
 
 
-def _int4_pages(t: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, n_kv_heads: Optional[int]) -> int:
-    _check(k_cache, "k_cache", torch.uint8, 3)
-    _check(v_cache, "v_cache", torch.uint8, 3)
-    _same_device(t, k_cache=k_cache, v_cache=v_cache)
-    hk = k_cache.shape[1] if n_kv_heads is None else n_kv_heads
-    if k_cache.shape != v_cache.shape or tuple(k_cache.shape[1:]) != (hk, INT4_BLOCK):
-        raise ValueError(f"4-bit caches must both be [pages, {hk}, {INT4_BLOCK}], got {tuple(k_cache.shape)} and "
-                         f"{tuple(v_cache.shape)}")
-    return k_cache.shape[0]
-
-
-def _page_table(t: torch.Tensor, page_table: Optional[torch.Tensor], seqlen_max: int) -> Tuple[int, int]:
-    """(batch, pages per sequence) of a page table; (0, 0) without one."""
-    if seqlen_max <= 0:
-        raise ValueError("seqlen_max must be positive")
-    if page_table is None:
-        if seqlen_max % PAGE:
-            raise ValueError(f"without a page table seqlen_max must be a multiple of {PAGE}")
-        return 0, 0
-    _check(page_table, "page_table", torch.int32, 2)
-    _same_device(t, page_table=page_table)
-    if page_table.shape[1] * PAGE < seqlen_max or page_table.shape[0] == 0:
-        raise ValueError(f"page_table must be [batch, at least {-(-seqlen_max // PAGE)}], got {tuple(page_table.shape)}")
-    return page_table.shape[0], page_table.shape[1]
-
-
-@_on_device
 def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, sin: Optional[torch.Tensor],
                 cos: Optional[torch.Tensor], k_cache: torch.Tensor, v_cache: torch.Tensor, n_heads: int,
                 n_kv_heads: int, seqlen_max: int, page_table: Optional[torch.Tensor] = None,
@@ -428,67 +262,15 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.
     pages]: position p of sequence b is line p % 64 of page
     ``page_table[b, p // 64]`` (None: page slot // 64).  Returns the rotated Q
     [rows, n_heads * 128]; ``q_out`` may be ``q`` itself."""
-    rows = slots.shape[0]
-    _check(slots, "slots", torch.int64, 1)
-    _same_device(q, slots=slots, k=k, v=v, sin=sin, cos=cos, q_out=q_out)
-    ldq = _rows_view(q, "q", n_heads * HEAD_DIM)
-    ldk = _rows_view(k, "k", n_kv_heads * HEAD_DIM)
-    ldv = _rows_view(v, "v", n_kv_heads * HEAD_DIM)
-    if q.shape[0] != rows or k.shape[0] != rows or v.shape[0] != rows:
-        raise ValueError(f"q, k and v must have a row per slot ({rows})")
-    batch, pps = _page_table(q, page_table, seqlen_max)
-    if k_cache.dtype == torch.uint8:
-        bits, n_pages = 4, _int4_pages(q, k_cache, v_cache, n_kv_heads)
-    else:
-        bits = 16
-        for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-            _check(t, name, BF16, 2)
-            if t.shape[1] != n_kv_heads * HEAD_DIM or t.shape[0] % PAGE or t.shape != k_cache.shape:
-                raise ValueError(f"{name} must be [pages * {PAGE}, {n_kv_heads * HEAD_DIM}], got {tuple(t.shape)}")
-        _same_device(q, k_cache=k_cache, v_cache=v_cache)
-        n_pages = k_cache.shape[0] // PAGE
-    if (sin is None) != (cos is None):
-        raise ValueError("sin and cos go together")
-    if sin is not None:
-        for t, name in ((sin, "sin"), (cos, "cos")):
-            _check(t, name, torch.float32, 2)
-            if t.shape[1] != HEAD_DIM or t.shape[0] < seqlen_max:
-                raise ValueError(f"{name} must be [at least {seqlen_max}, {HEAD_DIM}], got {tuple(t.shape)}")
-    if q_out is None:
-        q_out = torch.empty(rows, n_heads * HEAD_DIM, dtype=BF16, device=q.device) if sin is not None else None
-    else:
-        _check(q_out, "q_out", BF16, 2)
-        if tuple(q_out.shape) != (rows, n_heads * HEAD_DIM):
-            raise ValueError(f"q_out must be [{rows}, {n_heads * HEAD_DIM}]")
-    call("fdllm_rope_append", ptr(q), ptr(k), ptr(v), ldq, ldk, ldv, ptr(slots), ptr(sin), ptr(cos), ptr(q_out),
-         ptr(k_cache), ptr(v_cache), bits, rows, n_heads, n_kv_heads, seqlen_max, n_pages, ptr(page_table), batch, pps,
-         _stream())
-    return q if q_out is None else q_out
+    return _T.rope_append(q, k, v, slots, sin, cos, k_cache, v_cache, n_heads, n_kv_heads, seqlen_max, page_table, q_out)
 
 
-@_on_device
 def read_cache_int4(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor, seqlen_max: int,
                     page_table: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """The tokens of ``slots`` from a 4-bit cache as bf16 (k, v) [rows, n_kv_heads * 128]."""
-    n_pages = _int4_pages(k_cache, k_cache, v_cache, None)
-    _check(slots, "slots", torch.int64, 1)
-    _same_device(k_cache, slots=slots)
-    batch, pps = _page_table(k_cache, page_table, seqlen_max)
-    rows, hk = slots.shape[0], k_cache.shape[1]
-    k, v = (torch.empty(rows, hk * HEAD_DIM, dtype=BF16, device=k_cache.device) for _ in range(2))
-    call("fdllm_read_cache_int4", ptr(k_cache), ptr(v_cache), ptr(slots), ptr(k), ptr(v), rows, hk, seqlen_max, n_pages,
-         ptr(page_table), batch, pps, _stream())
-    return k, v
+    return _T.read_cache_int4(k_cache, v_cache, slots, seqlen_max, page_table)
 
 
-@functools.lru_cache(maxsize=256)
-def _attn_int4_workspace(device: int, *args) -> Tuple[int, int]:
-    scratch = ctypes.c_size_t()
-    n = _lib.lib().fdllm_attn_int4_workspace_bytes(*args, ctypes.addressof(scratch))
-    return n, scratch.value
-
-
-@_on_device
 def attn_cache_int4(q: torch.Tensor, o: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                     plan: torch.Tensor, capacity: int, attn_scores: Optional[torch.Tensor], score_scale: float,
                     n_heads: int, n_kv_heads: int, seqlen_max: int, softmax_scale: float, kv_splits: int = 0,
@@ -500,33 +282,8 @@ def attn_cache_int4(q: torch.Tensor, o: torch.Tensor, k_cache: torch.Tensor, v_c
     seqlen_max] accumulates ``score_scale`` times the raw q.k sums of the
     masked rows over all heads.  ``rows_hint``: rows of one sequence to expect
     at most (chooses the kernel; 0: unknown)."""
-    for t, name in ((q, "q"), (o, "o")):
-        _check(t, name, BF16, 2)
-    if n_kv_heads <= 0 or n_heads % n_kv_heads:
-        raise ValueError("n_heads must be a multiple of n_kv_heads")
-    if q.shape[1] != n_heads * HEAD_DIM or o.shape != q.shape:
-        raise ValueError(f"q and o must be [rows, {n_heads * HEAD_DIM}], got {tuple(q.shape)} and {tuple(o.shape)}")
-    n_pages = _int4_pages(q, k_cache, v_cache, n_kv_heads)
-    _check(plan, "plan", torch.int32, 1)
-    batch, pps = _page_table(q, page_table, seqlen_max)
-    _same_device(q, o=o, plan=plan, attn_scores=attn_scores)
-    if plan.numel() < 8 + 8 * capacity:
-        raise ValueError("plan is smaller than its capacity")
-    rows = q.shape[0]
-    if attn_scores is not None:
-        _check(attn_scores, "attn_scores", torch.float32)
-        # (the plan's sequences: its capacity minus an item per 64 rows)
-        if attn_scores.numel() < (capacity - (rows + 63) // 64) * seqlen_max:
-            raise ValueError("attn_scores must be [batch * seqlen_max]")
-    nws, nscratch = _attn_int4_workspace(q.device.index, rows, capacity, n_heads, n_kv_heads, seqlen_max, kv_splits,
-                                         rows_hint, int(attn_scores is not None))
-    stream = _stream()
-    ws = Workspace.on_stream(q.device, stream, nws, "attn4", nws) if nws else None
-    scratch = Workspace.on_stream(q.device, stream, nscratch, "attn4s", 0) if nscratch else None
-    call("fdllm_attn_cache_int4", ptr(q), ptr(o), ptr(k_cache), ptr(v_cache), ptr(plan), capacity, ptr(attn_scores),
-         float(score_scale), rows, n_heads, n_kv_heads, seqlen_max, n_pages, float(softmax_scale), kv_splits, rows_hint,
-         ptr(page_table), batch, pps, ptr(ws), ws.numel() if nws else 0, ptr(scratch), scratch.numel() if nscratch else 0,
-         stream)
+    _T.attn_cache_int4(q, o, k_cache, v_cache, plan, capacity, attn_scores, score_scale, n_heads, n_kv_heads, seqlen_max,
+                       softmax_scale, kv_splits, rows_hint, page_table)
 
 
 def _qkv(entry: str, xn, wq, wk, wv, pos, sin, cos, q_out, k_out, v_out, n_heads: int) -> None:
