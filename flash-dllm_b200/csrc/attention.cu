@@ -43,10 +43,11 @@ constexpr int kTileBytes = 2 * kHalfBytes;          // one K or V tile (128 dims
 //             [4] tracked row start, [5] tracked rows, [6] masked-item number
 //             (-1: no masked rows), [7] 0
 //   sequence: [0] number of its first masked item, [1] its masked items
-//             (consecutive), [2] k_end (0: no rows)
+//             (consecutive), [2] k_end (0: no rows), [3] masked row start,
+//             [4] masked rows, [5] tracked row start, [6] tracked rows, [7] 0
 constexpr int kPlanHeader = 8;
 constexpr int kPlanItem = 8;
-constexpr int kPlanSeq = 3;
+constexpr int kPlanSeq = 8;
 constexpr int kAttnKernelId = 2;
 constexpr int kPlanKernelId = 3;
 
@@ -1055,6 +1056,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int64_t* __res
     e[0] = live ? moff[b] : 0;
     e[1] = live ? (m_len[b] + kItemRows - 1) / kItemRows : 0;
     e[2] = live ? k_end[b] : 0;
+    e[3] = m_start[b];
+    e[4] = live ? m_len[b] : 0;
+    e[5] = t_len[b] > 0 ? t_min[b] : 0;
+    e[6] = live ? t_len[b] : 0;
+    e[7] = 0;
   }
   if (bad != 0) return;
   for (int b = tid; b < batch; b += kPlanThreads) {

@@ -15,7 +15,10 @@
 #include "int4.cuh"
 #include "internal.h"
 
+#include <cuda_fp16.h>
+
 #include <algorithm>
+#include <cstddef>
 
 namespace fdllm {
 
@@ -24,7 +27,7 @@ constexpr int kA4HeadDim = 128;
 // the plan's layout (attention.cu)
 constexpr int kA4PlanHeader = 8;
 constexpr int kA4PlanItem = 8;
-constexpr int kA4PlanSeq = 3;
+constexpr int kA4PlanSeq = 8;
 constexpr int kA4ItemRows = 64;
 
 struct A4Params {
@@ -100,10 +103,10 @@ __device__ __forceinline__ void a4_add_score(unsigned long long* acc, float x, b
 
 // The sequence's column sums are complete: add them to attn_scores once and
 // leave the accumulator zeroed for the next call.
-__device__ __forceinline__ void a4_convert_scores(const A4Params& p, int seq, int k_end) {
+__device__ __forceinline__ void a4_convert_scores(const A4Params& p, int seq, int k_end, int threads) {
   unsigned long long* acc = p.score_acc + static_cast<int64_t>(seq) * p.seqlen_max;
   float* dst = p.scores + static_cast<int64_t>(seq) * p.seqlen_max;
-  for (int n = threadIdx.x; n < k_end; n += blockDim.x) {
+  for (int n = threadIdx.x; n < k_end; n += threads) {
     const long long v = __ldcg(reinterpret_cast<const long long*>(acc + n));
     __stcg(reinterpret_cast<long long*>(acc + n), 0ll);
     dst[n] += static_cast<float>(static_cast<double>(v) * 2.3283064365386963e-10 * static_cast<double>(p.score_scale));
@@ -487,13 +490,771 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_int4_few_kernel(const A4P
       }
     }
     __syncthreads();
-    if (s_convert >= 0) a4_convert_scores(p, it.seq, min(it.k_end, p.seqlen_max));
+    if (s_convert >= 0) a4_convert_scores(p, it.seq, min(it.k_end, p.seqlen_max), kFewThreads);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: tcgen05, 128 query rows x 128 keys a tile.
+//
+// The second form of the products, for the tensor cores.  A tile row is one
+// (query row, head of the group); rows of a sequence are taken in order, its
+// masked rows first, 128 to a CTA (120 and three rows for the importance
+// scores when those are wanted).  Both operands are fp16, normalised by powers
+// of two so that no cache or query can leave its range: a query row by its
+// largest value (2^-e_m), K and V by the largest value of each 32-key piece of
+// a tile (2^-ek, 2^-ev).  With 11 bits, fp16 holds (code - 8) * step exactly
+// (3 bits by 8), so
+//   K operand   (code - 8) * step * 2^-ek for 128 dims, and 16 more columns in
+//               which base_n * sum_d q_d is formed from two fp16 halves of the
+//               base and three of the sum (22 bits): the S tile is the whole
+//               logit, and a softmax thread needs no per-key constant;
+//   V operand   fp16((code - 8) * step + base): half an ulp is 2^-12 of the
+//               value, an eighth of what bf16 keys and values themselves carry;
+//   P operand   2^(logit + ev - R) in fp16 (2^-12, against bf16's 2^-9): the
+//               running reference R follows the largest logit + ev, that is
+//               the largest contribution to O, so what fp16 drops (2^-30 of
+//               it and less) is small against the result itself, whatever
+//               the sizes of single keys and values.  The sum takes
+//               2^(logit - R), so the quotient needs no other scale.
+// The scores use the rows sum_masked q split into three fp16 parts, so their
+// column sums carry 22 bits and more.
+//
+// P goes from the registers to tensor memory and is the second product's A
+// operand there: the kernel's tightest resource is shared memory (per tile 72
+// KB of operands for S, 32 for P V, 72 written by the conversion, 34 of codes
+// in and out = 210 KB, 1640 clocks at 128 bytes a clock, against 1000 for the
+// tensor cores' 17 instructions of about 60 clocks, 1024 for the exponentials
+// at 16 a clock and about 900 issue slots of each scheduler).
+//
+// Warps (16): 0-3 and 4-7 softmax of the even and the odd key tiles (thread =
+// tile row, with its own running maximum, sum and O accumulator: the two
+// halves never wait on each other and are joined at the end), 8-11 conversion
+// (each a 32-key piece of every tile), 12 bulk copies of pages, 13 the MMA
+// thread.  Tensor memory: S (and P over it) of the two halves, O of the two.
+// Key ranges are split over CTAs as in the other kernel.
+// ---------------------------------------------------------------------------
+constexpr int kMnThreads = 512;
+constexpr int kMnKeys = 128;
+constexpr int kMnRows = 128;
+constexpr int kMnScoreRows = 120;  // with scores: rows 120, 121, 122 carry the masked rows' sum
+constexpr int kMnRing = 4;         // pages
+constexpr int kMnHalf = 128 * 128;             // 128 rows x 64 dims (128-byte swizzle)
+constexpr int kMnExt = 128 * 32;               // 128 rows x 16 columns (32-byte swizzle)
+constexpr int kMnQ = 0;                        // two halves, then the 16 columns
+constexpr int kMnQx = kMnQ + 2 * kMnHalf;
+constexpr int kMnK = kMnQx + kMnExt;           // 2 stages of two halves; each 16 columns after both
+constexpr int kMnV = kMnK + 4 * kMnHalf;
+constexpr int kMnKx = kMnV + 4 * kMnHalf;
+constexpr int kMnRaw = kMnKx + 2 * kMnExt;
+constexpr int kMnMisc = kMnRaw + kMnRing * kFewStageBytes;
+constexpr int kMnMiscBytes = 7 * 1024;
+constexpr int kMnSmem = 1024 + kMnMisc + kMnMiscBytes;
+static_assert(kMnK % 1024 == 0 && kMnV % 1024 == 0 && kMnKx % 1024 == 0 && kMnRaw % 128 == 0, "operand alignment");
+static_assert(kMnSmem <= 227 * 1024, "shared memory");
+constexpr int kMnRegsSoft = 184, kMnRegsConv = 88, kMnRegsMisc = 40;
+static_assert(256 * kMnRegsSoft + 128 * kMnRegsConv + 128 * kMnRegsMisc <= kMnThreads * 128, "setmaxnreg split");
+constexpr float kMnLazy = 8.f;   // log2 units a contribution may pass the reference by before it moves
+constexpr float kMnRaise = 6.f;  // P is raised by 2^6: with the 8 above, below fp16's 2^16
+constexpr int kMnPartFloats = kMnRows * kA4HeadDim + 2 * kMnRows;
+
+// 2^e for |e| <= 126
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((127 + e) << 23); }
+// exponent of a magnitude, held to what pow2i takes (0 and denormals: the least)
+__device__ __forceinline__ int exponent_of(float mag) {
+  const int e = static_cast<int>((__float_as_uint(mag) >> 23) & 255u) - 127;
+  return max(-100, min(e, 126));
+}
+
+// fp16 operands (kind::f16, fp32 accumulate); the A operand in shared or in tensor memory
+__host__ __device__ constexpr uint32_t umma_idesc_f16(int M, int N) {
+  return (1u << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// K-major operand of 16 columns (32-byte rows, 32-byte swizzle: layout type
+// 6; 8-row groups of 256 bytes)
+__device__ __forceinline__ uint64_t umma_desc_kmajor_sw32(uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(1u) << 16;
+  d |= static_cast<uint64_t>(256u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(6u) << 61;
+  return d;
+}
+__device__ __forceinline__ uint8_t* ext_chunk(uint8_t* base, int row, int chunk) {
+  return base + row * 32 + ((chunk ^ ((row >> 2) & 1)) << 4);
+}
+
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// code - 8 of the pairs at bits 0 (even) or 4 (odd) of each half: 1024 + code
+// and 1024 + 16 code are fp16 values whose mantissas hold the code
+__device__ __forceinline__ __half2 i4_even_f16(uint32_t w) {
+  uint32_t m;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(m) : "r"(w), "n"(0x000f000f), "r"(0x64006400u));
+  return __hsub2(*reinterpret_cast<const __half2*>(&m), __float2half2_rn(1032.f));
+}
+__device__ __forceinline__ __half2 i4_odd_f16(uint32_t w) {
+  uint32_t m;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(m) : "r"(w), "n"(0x00f000f0), "r"(0x64006400u));
+  return __hfma2(*reinterpret_cast<const __half2*>(&m), __float2half2_rn(0.0625f), __float2half2_rn(-72.f));
+}
+
+// the parameters of a lane's key, normalised over the warp's 32 keys
+struct MnParams {
+  __half2 step;      // twice
+  float base;        // normalised, fp32
+  int e;             // exponent of the piece
+};
+__device__ __forceinline__ MnParams mn_params(const uint8_t* block, int line, bool valid) {
+  MnParams r;
+  const uint32_t pr = valid ? reinterpret_cast<const uint32_t*>(block + kI4Codes)[line] : 0u;
+  const float step = __uint_as_float(pr << 16), low = __uint_as_float(pr & 0xffff0000u);
+  const float mag = fmaxf(fabsf(low), fabsf(fmaf(15.f, step, low)));
+  // (a NaN group says nothing about the others' size)
+  r.e = __reduce_max_sync(0xffffffffu, mag <= 3.4e38f ? exponent_of(mag) : -100);
+  const float s = pow2i(-r.e);
+  r.step = __float2half2_rn(step * s);
+  r.base = fmaf(8.f, step, low) * s;
+  return r;
+}
+
+// The warp's 32 keys of a K or V block into a tile (rows row0 ..): lane ->
+// key 8 i + lane / 4, 16 bytes of codes = 32 dims, four 16-byte chunks out.
+// The words of the lanes of dims 64 .. 127 are taken in another order, so that
+// a quarter-warp's stores fall into different banks.
+template <bool IS_V>
+__device__ __forceinline__ void mn_convert(const uint8_t* block, int line0, bool has, uint8_t* tile, int row0, int lane,
+                                           const MnParams& pm) {
+  const int q = lane & 3;
+  const bool upper = (q >> 1) != 0;
+  uint4 w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = has ? *reinterpret_cast<const uint4*>(block + (line0 + 8 * i + (lane >> 2)) * kI4Row + 16 * q)
+               : make_uint4(0, 0, 0, 0);
+  const uint32_t step_bits = *reinterpret_cast<const uint32_t*>(&pm.step);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int key = 8 * i + (lane >> 2);
+    const uint32_t sb = __shfl_sync(0xffffffffu, step_bits, key);
+    const __half2 step = *reinterpret_cast<const __half2*>(&sb);
+    __half2 base = step;
+    if (IS_V) base = __float2half2_rn(__shfl_sync(0xffffffffu, pm.base, key));
+    const int r = row0 + key;
+    uint8_t* row = tile + (q >> 1) * kMnHalf + r * 128;
+    const uint32_t v[4] = {upper ? w[i].z : w[i].x, upper ? w[i].w : w[i].y, upper ? w[i].x : w[i].z,
+                           upper ? w[i].y : w[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = (q & 1) * 4 + (j ^ (upper ? 2 : 0));
+      const uint32_t hi = v[j] >> 8;
+      __half2 o[4] = {i4_even_f16(v[j]), i4_odd_f16(v[j]), i4_even_f16(hi), i4_odd_f16(hi)};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] = IS_V ? __hfma2(o[k], step, base) : __hmul2(o[k], step);
+      *reinterpret_cast<uint4*>(row + ((c ^ (r & 7)) << 4)) = *reinterpret_cast<const uint4*>(o);
+    }
+  }
+}
+
+// a sequence's rows, from the plan's per-sequence section
+struct MnSeq {
+  int k_end, m_start, m_len, t_start, rows;
+};
+__device__ __forceinline__ bool mn_load_seq(const A4Params& p, int seq, MnSeq& s) {
+  if (p.plan[0] <= 0 || seq >= p.plan[1]) return false;
+  const int4* e = reinterpret_cast<const int4*>(p.plan + p.plan[3] + seq * kA4PlanSeq);
+  const int4 e0 = e[0], e1 = e[1];
+  s.k_end = e0.z;
+  s.m_start = e0.w;
+  s.m_len = e1.x;
+  s.t_start = e1.y;
+  s.rows = e1.x + e1.z;
+  if (s.rows <= 0) return false;
+  if (seq >= p.batch || s.k_end <= 0 || s.k_end > p.seqlen_max || s.m_start < 0 || s.t_start < 0 ||
+      s.m_start + s.m_len > p.n_rows || s.t_start + e1.z > p.n_rows) {
+    if (threadIdx.x == 0) report(p.status, FDLLM_ERR_TABLE, seq, kA4KernelId);
+    return false;
+  }
+  return true;
+}
+// element offset of tile row m (query row m / group, head m % group of the kv head)
+__device__ __forceinline__ int64_t mn_row(const A4Params& p, const MnSeq& s, int kvh, int m) {
+  const int r = m / p.group;
+  const int row = r < s.m_len ? s.m_start + r : s.t_start + (r - s.m_len);
+  return (static_cast<int64_t>(row) * p.n_heads + kvh * p.group + m % p.group) * kA4HeadDim;
+}
+
+struct MnMisc {
+  uint64_t raw_full[kMnRing], raw_empty[kMnRing];
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2], mma_done;
+  uint32_t tmem;
+  int32_t last, convert;
+  alignas(16) int32_t ek[4][4];     // [tile % 4][32-key piece]
+  alignas(16) int32_t ev[4][4];
+  float red[4][8];                  // score rows: warp partials
+  float q_amax[2][kMnRows], q_sum[2][kMnRows];
+  float score_scale[4];             // scale of the score rows
+  alignas(16) float score[2][3][kMnKeys];
+  float2 ml[kMnRows];               // the odd half's (m, l)
+};
+static_assert(sizeof(MnMisc) <= kMnMiscBytes, "misc");
+static_assert(offsetof(MnMisc, tmem) == (2 * kMnRing + 15) * 8, "the barriers lie in a row");
+
+// What one row tile of a CTA takes: every role computes the same.
+struct MnTile {
+  int first, n_pages, n_splits, n_kt, m0, rows;
+  bool with_scores;
+};
+__device__ __forceinline__ bool mn_tile(const A4Params& p, const MnSeq& sq, int tile, MnTile& c) {
+  const int split = blockIdx.z;
+  const int seq_pages = (sq.k_end + kI4Page - 1) / kI4Page;
+  // a sequence of more rows than the caller's hint: its further tiles take
+  // the whole key range in the first split's CTA
+  const bool extra = tile >= p.chunks;
+  if (extra && split != 0) return false;
+  const int tile_rows = p.scores != nullptr ? kMnScoreRows : kMnRows;
+  c.first = extra ? 0 : split * p.split_pages;
+  c.n_pages = extra ? seq_pages : min(p.split_pages, seq_pages - c.first);
+  c.n_splits = extra ? 1 : (seq_pages + p.split_pages - 1) / p.split_pages;
+  c.n_kt = (c.n_pages + 1) / 2;
+  c.m0 = tile * tile_rows;
+  c.rows = min(tile_rows, sq.rows * p.group - c.m0);
+  c.with_scores = p.scores != nullptr && sq.m_len > 0 && tile == 0;
+  return true;
+}
+
+__global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  MnMisc& ms = *reinterpret_cast<MnMisc*>(smem + kMnMisc);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int seq = blockIdx.x / p.chunks, tile0 = blockIdx.x % p.chunks;
+  const int kvh = blockIdx.y;
+  const int split = blockIdx.z;
+  MnSeq sq{};
+  if (!mn_load_seq(p, seq, sq)) return;
+  const int tile_rows = p.scores != nullptr ? kMnScoreRows : kMnRows;
+  const int n_tiles = (sq.rows * p.group + tile_rows - 1) / tile_rows;
+  if (split * p.split_pages * kI4Page >= sq.k_end || tile0 >= n_tiles) return;
+
+  if (warp == 12) tmem_alloc(&ms.tmem, 512);
+  // Every role runs its own loop over the CTA's row tiles (one, unless the
+  // hint was low) with two CTA barriers a tile: operands and barriers in place
+  // / everyone done.
+  if (warp < 8) {
+    // ------------------------------------------------------- softmax ----
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMnRegsSoft));
+    const int h = warp >> 2, r = threadIdx.x & 127;
+    MnTile c;
+    for (int tile = tile0; tile < n_tiles && mn_tile(p, sq, tile, c); tile += p.chunks) {
+      const int first = c.first, n_splits = c.n_splits, n_kt = c.n_kt, m0 = c.m0, rows = c.rows;
+      const bool with_scores = c.with_scores;
+      if (threadIdx.x == 0) {
+        for (int s = 0; s < kMnRing; ++s) {
+          mbar_init(&ms.raw_full[s], 1);
+          mbar_init(&ms.raw_empty[s], 2);  // two conversion warps a page
+        }
+        for (int s = 0; s < 2; ++s) {
+          mbar_init(&ms.k_full[s], 4);
+          mbar_init(&ms.k_empty[s], 1);
+          mbar_init(&ms.v_full[s], 4);
+          mbar_init(&ms.v_empty[s], 1);
+          mbar_init(&ms.s_full[s], 1);
+          mbar_init(&ms.p_full[s], 4);
+          mbar_init(&ms.pv_done[s], 1);
+        }
+        mbar_init(&ms.mma_done, 1);
+        fence_barrier_init();
+      }
+      // ---- the query operand ----
+      float row_mul;  // 2^e of the row
+      const bool fill = !(with_scores && r >= kMnScoreRows);  // rows the conversion warps fill instead
+      uint4 v[8];
+      const uint4* src = reinterpret_cast<const uint4*>(p.q + mn_row(p, sq, kvh, m0 + min(r, rows - 1)) + 64 * h);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) v[c] = r < rows ? src[c] : make_uint4(0, 0, 0, 0);
+      uint32_t mag = 0;
+      float sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          mag = __vmaxu2(mag, w[k] & 0x7fff7fffu);
+          const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]));
+          sum += f.x + f.y;
+        }
+      }
+      mag = max(mag & 0xffffu, mag >> 16);
+      ms.q_amax[h][r] = __uint_as_float(mag << 16);
+      ms.q_sum[h][r] = sum;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      // (patterns order as magnitudes: an infinity or NaN keeps e = 126 and stays what it is)
+      const uint32_t both = max(__float_as_uint(ms.q_amax[0][r]), __float_as_uint(ms.q_amax[1][r]));
+      const int e = exponent_of(__uint_as_float(both));
+      const float s = pow2i(-e);
+      row_mul = pow2i(e);
+      if (fill) {
+        uint8_t* row = smem + kMnQ + h * kMnHalf + r * 128;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+          uint32_t o[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]));
+            o[k] = pack_f16x2(f.x * s, f.y * s);
+          }
+          *reinterpret_cast<uint4*>(row + ((c ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+        if (h == 0) {
+          const float qs = (ms.q_sum[0][r] + ms.q_sum[1][r]) * s;
+          const float qh = __half2float(__float2half_rn(qs)), qm = __half2float(__float2half_rn(qs - qh));
+          const uint32_t a = pack_f16x2(qh, qm);
+          *reinterpret_cast<uint4*>(ext_chunk(smem + kMnQx, r, 0)) = make_uint4(a, a, pack_f16x2(qs - qh - qm, 0.f), 0);
+          *reinterpret_cast<uint4*>(ext_chunk(smem + kMnQx, r, 1)) = make_uint4(0, 0, 0, 0);
+        }
+      }
+      fence_proxy_async_smem();
+      tc_fence_before();
+      __syncthreads();
+      tc_fence_after();
+      const uint32_t tmem = ms.tmem;
+      const uint32_t tl = static_cast<uint32_t>((warp & 3) * 32) << 16;
+      const uint32_t ts = tmem + 128 * h + tl, to = tmem + 256 + 128 * h + tl;
+      if (with_scores && r >= kMnScoreRows) row_mul = ms.score_scale[0];
+      const bool score_warp = with_scores && (warp & 3) == 3;
+      const float log_mul = with_scores && r >= kMnScoreRows ? 0.f : row_mul * p.scale_log2;
+      float m_used = -INFINITY, l = 0.f;  // the reference R, and the sum of 2^(logit - R + kMnRaise)
+      bool ok = true, range_ok = true;
+      for (int t = h; t < n_kt; t += 2) {
+        ok = mbar_wait(&ms.s_full[h], (t >> 1) & 1, p.status, kA4KernelId);
+        if (!ok) break;
+        tc_fence_after();
+        float sv[4][32];
+        tmem_ld2_32x32b_x32(ts, ts + 32, sv[0], sv[1]);
+        tmem_ld2_32x32b_x32(ts + 64, ts + 96, sv[2], sv[3]);
+        const int4 ek4 = *reinterpret_cast<const int4*>(ms.ek[t & 3]);
+        const int4 ev4 = *reinterpret_cast<const int4*>(ms.ev[t & 3]);
+        const int ek[4] = {ek4.x, ek4.y, ek4.z, ek4.w}, ev[4] = {ev4.x, ev4.y, ev4.z, ev4.w};
+        const int n0 = first * kI4Page + t * kMnKeys;
+        const int n_valid = sq.k_end - n0;
+        if (score_warp) {
+          // lanes 24 .. 26 hold the three parts' logits of all keys
+          if (lane >= 24 && lane < 27) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const float k = row_mul * pow2i(ek[g]);
+#pragma unroll
+              for (int j = 0; j < 32; j += 4)
+                *reinterpret_cast<float4*>(&ms.score[h][lane - 24][32 * g + j]) =
+                    make_float4(sv[g][j] * k, sv[g][j + 1] * k, sv[g][j + 2] * k, sv[g][j + 3] * k);
+            }
+          }
+          __syncwarp();
+          unsigned long long* acc = p.score_acc + static_cast<int64_t>(seq) * p.seqlen_max + n0;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int n = 32 * g + lane;
+            if (n < n_valid) a4_add_score(acc + n, ms.score[h][0][n] + ms.score[h][1][n] + ms.score[h][2][n], range_ok);
+          }
+          __syncwarp();
+        }
+        if (n_valid < kMnKeys) {  // uniform
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) sv[g][j] = 32 * g + j < n_valid ? sv[g][j] : -INFINITY;
+        }
+        // logits in log2 units are sv * mul; mt = max (logit + ev)
+        float mul[4], mt = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          mul[g] = log_mul * pow2i(ek[g]);
+          float a[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) a[i] = sv[g][i];
+#pragma unroll
+          for (int j = 4; j < 32; ++j) a[j & 3] = fmaxf(a[j & 3], sv[g][j]);
+          mt = fmaxf(mt, fmaf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])), mul[g], static_cast<float>(ev[g])));
+        }
+        const bool need = mt > m_used + kMnLazy;
+        if (__any_sync(0xffffffffu, need)) {
+          const float a = need ? ex2_approx(m_used - mt) : 1.f;
+          if (t >= 2) {
+            // O holds this half's P V so far (done: S of this tile was issued after it)
+#pragma unroll 1
+            for (int c = 0; c < kA4HeadDim / 32; ++c) {
+              float ov[32];
+              tmem_ld_32x32b_x32(to + 32 * c, ov);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) ov[j] *= a;
+              tmem_st_32x32b_x32(to + 32 * c, ov);
+            }
+          }
+          l *= a;
+          if (need) m_used = mt;
+        }
+        const float ref = m_used == -INFINITY ? 0.f : m_used;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float shift = kMnRaise + static_cast<float>(ev[g]) - ref;
+          float ps[4] = {0.f, 0.f, 0.f, 0.f};
+          float pw[16];
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const float x = ex2_approx(fmaf(sv[g][j], mul[g], shift));
+            const float y = ex2_approx(fmaf(sv[g][j + 1], mul[g], shift));
+            ps[j & 3] += x;
+            ps[(j + 1) & 3] += y;
+            pw[j >> 1] = __uint_as_float(pack_f16x2(x, y));
+          }
+          l = fmaf((ps[0] + ps[1]) + (ps[2] + ps[3]), pow2i(-ev[g]), l);
+          tmem_st_32x32b_x16(ts + 16 * g, pw);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ms.p_full[h]);
+      }
+      if (score_warp && !__all_sync(0xffffffffu, range_ok) && lane == 0)
+        report(p.status, FDLLM_ERR_RANGE, seq, kA4KernelId);
+      // ---- join the two halves; this half's last product ----
+      const int mine = (n_kt - h + 1) / 2;  // tiles of this half
+      const bool have = ok && mine > 0 && mbar_wait(&ms.pv_done[h], (mine - 1) & 1, p.status, kA4KernelId);
+      if (have) tc_fence_after();
+      // the odd half's O rows through the K stages (its tiles' MMAs and, by
+      // the other half's wait below, all others are done): 16-byte units
+      // XOR-swizzled by row
+      float* stage = reinterpret_cast<float*>(smem + kMnK);
+      const bool two = n_kt > 1;
+      float m_o = m_used, l_o = have ? l : 0.f;
+      float f_mine = 1.f, f_other = 0.f;
+      if (h == 1 && two) {
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // both halves' products are done
+#pragma unroll 1
+        for (int c = 0; c < kA4HeadDim / 32; ++c) {
+          float ov[32];
+          tmem_ld_32x32b_x32(to + 32 * c, ov);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<float4*>(stage + r * kA4HeadDim + (((8 * c + j) ^ (r & 7)) << 2)) =
+                make_float4(ov[4 * j], ov[4 * j + 1], ov[4 * j + 2], ov[4 * j + 3]);
+        }
+        ms.ml[r] = make_float2(m_used, l_o);
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+      }
+      if (h == 0) {
+        if (two) {
+          asm volatile("bar.sync 1, 256;" ::: "memory");
+          asm volatile("bar.sync 1, 256;" ::: "memory");
+          const float2 o = ms.ml[r];
+          m_o = fmaxf(m_used, o.x);
+          const float ref = m_o == -INFINITY ? 0.f : m_o;
+          const float a = ex2_approx(m_used - ref), b = ex2_approx(o.x - ref);
+          l_o = a * l_o + b * o.y;
+          f_mine *= a;
+          f_other = b;
+        }
+        const bool direct = n_splits == 1;
+        const float inv = direct ? (l_o > 0.f ? 1.f / l_o : (l_o == 0.f ? 0.f : l_o)) : 1.f;
+        f_mine *= inv;
+        f_other *= inv;
+        __nv_bfloat16* dst = p.o + mn_row(p, sq, kvh, m0 + min(r, rows - 1));
+        const int64_t cell = (static_cast<int64_t>(seq) * p.n_kv + kvh) * p.chunks + tile;
+        float* part = direct ? nullptr : p.part + (cell * p.splits + split) * kMnPartFloats;
+#pragma unroll 1
+        for (int c = 0; c < kA4HeadDim / 32; ++c) {
+          float ov[32];
+          tmem_ld_32x32b_x32(to + 32 * c, ov);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (two) x = *reinterpret_cast<const float4*>(stage + r * kA4HeadDim + (((8 * c + j) ^ (r & 7)) << 2));
+            ov[4 * j] = fmaf(ov[4 * j], f_mine, x.x * f_other);
+            ov[4 * j + 1] = fmaf(ov[4 * j + 1], f_mine, x.y * f_other);
+            ov[4 * j + 2] = fmaf(ov[4 * j + 2], f_mine, x.z * f_other);
+            ov[4 * j + 3] = fmaf(ov[4 * j + 3], f_mine, x.w * f_other);
+          }
+          if (r >= rows) continue;
+          if (direct) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 8)
+              *reinterpret_cast<uint4*>(dst + 32 * c + j) =
+                  make_uint4(pack_bf16x2(ov[j], ov[j + 1]), pack_bf16x2(ov[j + 2], ov[j + 3]),
+                             pack_bf16x2(ov[j + 4], ov[j + 5]), pack_bf16x2(ov[j + 6], ov[j + 7]));
+          } else {
+            // [dim / 4][row][4]: a warp's stores are 512 contiguous bytes
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              __stcg(reinterpret_cast<float4*>(part) + (8 * c + j) * kMnRows + r,
+                     make_float4(ov[4 * j], ov[4 * j + 1], ov[4 * j + 2], ov[4 * j + 3]));
+          }
+        }
+        if (!direct && r < rows) {
+          __stcg(part + kMnRows * kA4HeadDim + r, m_o);
+          __stcg(part + kMnRows * kA4HeadDim + kMnRows + r, l_o);
+        }
+      }
+      // every role is done with this tile: its barriers and buffers are free
+      __threadfence();
+      tc_fence_before();
+      __syncthreads();
+      tc_fence_after();
+      if (threadIdx.x == 0) {
+        uint64_t* b = ms.raw_full;  // every barrier, in a row
+        for (int i = 0; i < 2 * kMnRing + 15; ++i) mbar_inval(b + i);
+      }
+      if (n_splits > 1) {
+        const int64_t cell = (static_cast<int64_t>(seq) * p.n_kv + kvh) * p.chunks + tile;
+        if (threadIdx.x == 0) {
+          ms.last = atomicAdd(p.part_cnt + cell, 1) == n_splits - 1;
+          if (ms.last) p.part_cnt[cell] = 0;
+          __threadfence();
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (ms.last) {
+          // thread -> (row, 4 dims) units; splits joined in order
+          const float* all = p.part + cell * p.splits * kMnPartFloats;
+          const int r = threadIdx.x & 127;
+          if (r < rows) {
+            float M = -INFINITY;
+            for (int k = 0; k < n_splits; ++k) M = fmaxf(M, __ldcg(all + k * kMnPartFloats + kMnRows * kA4HeadDim + r));
+            const float ref = M == -INFINITY ? 0.f : M;
+            float L = 0.f;
+            for (int k = 0; k < n_splits; ++k) {
+              const float* ml = all + k * kMnPartFloats + kMnRows * kA4HeadDim;
+              L = fmaf(ex2_approx(__ldcg(ml + r) - ref), __ldcg(ml + kMnRows + r), L);
+            }
+            const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+            __nv_bfloat16* dst = p.o + mn_row(p, sq, kvh, m0 + r);
+#pragma unroll 1
+            for (int u = (threadIdx.x >> 7); u < kA4HeadDim / 4; u += 2) {
+              float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+              for (int k = 0; k < n_splits; ++k) {
+                const float f = ex2_approx(__ldcg(all + k * kMnPartFloats + kMnRows * kA4HeadDim + r) - ref);
+                const float4 x = __ldcg(reinterpret_cast<const float4*>(all + k * kMnPartFloats) + u * kMnRows + r);
+                o.x = fmaf(f, x.x, o.x);
+                o.y = fmaf(f, x.y, o.y);
+                o.z = fmaf(f, x.z, o.z);
+                o.w = fmaf(f, x.w, o.w);
+              }
+              *reinterpret_cast<uint2*>(dst + 4 * u) =
+                  make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+            }
+          }
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+      }
+    }
+    if (p.scores != nullptr && sq.m_len > 0 && tile0 == 0) {
+      if (threadIdx.x == 0) {
+        const int splits = (sq.k_end + p.split_pages * kI4Page - 1) / (p.split_pages * kI4Page);
+        const bool done = atomicAdd(p.score_cnt + seq, 1) == p.n_kv * splits - 1;
+        if (done) p.score_cnt[seq] = 0;
+        __threadfence();
+        ms.convert = done;
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (ms.convert) a4_convert_scores(p, seq, min(sq.k_end, p.seqlen_max), 256);
+    }
+  } else if (warp < 12) {
+    // ---------------------------------------------------- conversion ----
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMnRegsConv));
+    MnTile c;
+    for (int tile = tile0; tile < n_tiles && mn_tile(p, sq, tile, c); tile += p.chunks) {
+      const int first = c.first, n_pages = c.n_pages, n_kt = c.n_kt;
+      if (c.with_scores) {
+        // rows 120 .. 122: the sum of the masked rows over rows and heads, in
+        // three fp16 parts; rows 123 .. 127 zero.  Thread = dim.
+        const int d = threadIdx.x - 256;
+        float acc = 0.f;
+        const int n = sq.m_len * p.group;
+#pragma unroll 8
+        for (int m = 0; m < n; ++m) acc += __bfloat162float(p.q[mn_row(p, sq, kvh, m) + d]);
+        float mag = fabsf(acc) <= 3.4e38f ? fabsf(acc) : 3.4e38f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mag = fmaxf(mag, __shfl_xor_sync(0xffffffffu, mag, o));
+        if (lane == 0) ms.red[warp - 8][0] = mag;
+        asm volatile("bar.sync 2, 128;" ::: "memory");
+        mag = fmaxf(fmaxf(ms.red[0][0], ms.red[1][0]), fmaxf(ms.red[2][0], ms.red[3][0]));
+        const int e = exponent_of(mag);
+        float x = acc * pow2i(-e), part[3];
+        uint8_t* col = smem + kMnQ + (d >> 6) * kMnHalf + (d & 7) * 2;
+        const int c = (d & 63) >> 3;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const __half hv = k < 3 ? __float2half_rn(x) : __float2half_rn(0.f);
+          *reinterpret_cast<__half*>(col + (kMnScoreRows + k) * 128 + ((c ^ k) << 4)) = hv;
+          if (k < 3) {
+            part[k] = __half2float(hv);
+            x -= part[k];
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) part[k] += __shfl_xor_sync(0xffffffffu, part[k], o);
+          if (lane == 0) ms.red[warp - 8][1 + k] = part[k];
+        }
+        asm volatile("bar.sync 2, 128;" ::: "memory");
+        if (d < 8) {
+          float qs = 0.f;
+          if (d < 3) qs = (ms.red[0][1 + d] + ms.red[1][1 + d]) + (ms.red[2][1 + d] + ms.red[3][1 + d]);
+          const float qh = __half2float(__float2half_rn(qs)), qm = __half2float(__float2half_rn(qs - qh));
+          const uint32_t a = pack_f16x2(qh, qm);
+          *reinterpret_cast<uint4*>(ext_chunk(smem + kMnQx, kMnScoreRows + d, 0)) =
+              make_uint4(a, a, pack_f16x2(qs - qh - qm, 0.f), 0);
+          *reinterpret_cast<uint4*>(ext_chunk(smem + kMnQx, kMnScoreRows + d, 1)) = make_uint4(0, 0, 0, 0);
+        }
+        if (d == 0) ms.score_scale[0] = pow2i(e);
+      }
+      fence_proxy_async_smem();
+      tc_fence_before();
+      __syncthreads();
+      tc_fence_after();
+      const int w = warp - 8;
+      for (int t = 0; t < n_kt; ++t) {
+        const int s = t & 1, j = 2 * t + (w >> 1), rs = j % kMnRing;
+        const bool has = j < n_pages;
+        if (has && !mbar_wait(&ms.raw_full[rs], (j / kMnRing) & 1, p.status, kA4KernelId)) break;
+        const uint8_t* kb = smem + kMnRaw + rs * kFewStageBytes;
+        const int line0 = 32 * (w & 1);
+        const bool valid = has && (first + j) * kI4Page + line0 + lane < sq.k_end;
+        const MnParams pk = mn_params(kb, line0 + lane, valid);
+        const MnParams pv = mn_params(kb + kI4Block, line0 + lane, valid);
+        if (t >= 2 && !mbar_wait(&ms.k_empty[s], ((t >> 1) - 1) & 1, p.status, kA4KernelId)) break;
+        if (lane == 0) {
+          ms.ek[t & 3][w] = pk.e;
+          ms.ev[t & 3][w] = pv.e;
+        }
+        {
+          const float bh = __half2float(__float2half_rn(pk.base));
+          uint8_t* kx = smem + kMnKx + s * kMnExt;
+          const uint32_t hh = pack_f16x2(bh, bh), ll = pack_f16x2(pk.base - bh, pk.base - bh);
+          *reinterpret_cast<uint4*>(ext_chunk(kx, 32 * w + lane, 0)) = make_uint4(hh, ll, pack_f16x2(bh, 0.f), 0);
+          *reinterpret_cast<uint4*>(ext_chunk(kx, 32 * w + lane, 1)) = make_uint4(0, 0, 0, 0);
+        }
+        mn_convert<false>(kb, line0, has, smem + kMnK + s * 2 * kMnHalf, 32 * w, lane, pk);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ms.k_full[s]);
+        if (t >= 2 && !mbar_wait(&ms.v_empty[s], ((t >> 1) - 1) & 1, p.status, kA4KernelId)) break;
+        mn_convert<true>(kb + kI4Block, line0, has, smem + kMnV + s * 2 * kMnHalf, 32 * w, lane, pv);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&ms.v_full[s]);
+          if (has) mbar_arrive(&ms.raw_empty[rs]);
+        }
+      }
+      tc_fence_before();
+      __syncthreads();
+      tc_fence_after();
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMnRegsMisc));
+    MnTile c;
+    for (int tile = tile0; tile < n_tiles && mn_tile(p, sq, tile, c); tile += p.chunks) {
+      const int first = c.first, n_pages = c.n_pages, n_kt = c.n_kt;
+      tc_fence_before();
+      __syncthreads();
+      tc_fence_after();
+      const uint32_t tmem = ms.tmem;
+      if (warp == 12) {
+        // ----------------------------------------------------- pages ----
+        if (lane == 0)
+          for (int j = 0; j < n_pages; ++j) {
+            const int s = j % kMnRing;
+            if (j >= kMnRing && !mbar_wait(&ms.raw_empty[s], (j / kMnRing - 1) & 1, p.status, kA4KernelId)) break;
+            const int64_t page = a4_page(p, seq, first + j);
+            const size_t off = (static_cast<size_t>(page) * p.n_kv + kvh) * kI4Block;
+            uint8_t* dst = smem + kMnRaw + s * kFewStageBytes;
+            mbar_arrive_expect_tx(&ms.raw_full[s], kFewStageBytes);
+            bulk_load(dst, p.kc + off, kI4Block, &ms.raw_full[s]);
+            bulk_load(dst + kI4Block, p.vc + off, kI4Block, &ms.raw_full[s]);
+          }
+      } else if (warp == 13) {
+        // ------------------------------------------------------- MMA ----
+        if (lane == 0) {
+          constexpr uint32_t idesc_s = umma_idesc_f16(128, kMnKeys);
+          constexpr uint32_t idesc_pv = umma_idesc_f16(128, kA4HeadDim) | kUmmaBMajorMN;
+          const uint64_t dq[2] = {umma_desc_kmajor_sw128(smem_u32(smem + kMnQ)),
+                                  umma_desc_kmajor_sw128(smem_u32(smem + kMnQ + kMnHalf))};
+          const uint64_t dqx = umma_desc_kmajor_sw32(smem_u32(smem + kMnQx));
+          auto pv = [&](int t) -> bool {
+            const int s = t & 1;
+            if (!mbar_wait(&ms.p_full[s], (t >> 1) & 1, p.status, kA4KernelId) ||
+                !mbar_wait(&ms.v_full[s], (t >> 1) & 1, p.status, kA4KernelId))
+              return false;
+            tc_fence_after();
+            const uint64_t dv = umma_desc_mnmajor_sw128(smem_u32(smem + kMnV + s * 2 * kMnHalf), kMnHalf);
+#pragma unroll
+            for (int kk = 0; kk < kMnKeys / 16; ++kk)
+              umma_f16_ts(tmem + 256 + 128 * s, tmem + 128 * s + 8 * kk, dv + (kk * 2048 >> 4), idesc_pv,
+                          (t > 1 || kk > 0) ? 1u : 0u);
+            umma_commit(&ms.v_empty[s]);
+            umma_commit(&ms.pv_done[s]);
+            return true;
+          };
+          bool ok = true;
+          for (int t = 0; t < n_kt && ok; ++t) {
+            const int s = t & 1;
+            // S(t) goes over P(t - 2), which P V(t - 2) has read
+            ok = mbar_wait(&ms.k_full[s], (t >> 1) & 1, p.status, kA4KernelId) &&
+                 (t < 2 || mbar_wait(&ms.pv_done[s], ((t >> 1) - 1) & 1, p.status, kA4KernelId));
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t kst = smem_u32(smem + kMnK + s * 2 * kMnHalf);
+            const uint64_t dk[2] = {umma_desc_kmajor_sw128(kst), umma_desc_kmajor_sw128(kst + kMnHalf)};
+#pragma unroll
+            for (int kk = 0; kk < kA4HeadDim / 16; ++kk)
+              umma_bf16(tmem + 128 * s, dq[kk >> 2] + 2 * (kk & 3), dk[kk >> 2] + 2 * (kk & 3), idesc_s, kk > 0 ? 1u : 0u);
+            umma_bf16(tmem + 128 * s, dqx, umma_desc_kmajor_sw32(smem_u32(smem + kMnKx + s * kMnExt)), idesc_s, 1u);
+            umma_commit(&ms.k_empty[s]);
+            umma_commit(&ms.s_full[s]);
+            if (t >= 1) ok = pv(t - 1);
+          }
+          if (ok) pv(n_kt - 1);
+          // every arrival of the tensor cores is in before the barriers go
+          umma_commit(&ms.mma_done);
+          mbar_wait(&ms.mma_done, 0, p.status, kA4KernelId);
+        }
+      }
+      __syncwarp();
+      tc_fence_before();
+      __syncthreads();
+      tc_fence_after();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_dealloc(ms.tmem, 512);
   }
 }
 
 namespace {
 
 struct A4Plan {
+  bool many;        // the tcgen05 kernel
+  int batch;        // many: sequences
   int chunks, splits, split_pages;
 };
 
@@ -502,8 +1263,10 @@ struct A4Plan {
 // item, and the longest cache.  One CTA runs per SM and its eight warps take a
 // page each, so keys are split until the grid covers the SMs twice, and no
 // further than two pages per warp.
+constexpr int kFewMaxRows = 16;
+
 A4Plan a4_plan_few(int items, int rows, int group, int n_kv, int seqlen_max, int kv_splits) {
-  A4Plan pl;
+  A4Plan pl{};
   const int pages = (seqlen_max + kI4Page - 1) / kI4Page;
   pl.chunks = (rows * group + kFewRows - 1) / kFewRows;
   int s = kv_splits;
@@ -521,6 +1284,40 @@ A4Plan a4_plan_few(int items, int rows, int group, int n_kv, int seqlen_max, int
   return pl;
 }
 
+// Tiles of 128 rows x heads of a sequence, and key splits.  One CTA runs per
+// SM; a split costs a CTA about two tiles (the query operand, the pipeline's
+// fill, writing and joining the parts), so the count is the one whose waves of
+// CTAs take the fewest tile times.
+A4Plan a4_plan_many(int batch, int rows, int group, int n_kv, int seqlen_max, int kv_splits, bool scores) {
+  A4Plan pl{};
+  pl.many = true;
+  pl.batch = batch;
+  const int tile_rows = scores ? kMnScoreRows : kMnRows;
+  const int kt = (seqlen_max + kMnKeys - 1) / kMnKeys;
+  pl.chunks = static_cast<int>((static_cast<long long>(rows) * group + tile_rows - 1) / tile_rows);
+  if (pl.chunks < 1) pl.chunks = 1;
+  int s = kv_splits;
+  if (s <= 0) {
+    const long long ctas = static_cast<long long>(batch) * pl.chunks * n_kv;
+    long long best = 0;
+    for (int k = 1; k <= kt && k <= 64; ++k) {
+      const long long waves = (ctas * k + sm_count() - 1) / sm_count();
+      const long long cost = waves * ((kt + k - 1) / k + 2 + (k > 1 ? 1 : 0));
+      if (k == 1 || cost < best) {
+        best = cost;
+        s = k;
+      }
+    }
+  }
+  if (s > kt) s = kt;
+  if (s > 1024) s = 1024;
+  if (s < 1) s = 1;
+  const int tiles = (kt + s - 1) / s;
+  pl.split_pages = 2 * tiles;
+  pl.splits = (kt + tiles - 1) / tiles;
+  return pl;
+}
+
 struct A4Workspace {
   size_t score_acc, score_cnt, part_cnt, total;  // offsets; all of it is zero between calls
   size_t scratch;                                // bytes of partial results, never cleared
@@ -533,11 +1330,11 @@ A4Workspace a4_workspace(int32_t max_items, int32_t n_kv, int32_t seqlen_max, co
   if (scores) at += align_up(static_cast<size_t>(max_items) * seqlen_max * sizeof(unsigned long long), 256);
   w.score_cnt = at;
   if (scores) at += align_up(static_cast<size_t>(max_items) * sizeof(int32_t), 256);
-  const size_t cells = pl.splits > 1 ? static_cast<size_t>(max_items) * n_kv * pl.chunks : 0;
+  const size_t cells = pl.splits > 1 ? static_cast<size_t>(pl.many ? pl.batch : max_items) * n_kv * pl.chunks : 0;
   w.part_cnt = at;
   at += align_up(cells * sizeof(int32_t), 256);
   w.total = at;
-  w.scratch = cells * pl.splits * kFewPartFloats * sizeof(float);
+  w.scratch = cells * pl.splits * (pl.many ? kMnPartFloats : kFewPartFloats) * sizeof(float);
   return w;
 }
 
@@ -548,10 +1345,14 @@ bool a4_args_ok(int32_t n_rows, int32_t max_items, int32_t n_heads, int32_t n_kv
 }
 
 A4Plan a4_plan(int32_t n_rows, int32_t max_items, int32_t n_heads, int32_t n_kv, int32_t seqlen_max,
-               int32_t kv_splits, int32_t rows_hint) {
+               int32_t kv_splits, int32_t rows_hint, bool scores) {
   const int row_items = (n_rows + kA4ItemRows - 1) / kA4ItemRows;  // max_items = row_items + sequences
   const int items = max_items - row_items > row_items ? max_items - row_items : row_items;
-  const int rows = rows_hint > 0 && rows_hint < kA4ItemRows ? rows_hint : kA4ItemRows;
+  const int batch = max_items > row_items ? max_items - row_items : 1;
+  const int seq_rows = rows_hint > 0 && rows_hint < n_rows ? rows_hint : n_rows;
+  if (static_cast<long long>(seq_rows) * (n_heads / n_kv) > kFewMaxRows)
+    return a4_plan_many(batch, seq_rows, n_heads / n_kv, n_kv, seqlen_max, kv_splits, scores);
+  const int rows = seq_rows < kA4ItemRows ? seq_rows : kA4ItemRows;
   return a4_plan_few(items > 0 ? items : 1, rows, n_heads / n_kv, n_kv, seqlen_max, kv_splits);
 }
 
@@ -564,7 +1365,7 @@ extern "C" size_t fdllm_attn_int4_workspace_bytes(int32_t n_rows, int32_t max_it
   using namespace fdllm;
   if (scratch_bytes != nullptr) *scratch_bytes = 0;
   if (!a4_args_ok(n_rows, max_items, n_heads, n_kv_heads, seqlen_max, kv_splits, rows_hint)) return 0;
-  const A4Plan pl = a4_plan(n_rows, max_items, n_heads, n_kv_heads, seqlen_max, kv_splits, rows_hint);
+  const A4Plan pl = a4_plan(n_rows, max_items, n_heads, n_kv_heads, seqlen_max, kv_splits, rows_hint, scores != 0);
   const A4Workspace w = a4_workspace(max_items, n_kv_heads, seqlen_max, pl, scores != 0);
   if (scratch_bytes != nullptr) *scratch_bytes = w.scratch;
   return w.total;
@@ -589,7 +1390,8 @@ extern "C" int fdllm_attn_cache_int4(const void* q, void* o, const void* k_cache
   const void* ptrs[] = {q, o, k_cache, v_cache, plan};
   for (const void* x : ptrs)
     if (x == nullptr || !aligned16(x)) return FDLLM_ERR_ARG;
-  const A4Plan pl = a4_plan(n_rows, max_items, n_heads, n_kv_heads, seqlen_max, kv_splits, rows_hint);
+  const A4Plan pl = a4_plan(n_rows, max_items, n_heads, n_kv_heads, seqlen_max, kv_splits, rows_hint,
+                            attn_scores != nullptr);
   const A4Workspace w = a4_workspace(max_items, n_kv_heads, seqlen_max, pl, attn_scores != nullptr);
   if (w.total > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < w.total))
     return FDLLM_ERR_WORKSPACE;
@@ -630,9 +1432,18 @@ extern "C" int fdllm_attn_cache_int4(const void* q, void* o, const void* k_cache
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return FDLLM_ERR_CUDA;
   if (!attr[dev]) {
     if (cudaFuncSetAttribute(attn_int4_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem) !=
-        cudaSuccess)
+            cudaSuccess ||
+        cudaFuncSetAttribute(attn_int4_many_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMnSmem) !=
+            cudaSuccess)
       return FDLLM_ERR_CUDA;
     attr[dev] = true;
+  }
+  if (pl.many) {
+    const dim3 grid(static_cast<unsigned>(pl.batch) * pl.chunks, static_cast<unsigned>(n_kv_heads),
+                    static_cast<unsigned>(pl.splits));
+    if (launch_ex(attn_int4_many_kernel, grid, dim3(kMnThreads), kMnSmem, stream, 1, pdl_enabled(), p) != cudaSuccess)
+      return FDLLM_ERR_CUDA;
+    return cudaPeekAtLastError() == cudaSuccess ? FDLLM_OK : FDLLM_ERR_CUDA;
   }
   const dim3 grid(static_cast<unsigned>(max_items) * pl.chunks, static_cast<unsigned>(n_kv_heads),
                   static_cast<unsigned>(pl.splits));
