@@ -507,8 +507,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_int4_few_kernel(const A4P
 // (3 bits by 8), so
 //   K operand   (code - 8) * step * 2^-ek for 128 dims, and 16 more columns in
 //               which base_n * sum_d q_d is formed from two fp16 halves of the
-//               base and three of the sum (22 bits): the S tile is the whole
-//               logit, and a softmax thread needs no per-key constant;
+//               base and three of the sum (22 bits), and 0 or -infinity for a
+//               key past the end: the S tile is the whole logit, and a softmax
+//               thread needs no per-key constant;
 //   V operand   fp16((code - 8) * step + base): half an ulp is 2^-12 of the
 //               value, an eighth of what bf16 keys and values themselves carry;
 //   P operand   2^(logit + ev - R) in fp16 (2^-12, against bf16's 2^-9): the
@@ -527,18 +528,23 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_int4_few_kernel(const A4P
 // tensor cores' 17 instructions of about 60 clocks, 1024 for the exponentials
 // at 16 a clock and about 900 issue slots of each scheduler).
 //
-// Warps (16): 0-3 and 4-7 softmax of the even and the odd key tiles (thread =
-// tile row, with its own running maximum, sum and O accumulator: the two
-// halves never wait on each other and are joined at the end), 8-11 conversion
-// (each a 32-key piece of every tile), 12 bulk copies of pages, 13 the MMA
-// thread.  Tensor memory: S (and P over it) of the two halves, O of the two.
+// Warps (17): 0-3 and 4-7 softmax of the even and the odd key tiles (thread =
+// tile row; the reference R of a row passes from tile to tile through shared
+// memory, right after a tile's maximum, so the exponentials of consecutive
+// tiles overlap), 8-11 and 12-15 conversion of K and of V (each a 32-key piece
+// of every tile, which it fetches into a ring of its own), 16 the MMA thread.
+// Tensor memory: O and three S tiles with P over them: S(t) is issued two
+// tiles ahead of P V(t).
 // Key ranges are split over CTAs as in the other kernel.
 // ---------------------------------------------------------------------------
-constexpr int kMnThreads = 512;
+constexpr int kMnThreads = 17 * 32;
+constexpr int kMnConv = 8;         // conversion warps
 constexpr int kMnKeys = 128;
 constexpr int kMnRows = 128;
 constexpr int kMnScoreRows = 120;  // with scores: rows 120, 121, 122 carry the masked rows' sum
-constexpr int kMnRing = 4;         // pages
+constexpr int kMnRing = 2;         // raw pieces of a conversion warp
+constexpr int kMnPiece = 32;       // keys of a conversion warp
+constexpr int kMnPieceBytes = kMnPiece * (kI4Row + 4);  // codes, then parameters
 constexpr int kMnHalf = 128 * 128;             // 128 rows x 64 dims (128-byte swizzle)
 constexpr int kMnExt = 128 * 32;               // 128 rows x 16 columns (32-byte swizzle)
 constexpr int kMnQ = 0;                        // two halves, then the 16 columns
@@ -547,13 +553,11 @@ constexpr int kMnK = kMnQx + kMnExt;           // 2 stages of two halves; each 1
 constexpr int kMnV = kMnK + 4 * kMnHalf;
 constexpr int kMnKx = kMnV + 4 * kMnHalf;
 constexpr int kMnRaw = kMnKx + 2 * kMnExt;
-constexpr int kMnMisc = kMnRaw + kMnRing * kFewStageBytes;
-constexpr int kMnMiscBytes = 7 * 1024;
+constexpr int kMnMisc = kMnRaw + kMnConv * kMnRing * kMnPieceBytes;
+constexpr int kMnMiscBytes = 8 * 1024;
 constexpr int kMnSmem = 1024 + kMnMisc + kMnMiscBytes;
 static_assert(kMnK % 1024 == 0 && kMnV % 1024 == 0 && kMnKx % 1024 == 0 && kMnRaw % 128 == 0, "operand alignment");
 static_assert(kMnSmem <= 227 * 1024, "shared memory");
-constexpr int kMnRegsSoft = 184, kMnRegsConv = 88, kMnRegsMisc = 40;
-static_assert(256 * kMnRegsSoft + 128 * kMnRegsConv + 128 * kMnRegsMisc <= kMnThreads * 128, "setmaxnreg split");
 constexpr float kMnLazy = 8.f;   // log2 units a contribution may pass the reference by before it moves
 constexpr float kMnRaise = 6.f;  // P is raised by 2^6: with the 8 above, below fp16's 2^16
 constexpr int kMnPartFloats = kMnRows * kA4HeadDim + 2 * kMnRows;
@@ -590,6 +594,25 @@ __device__ __forceinline__ uint64_t umma_desc_kmajor_sw32(uint32_t smem_addr) {
   d |= static_cast<uint64_t>(6u) << 61;
   return d;
 }
+// pairs of fp32 in one instruction
+__device__ __forceinline__ uint64_t pack_f32x2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpack_f32x2(uint64_t v, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ uint8_t* ext_chunk(uint8_t* base, int row, int chunk) {
   return base + row * 32 + ((chunk ^ ((row >> 2) & 1)) << 4);
 }
@@ -600,71 +623,83 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 }
 // code - 8 of the pairs at bits 0 (even) or 4 (odd) of each half: 1024 + code
 // and 1024 + 16 code are fp16 values whose mantissas hold the code
-__device__ __forceinline__ __half2 i4_even_f16(uint32_t w) {
-  uint32_t m;
+__device__ __forceinline__ uint32_t i4_even_f16(uint32_t w) {
+  uint32_t m, r;
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(m) : "r"(w), "n"(0x000f000f), "r"(0x64006400u));
-  return __hsub2(*reinterpret_cast<const __half2*>(&m), __float2half2_rn(1032.f));
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(m), "r"(0xE408E408u));  // - 1032
+  return r;
 }
-__device__ __forceinline__ __half2 i4_odd_f16(uint32_t w) {
-  uint32_t m;
+__device__ __forceinline__ uint32_t i4_odd_f16(uint32_t w) {
+  uint32_t m, r;
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(m) : "r"(w), "n"(0x00f000f0), "r"(0x64006400u));
-  return __hfma2(*reinterpret_cast<const __half2*>(&m), __float2half2_rn(0.0625f), __float2half2_rn(-72.f));
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(m), "r"(0x2C002C00u), "r"(0xD480D480u));  // / 16 - 72
+  return r;
+}
+__device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 
 // the parameters of a lane's key, normalised over the warp's 32 keys
 struct MnParams {
-  __half2 step;      // twice
+  uint32_t step;     // fp16, twice
   float base;        // normalised, fp32
   int e;             // exponent of the piece
 };
-__device__ __forceinline__ MnParams mn_params(const uint8_t* block, int line, bool valid) {
+__device__ __forceinline__ MnParams mn_params(const uint8_t* piece, int lane, bool valid) {
   MnParams r;
-  const uint32_t pr = valid ? reinterpret_cast<const uint32_t*>(block + kI4Codes)[line] : 0u;
+  const uint32_t pr = valid ? reinterpret_cast<const uint32_t*>(piece + kMnPiece * kI4Row)[lane] : 0u;
   const float step = __uint_as_float(pr << 16), low = __uint_as_float(pr & 0xffff0000u);
   const float mag = fmaxf(fabsf(low), fabsf(fmaf(15.f, step, low)));
   // (a NaN group says nothing about the others' size)
   r.e = __reduce_max_sync(0xffffffffu, mag <= 3.4e38f ? exponent_of(mag) : -100);
   const float s = pow2i(-r.e);
-  r.step = __float2half2_rn(step * s);
+  r.step = pack_f16x2(step * s, step * s);
   r.base = fmaf(8.f, step, low) * s;
   return r;
 }
 
 // The warp's 32 keys of a K or V block into a tile (rows row0 ..): lane ->
 // key 8 i + lane / 4, 16 bytes of codes = 32 dims, four 16-byte chunks out.
-// The words of the lanes of dims 64 .. 127 are taken in another order, so that
-// a quarter-warp's stores fall into different banks.
+// The lanes of dims 64 .. 127 take their words in another order, so that a
+// quarter-warp's stores fall into different banks.  (A loop of four short
+// turns: unrolled, the roles' code together overran the instruction caches.)
 template <bool IS_V>
-__device__ __forceinline__ void mn_convert(const uint8_t* block, int line0, bool has, uint8_t* tile, int row0, int lane,
-                                           const MnParams& pm) {
-  const int q = lane & 3;
-  const bool upper = (q >> 1) != 0;
-  uint4 w[4];
+__device__ __forceinline__ void mn_convert(const uint8_t* piece, uint8_t* tile, int row0, int lane, const MnParams& pm) {
+  const int q = lane & 3, r = lane >> 2;
+  const int swap = (q >> 1) << 3;
+  const uint8_t* src = piece + r * kI4Row + 16 * q;
+  uint8_t* dst = tile + (q >> 1) * kMnHalf + (row0 + r) * 128;  // (row0 a multiple of 8)
+  int off[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    w[i] = has ? *reinterpret_cast<const uint4*>(block + (line0 + 8 * i + (lane >> 2)) * kI4Row + 16 * q)
-               : make_uint4(0, 0, 0, 0);
-  const uint32_t step_bits = *reinterpret_cast<const uint32_t*>(&pm.step);
-#pragma unroll
+  for (int j = 0; j < 4; ++j) off[j] = (((q & 1) * 4 + (j ^ (swap >> 2))) ^ r) << 4;
+  const uint32_t base_bits = IS_V ? pack_f16x2(pm.base, pm.base) : 0u;
+  uint2 a = *reinterpret_cast<const uint2*>(src + swap), b = *reinterpret_cast<const uint2*>(src + (swap ^ 8));
+#pragma unroll 1
   for (int i = 0; i < 4; ++i) {
-    const int key = 8 * i + (lane >> 2);
-    const uint32_t sb = __shfl_sync(0xffffffffu, step_bits, key);
-    const __half2 step = *reinterpret_cast<const __half2*>(&sb);
-    __half2 base = step;
-    if (IS_V) base = __float2half2_rn(__shfl_sync(0xffffffffu, pm.base, key));
-    const int r = row0 + key;
-    uint8_t* row = tile + (q >> 1) * kMnHalf + r * 128;
-    const uint32_t v[4] = {upper ? w[i].z : w[i].x, upper ? w[i].w : w[i].y, upper ? w[i].x : w[i].z,
-                           upper ? w[i].y : w[i].w};
+    const uint32_t v[4] = {a.x, a.y, b.x, b.y};
+    src += 8 * kI4Row;
+    if (i < 3) {
+      a = *reinterpret_cast<const uint2*>(src + swap);
+      b = *reinterpret_cast<const uint2*>(src + (swap ^ 8));
+    }
+    const uint32_t step = __shfl_sync(0xffffffffu, pm.step, 8 * i + r);
+    const uint32_t base = IS_V ? __shfl_sync(0xffffffffu, base_bits, 8 * i + r) : 0u;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int c = (q & 1) * 4 + (j ^ (upper ? 2 : 0));
       const uint32_t hi = v[j] >> 8;
-      __half2 o[4] = {i4_even_f16(v[j]), i4_odd_f16(v[j]), i4_even_f16(hi), i4_odd_f16(hi)};
+      uint32_t o[4] = {i4_even_f16(v[j]), i4_odd_f16(v[j]), i4_even_f16(hi), i4_odd_f16(hi)};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) o[k] = IS_V ? __hfma2(o[k], step, base) : __hmul2(o[k], step);
-      *reinterpret_cast<uint4*>(row + ((c ^ (r & 7)) << 4)) = *reinterpret_cast<const uint4*>(o);
+      for (int k = 0; k < 4; ++k) o[k] = IS_V ? fma_f16x2(o[k], step, base) : mul_f16x2(o[k], step);
+      *reinterpret_cast<uint4*>(dst + off[j]) = make_uint4(o[0], o[1], o[2], o[3]);
     }
+    dst += 8 * 128;
   }
 }
 
@@ -697,20 +732,25 @@ __device__ __forceinline__ int64_t mn_row(const A4Params& p, const MnSeq& s, int
 }
 
 struct MnMisc {
-  uint64_t raw_full[kMnRing], raw_empty[kMnRing];
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2], mma_done;
+  uint64_t raw_full[kMnConv * kMnRing];  // [conversion warp][stage]
+  uint64_t ev_full[8];             // [tile % 8]
+  uint64_t k_full[2], v_full[2], s_full[3], p_full[3], pv_done[3], r_ready[4][2], mma_done;
   uint32_t tmem;
   int32_t last, convert;
-  alignas(16) int32_t ek[4][4];     // [tile % 4][32-key piece]
-  alignas(16) int32_t ev[4][4];
+  // [tile % 8][32-key piece]: a conversion warp that writes tile t's has seen
+  // S(t - 2), so P V(t - 5), so the softmax of every tile up to t - 5
+  alignas(16) int32_t ek[8][4];
+  alignas(16) int32_t ev[8][4];
   float red[4][8];                  // score rows: warp partials
   float q_amax[2][kMnRows], q_sum[2][kMnRows];
   float score_scale[4];             // scale of the score rows
   alignas(16) float score[2][3][kMnKeys];
-  float2 ml[kMnRows];               // the odd half's (m, l)
+  float ref[kMnRows];               // R of the last tile that was decided
+  float l[2][kMnRows];              // the two softmax groups' sums
 };
 static_assert(sizeof(MnMisc) <= kMnMiscBytes, "misc");
-static_assert(offsetof(MnMisc, tmem) == (2 * kMnRing + 15) * 8, "the barriers lie in a row");
+constexpr int kMnBars = kMnConv * kMnRing + 8 + 22;
+static_assert(offsetof(MnMisc, tmem) == kMnBars * 8, "the barriers lie in a row");
 
 // What one row tile of a CTA takes: every role computes the same.
 struct MnTile {
@@ -751,28 +791,26 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
   const int n_tiles = (sq.rows * p.group + tile_rows - 1) / tile_rows;
   if (split * p.split_pages * kI4Page >= sq.k_end || tile0 >= n_tiles) return;
 
-  if (warp == 12) tmem_alloc(&ms.tmem, 512);
+  if (warp == 16) tmem_alloc(&ms.tmem, 512);
   // Every role runs its own loop over the CTA's row tiles (one, unless the
   // hint was low) with two CTA barriers a tile: operands and barriers in place
   // / everyone done.
   if (warp < 8) {
     // ------------------------------------------------------- softmax ----
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMnRegsSoft));
     const int h = warp >> 2, r = threadIdx.x & 127;
     MnTile c;
     for (int tile = tile0; tile < n_tiles && mn_tile(p, sq, tile, c); tile += p.chunks) {
       const int first = c.first, n_splits = c.n_splits, n_kt = c.n_kt, m0 = c.m0, rows = c.rows;
       const bool with_scores = c.with_scores;
       if (threadIdx.x == 0) {
-        for (int s = 0; s < kMnRing; ++s) {
-          mbar_init(&ms.raw_full[s], 1);
-          mbar_init(&ms.raw_empty[s], 2);  // two conversion warps a page
-        }
+        for (int s = 0; s < kMnConv * kMnRing; ++s) mbar_init(&ms.raw_full[s], 1);
+        for (int s = 0; s < 8; ++s) mbar_init(&ms.ev_full[s], 4);
         for (int s = 0; s < 2; ++s) {
           mbar_init(&ms.k_full[s], 4);
-          mbar_init(&ms.k_empty[s], 1);
           mbar_init(&ms.v_full[s], 4);
-          mbar_init(&ms.v_empty[s], 1);
+          for (int q = 0; q < 4; ++q) mbar_init(&ms.r_ready[q][s], 1);
+        }
+        for (int s = 0; s < 3; ++s) {
           mbar_init(&ms.s_full[s], 1);
           mbar_init(&ms.p_full[s], 4);
           mbar_init(&ms.pv_done[s], 1);
@@ -825,7 +863,7 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
           const float qs = (ms.q_sum[0][r] + ms.q_sum[1][r]) * s;
           const float qh = __half2float(__float2half_rn(qs)), qm = __half2float(__float2half_rn(qs - qh));
           const uint32_t a = pack_f16x2(qh, qm);
-          *reinterpret_cast<uint4*>(ext_chunk(smem + kMnQx, r, 0)) = make_uint4(a, a, pack_f16x2(qs - qh - qm, 0.f), 0);
+          *reinterpret_cast<uint4*>(ext_chunk(smem + kMnQx, r, 0)) = make_uint4(a, a, pack_f16x2(qs - qh - qm, 1.f), 0);
           *reinterpret_cast<uint4*>(ext_chunk(smem + kMnQx, r, 1)) = make_uint4(0, 0, 0, 0);
         }
       }
@@ -835,177 +873,156 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
       tc_fence_after();
       const uint32_t tmem = ms.tmem;
       const uint32_t tl = static_cast<uint32_t>((warp & 3) * 32) << 16;
-      const uint32_t ts = tmem + 128 * h + tl, to = tmem + 256 + 128 * h + tl;
+      const uint32_t to = tmem + tl;
       if (with_scores && r >= kMnScoreRows) row_mul = ms.score_scale[0];
       const bool score_warp = with_scores && (warp & 3) == 3;
       const float log_mul = with_scores && r >= kMnScoreRows ? 0.f : row_mul * p.scale_log2;
-      float m_used = -INFINITY, l = 0.f;  // the reference R, and the sum of 2^(logit - R + kMnRaise)
+      float ref_l = -INFINITY, l = 0.f;  // the sum of 2^(logit - ref_l + kMnRaise) over this group's tiles
       bool ok = true, range_ok = true;
       for (int t = h; t < n_kt; t += 2) {
-        ok = mbar_wait(&ms.s_full[h], (t >> 1) & 1, p.status, kA4KernelId);
+        const int slot = t % 3;
+        const uint32_t ts = tmem + 128 + 128 * slot + tl;
+        ok = mbar_wait(&ms.s_full[slot], (t / 3) & 1, p.status, kA4KernelId) &&
+             mbar_wait(&ms.ev_full[t & 7], (t >> 3) & 1, p.status, kA4KernelId);
         if (!ok) break;
         tc_fence_after();
-        float sv[4][32];
-        tmem_ld2_32x32b_x32(ts, ts + 32, sv[0], sv[1]);
-        tmem_ld2_32x32b_x32(ts + 64, ts + 96, sv[2], sv[3]);
-        const int4 ek4 = *reinterpret_cast<const int4*>(ms.ek[t & 3]);
-        const int4 ev4 = *reinterpret_cast<const int4*>(ms.ev[t & 3]);
-        const int ek[4] = {ek4.x, ek4.y, ek4.z, ek4.w}, ev[4] = {ev4.x, ev4.y, ev4.z, ev4.w};
-        const int n0 = first * kI4Page + t * kMnKeys;
-        const int n_valid = sq.k_end - n0;
-        if (score_warp) {
-          // lanes 24 .. 26 hold the three parts' logits of all keys
-          if (lane >= 24 && lane < 27) {
+        // pass 1: logits in log2 units are s * mul (keys past the end -inf);
+        // mt = max (logit + ev)
+        float mt = -INFINITY;
+#pragma unroll 1
+        for (int g = 0; g < 4; ++g) {
+          float v[32];
+          tmem_ld_32x32b_x32(ts + 32 * g, v);
+          const float k = pow2i(ms.ek[t & 7][g]);
+          if (score_warp && lane >= 24 && lane < 27) {
+            // lanes 24 .. 26 hold the three parts' logits of all keys
+            const float kr = k * row_mul;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const float k = row_mul * pow2i(ek[g]);
-#pragma unroll
-              for (int j = 0; j < 32; j += 4)
-                *reinterpret_cast<float4*>(&ms.score[h][lane - 24][32 * g + j]) =
-                    make_float4(sv[g][j] * k, sv[g][j + 1] * k, sv[g][j + 2] * k, sv[g][j + 3] * k);
-            }
+            for (int j = 0; j < 32; j += 4)
+              *reinterpret_cast<float4*>(&ms.score[h][lane - 24][32 * g + j]) =
+                  make_float4(v[j] * kr, v[j + 1] * kr, v[j + 2] * kr, v[j + 3] * kr);
           }
+#pragma unroll
+          for (int j = 4; j < 32; ++j) v[j & 3] = fmaxf(v[j & 3], v[j]);
+          mt = fmaxf(mt, fmaf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), log_mul * k,
+                              static_cast<float>(ms.ev[t & 7][g])));
+        }
+        if (score_warp) {
+          const int n0 = first * kI4Page + t * kMnKeys;
           __syncwarp();
           unsigned long long* acc = p.score_acc + static_cast<int64_t>(seq) * p.seqlen_max + n0;
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const int n = 32 * g + lane;
-            if (n < n_valid) a4_add_score(acc + n, ms.score[h][0][n] + ms.score[h][1][n] + ms.score[h][2][n], range_ok);
+            if (n0 + n < sq.k_end)
+              a4_add_score(acc + n, ms.score[h][0][n] + ms.score[h][1][n] + ms.score[h][2][n], range_ok);
           }
           __syncwarp();
         }
-        if (n_valid < kMnKeys) {  // uniform
-#pragma unroll
-          for (int g = 0; g < 4; ++g)
-#pragma unroll
-            for (int j = 0; j < 32; ++j) sv[g][j] = 32 * g + j < n_valid ? sv[g][j] : -INFINITY;
+        // the reference after the tile before, moved if this tile passes it
+        float ref = -INFINITY;
+        if (t > 0) {
+          ok = mbar_wait(&ms.r_ready[warp & 3][(t - 1) & 1], ((t - 1) >> 1) & 1, p.status, kA4KernelId);
+          if (!ok) break;
+          ref = ms.ref[r];
         }
-        // logits in log2 units are sv * mul; mt = max (logit + ev)
-        float mul[4], mt = -INFINITY;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          mul[g] = log_mul * pow2i(ek[g]);
-          float a[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) a[i] = sv[g][i];
-#pragma unroll
-          for (int j = 4; j < 32; ++j) a[j & 3] = fmaxf(a[j & 3], sv[g][j]);
-          mt = fmaxf(mt, fmaf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])), mul[g], static_cast<float>(ev[g])));
-        }
-        const bool need = mt > m_used + kMnLazy;
+        const bool need = mt > ref + kMnLazy;
         if (__any_sync(0xffffffffu, need)) {
-          const float a = need ? ex2_approx(m_used - mt) : 1.f;
-          if (t >= 2) {
-            // O holds this half's P V so far (done: S of this tile was issued after it)
+          if (t > 0) {
+            // O holds P V of the tiles before
+            ok = mbar_wait(&ms.pv_done[(t - 1) % 3], ((t - 1) / 3) & 1, p.status, kA4KernelId);
+            if (!ok) break;
+            tc_fence_after();
+            const float a = need ? ex2_approx(ref - mt) : 1.f;
 #pragma unroll 1
-            for (int c = 0; c < kA4HeadDim / 32; ++c) {
-              float ov[32];
-              tmem_ld_32x32b_x32(to + 32 * c, ov);
+            for (int c = 0; c < kA4HeadDim / 16; ++c) {
+              float ov[16];
+              tmem_ld_32x32b_x16(to + 16 * c, ov);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) ov[j] *= a;
-              tmem_st_32x32b_x32(to + 32 * c, ov);
+              for (int j = 0; j < 16; ++j) ov[j] *= a;
+              tmem_st_32x32b_x16(to + 16 * c, ov);
             }
+            tmem_wait_st();
           }
-          l *= a;
-          if (need) m_used = mt;
+          if (need) ref = mt;
         }
-        const float ref = m_used == -INFINITY ? 0.f : m_used;
-#pragma unroll
+        ms.ref[r] = ref;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ms.r_ready[warp & 3][t & 1]);
+        if (ref != ref_l) {
+          l *= ex2_approx(ref_l - ref);
+          ref_l = ref;
+        }
+        const float base = kMnRaise - (ref == -INFINITY ? 0.f : ref);
+        // pass 2: P = 2^(logit + ev - R + kMnRaise)
+        // (P goes over columns that have been read: 32 keys' over 16 columns)
+#pragma unroll 1
         for (int g = 0; g < 4; ++g) {
-          const float shift = kMnRaise + static_cast<float>(ev[g]) - ref;
+          float v[32];
+          tmem_ld_32x32b_x32(ts + 32 * g, v);
+          const int ev = ms.ev[t & 7][g];
+          const float shift = base + static_cast<float>(ev);
+          const float mul = log_mul * pow2i(ms.ek[t & 7][g]);
           float ps[4] = {0.f, 0.f, 0.f, 0.f};
           float pw[16];
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
-            const float x = ex2_approx(fmaf(sv[g][j], mul[g], shift));
-            const float y = ex2_approx(fmaf(sv[g][j + 1], mul[g], shift));
+            const float x = ex2_approx(fmaf(v[j], mul, shift));
+            const float y = ex2_approx(fmaf(v[j + 1], mul, shift));
             ps[j & 3] += x;
             ps[(j + 1) & 3] += y;
             pw[j >> 1] = __uint_as_float(pack_f16x2(x, y));
           }
-          l = fmaf((ps[0] + ps[1]) + (ps[2] + ps[3]), pow2i(-ev[g]), l);
+          l = fmaf((ps[0] + ps[1]) + (ps[2] + ps[3]), pow2i(-ev), l);
           tmem_st_32x32b_x16(ts + 16 * g, pw);
         }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&ms.p_full[h]);
+        if (lane == 0) mbar_arrive(&ms.p_full[slot]);
       }
       if (score_warp && !__all_sync(0xffffffffu, range_ok) && lane == 0)
         report(p.status, FDLLM_ERR_RANGE, seq, kA4KernelId);
-      // ---- join the two halves; this half's last product ----
-      const int mine = (n_kt - h + 1) / 2;  // tiles of this half
-      const bool have = ok && mine > 0 && mbar_wait(&ms.pv_done[h], (mine - 1) & 1, p.status, kA4KernelId);
-      if (have) tc_fence_after();
-      // the odd half's O rows through the K stages (its tiles' MMAs and, by
-      // the other half's wait below, all others are done): 16-byte units
-      // XOR-swizzled by row
-      float* stage = reinterpret_cast<float*>(smem + kMnK);
-      const bool two = n_kt > 1;
-      float m_o = m_used, l_o = have ? l : 0.f;
-      float f_mine = 1.f, f_other = 0.f;
-      if (h == 1 && two) {
-        asm volatile("bar.sync 1, 256;" ::: "memory");  // both halves' products are done
-#pragma unroll 1
-        for (int c = 0; c < kA4HeadDim / 32; ++c) {
-          float ov[32];
-          tmem_ld_32x32b_x32(to + 32 * c, ov);
+      // ---- O: this group's half of the dims of row r ----
+      ms.l[h][r] = l;
+      ms.q_amax[h][r] = ref_l;
+      if (ok) mbar_wait(&ms.pv_done[(n_kt - 1) % 3], ((n_kt - 1) / 3) & 1, p.status, kA4KernelId);
+      tc_fence_after();
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      {
+        const float m_o = ms.ref[r];
+        float l_o = 0.f;
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<float4*>(stage + r * kA4HeadDim + (((8 * c + j) ^ (r & 7)) << 2)) =
-                make_float4(ov[4 * j], ov[4 * j + 1], ov[4 * j + 2], ov[4 * j + 3]);
-        }
-        ms.ml[r] = make_float2(m_used, l_o);
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-      }
-      if (h == 0) {
-        if (two) {
-          asm volatile("bar.sync 1, 256;" ::: "memory");
-          asm volatile("bar.sync 1, 256;" ::: "memory");
-          const float2 o = ms.ml[r];
-          m_o = fmaxf(m_used, o.x);
-          const float ref = m_o == -INFINITY ? 0.f : m_o;
-          const float a = ex2_approx(m_used - ref), b = ex2_approx(o.x - ref);
-          l_o = a * l_o + b * o.y;
-          f_mine *= a;
-          f_other = b;
+        for (int g = 0; g < 2; ++g) {
+          const float rg = ms.q_amax[g][r];
+          l_o += ms.l[g][r] * (rg == m_o ? 1.f : ex2_approx(rg - m_o));
         }
         const bool direct = n_splits == 1;
         const float inv = direct ? (l_o > 0.f ? 1.f / l_o : (l_o == 0.f ? 0.f : l_o)) : 1.f;
-        f_mine *= inv;
-        f_other *= inv;
-        __nv_bfloat16* dst = p.o + mn_row(p, sq, kvh, m0 + min(r, rows - 1));
+        __nv_bfloat16* dst = p.o + mn_row(p, sq, kvh, m0 + min(r, rows - 1)) + 64 * h;
         const int64_t cell = (static_cast<int64_t>(seq) * p.n_kv + kvh) * p.chunks + tile;
         float* part = direct ? nullptr : p.part + (cell * p.splits + split) * kMnPartFloats;
 #pragma unroll 1
-        for (int c = 0; c < kA4HeadDim / 32; ++c) {
+        for (int c = 0; c < 2; ++c) {
           float ov[32];
-          tmem_ld_32x32b_x32(to + 32 * c, ov);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (two) x = *reinterpret_cast<const float4*>(stage + r * kA4HeadDim + (((8 * c + j) ^ (r & 7)) << 2));
-            ov[4 * j] = fmaf(ov[4 * j], f_mine, x.x * f_other);
-            ov[4 * j + 1] = fmaf(ov[4 * j + 1], f_mine, x.y * f_other);
-            ov[4 * j + 2] = fmaf(ov[4 * j + 2], f_mine, x.z * f_other);
-            ov[4 * j + 3] = fmaf(ov[4 * j + 3], f_mine, x.w * f_other);
-          }
+          tmem_ld_32x32b_x32(to + 64 * h + 32 * c, ov);
           if (r >= rows) continue;
           if (direct) {
 #pragma unroll
             for (int j = 0; j < 32; j += 8)
               *reinterpret_cast<uint4*>(dst + 32 * c + j) =
-                  make_uint4(pack_bf16x2(ov[j], ov[j + 1]), pack_bf16x2(ov[j + 2], ov[j + 3]),
-                             pack_bf16x2(ov[j + 4], ov[j + 5]), pack_bf16x2(ov[j + 6], ov[j + 7]));
+                  make_uint4(pack_bf16x2(ov[j] * inv, ov[j + 1] * inv), pack_bf16x2(ov[j + 2] * inv, ov[j + 3] * inv),
+                             pack_bf16x2(ov[j + 4] * inv, ov[j + 5] * inv),
+                             pack_bf16x2(ov[j + 6] * inv, ov[j + 7] * inv));
           } else {
             // [dim / 4][row][4]: a warp's stores are 512 contiguous bytes
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              __stcg(reinterpret_cast<float4*>(part) + (8 * c + j) * kMnRows + r,
+              __stcg(reinterpret_cast<float4*>(part) + (16 * h + 8 * c + j) * kMnRows + r,
                      make_float4(ov[4 * j], ov[4 * j + 1], ov[4 * j + 2], ov[4 * j + 3]));
           }
         }
-        if (!direct && r < rows) {
+        if (!direct && r < rows && h == 0) {
           __stcg(part + kMnRows * kA4HeadDim + r, m_o);
           __stcg(part + kMnRows * kA4HeadDim + kMnRows + r, l_o);
         }
@@ -1017,7 +1034,7 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
       tc_fence_after();
       if (threadIdx.x == 0) {
         uint64_t* b = ms.raw_full;  // every barrier, in a row
-        for (int i = 0; i < 2 * kMnRing + 15; ++i) mbar_inval(b + i);
+        for (int i = 0; i < kMnBars; ++i) mbar_inval(b + i);
       }
       if (n_splits > 1) {
         const int64_t cell = (static_cast<int64_t>(seq) * p.n_kv + kvh) * p.chunks + tile;
@@ -1073,13 +1090,12 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (ms.convert) a4_convert_scores(p, seq, min(sq.k_end, p.seqlen_max), 256);
     }
-  } else if (warp < 12) {
+  } else if (warp < 8 + kMnConv) {
     // ---------------------------------------------------- conversion ----
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMnRegsConv));
     MnTile c;
     for (int tile = tile0; tile < n_tiles && mn_tile(p, sq, tile, c); tile += p.chunks) {
       const int first = c.first, n_pages = c.n_pages, n_kt = c.n_kt;
-      if (c.with_scores) {
+      if (c.with_scores && warp < 12) {
         // rows 120 .. 122: the sum of the masked rows over rows and heads, in
         // three fp16 parts; rows 123 .. 127 zero.  Thread = dim.
         const int d = threadIdx.x - 256;
@@ -1119,7 +1135,7 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
           const float qh = __half2float(__float2half_rn(qs)), qm = __half2float(__float2half_rn(qs - qh));
           const uint32_t a = pack_f16x2(qh, qm);
           *reinterpret_cast<uint4*>(ext_chunk(smem + kMnQx, kMnScoreRows + d, 0)) =
-              make_uint4(a, a, pack_f16x2(qs - qh - qm, 0.f), 0);
+              make_uint4(a, a, pack_f16x2(qs - qh - qm, 1.f), 0);
           *reinterpret_cast<uint4*>(ext_chunk(smem + kMnQx, kMnScoreRows + d, 1)) = make_uint4(0, 0, 0, 0);
         }
         if (d == 0) ms.score_scale[0] = pow2i(e);
@@ -1128,69 +1144,76 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
       tc_fence_before();
       __syncthreads();
       tc_fence_after();
-      const int w = warp - 8;
+      const bool is_v = warp >= 12;
+      const int w = warp & 3;  // piece
+      uint8_t* ring = smem + kMnRaw + (warp - 8) * (kMnRing * kMnPieceBytes);
+      uint64_t* full = ms.raw_full + (warp - 8) * kMnRing;
+      const uint8_t* cache = is_v ? p.vc : p.kc;
+      // pages of tiles 32 k .. 32 k + 31, one a lane, read ahead of their use
+      auto page_of = [&](int t) -> int {
+        const int j = 2 * t + (w >> 1);
+        return j < n_pages ? static_cast<int>(a4_page(p, seq, first + j)) : 0;
+      };
+      int pages = page_of(lane);
+      auto load = [&](int t) {  // this warp's piece of tile t (the whole warp)
+        if ((t & 31) == 0 && t > 0) pages = page_of(t + lane);
+        const int page = __shfl_sync(0xffffffffu, pages, t & 31);
+        if (lane == 0 && 2 * t + (w >> 1) < n_pages) {
+          const int s = t % kMnRing;
+          const uint8_t* block = cache + (static_cast<size_t>(page) * p.n_kv + kvh) * kI4Block;
+          uint8_t* dst = ring + s * kMnPieceBytes;
+          mbar_arrive_expect_tx(&full[s], kMnPieceBytes);
+          bulk_load(dst, block + (w & 1) * (kMnPiece * kI4Row), kMnPiece * kI4Row, &full[s]);
+          bulk_load(dst + kMnPiece * kI4Row, block + kI4Codes + (w & 1) * (kMnPiece * 4), kMnPiece * 4, &full[s]);
+        }
+      };
+      for (int t = 0; t < min(n_kt, kMnRing); ++t) load(t);
       for (int t = 0; t < n_kt; ++t) {
-        const int s = t & 1, j = 2 * t + (w >> 1), rs = j % kMnRing;
+        const int s = t & 1, rs = t % kMnRing;
+        const int j = 2 * t + (w >> 1);
         const bool has = j < n_pages;
-        if (has && !mbar_wait(&ms.raw_full[rs], (j / kMnRing) & 1, p.status, kA4KernelId)) break;
-        const uint8_t* kb = smem + kMnRaw + rs * kFewStageBytes;
-        const int line0 = 32 * (w & 1);
-        const bool valid = has && (first + j) * kI4Page + line0 + lane < sq.k_end;
-        const MnParams pk = mn_params(kb, line0 + lane, valid);
-        const MnParams pv = mn_params(kb + kI4Block, line0 + lane, valid);
-        if (t >= 2 && !mbar_wait(&ms.k_empty[s], ((t >> 1) - 1) & 1, p.status, kA4KernelId)) break;
-        if (lane == 0) {
-          ms.ek[t & 3][w] = pk.e;
-          ms.ev[t & 3][w] = pv.e;
-        }
-        {
-          const float bh = __half2float(__float2half_rn(pk.base));
+        if (has && !mbar_wait(&full[rs], (t / kMnRing) & 1, p.status, kA4KernelId)) break;
+        const uint8_t* piece = ring + rs * kMnPieceBytes;
+        const bool valid = has && (first + j) * kI4Page + (w & 1) * kMnPiece + lane < sq.k_end;
+        const MnParams pm = mn_params(piece, lane, valid);
+        if (is_v) {
+          // (the exponents go out before V's stage is free: P needs them)
+          if (lane == 0) {
+            ms.ev[t & 7][w] = pm.e;
+            mbar_arrive(&ms.ev_full[t & 7]);
+          }
+          // V's stage is free when P V(t - 2) is done, K's when S(t - 2) is
+          if (t >= 2 && !mbar_wait(&ms.pv_done[(t - 2) % 3], ((t - 2) / 3) & 1, p.status, kA4KernelId)) break;
+          mn_convert<true>(piece, smem + kMnV + s * 2 * kMnHalf, kMnPiece * w, lane, pm);
+        } else {
+          if (t >= 2 && !mbar_wait(&ms.s_full[(t - 2) % 3], ((t - 2) / 3) & 1, p.status, kA4KernelId)) break;
+          if (lane == 0) ms.ek[t & 7][w] = pm.e;
+          const float bh = __half2float(__float2half_rn(pm.base));
           uint8_t* kx = smem + kMnKx + s * kMnExt;
-          const uint32_t hh = pack_f16x2(bh, bh), ll = pack_f16x2(pk.base - bh, pk.base - bh);
-          *reinterpret_cast<uint4*>(ext_chunk(kx, 32 * w + lane, 0)) = make_uint4(hh, ll, pack_f16x2(bh, 0.f), 0);
-          *reinterpret_cast<uint4*>(ext_chunk(kx, 32 * w + lane, 1)) = make_uint4(0, 0, 0, 0);
+          const uint32_t hh = pack_f16x2(bh, bh), ll = pack_f16x2(pm.base - bh, pm.base - bh);
+          *reinterpret_cast<uint4*>(ext_chunk(kx, kMnPiece * w + lane, 0)) =
+              make_uint4(hh, ll, pack_f16x2(bh, valid ? 0.f : -INFINITY), 0);
+          *reinterpret_cast<uint4*>(ext_chunk(kx, kMnPiece * w + lane, 1)) = make_uint4(0, 0, 0, 0);
+          mn_convert<false>(piece, smem + kMnK + s * 2 * kMnHalf, kMnPiece * w, lane, pm);
         }
-        mn_convert<false>(kb, line0, has, smem + kMnK + s * 2 * kMnHalf, 32 * w, lane, pk);
         fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ms.k_full[s]);
-        if (t >= 2 && !mbar_wait(&ms.v_empty[s], ((t >> 1) - 1) & 1, p.status, kA4KernelId)) break;
-        mn_convert<true>(kb + kI4Block, line0, has, smem + kMnV + s * 2 * kMnHalf, 32 * w, lane, pv);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&ms.v_full[s]);
-          if (has) mbar_arrive(&ms.raw_empty[rs]);
-        }
+        __syncwarp();  // (and every lane has read the raw stage)
+        if (lane == 0) mbar_arrive(is_v ? &ms.v_full[s] : &ms.k_full[s]);
+        if (t + kMnRing < n_kt) load(t + kMnRing);
       }
       tc_fence_before();
       __syncthreads();
       tc_fence_after();
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMnRegsMisc));
+    // ----------------------------------------------------------- MMA ----
     MnTile c;
     for (int tile = tile0; tile < n_tiles && mn_tile(p, sq, tile, c); tile += p.chunks) {
-      const int first = c.first, n_pages = c.n_pages, n_kt = c.n_kt;
+      const int n_kt = c.n_kt;
       tc_fence_before();
       __syncthreads();
       tc_fence_after();
       const uint32_t tmem = ms.tmem;
-      if (warp == 12) {
-        // ----------------------------------------------------- pages ----
-        if (lane == 0)
-          for (int j = 0; j < n_pages; ++j) {
-            const int s = j % kMnRing;
-            if (j >= kMnRing && !mbar_wait(&ms.raw_empty[s], (j / kMnRing - 1) & 1, p.status, kA4KernelId)) break;
-            const int64_t page = a4_page(p, seq, first + j);
-            const size_t off = (static_cast<size_t>(page) * p.n_kv + kvh) * kI4Block;
-            uint8_t* dst = smem + kMnRaw + s * kFewStageBytes;
-            mbar_arrive_expect_tx(&ms.raw_full[s], kFewStageBytes);
-            bulk_load(dst, p.kc + off, kI4Block, &ms.raw_full[s]);
-            bulk_load(dst + kI4Block, p.vc + off, kI4Block, &ms.raw_full[s]);
-          }
-      } else if (warp == 13) {
-        // ------------------------------------------------------- MMA ----
         if (lane == 0) {
           constexpr uint32_t idesc_s = umma_idesc_f16(128, kMnKeys);
           constexpr uint32_t idesc_pv = umma_idesc_f16(128, kA4HeadDim) | kUmmaBMajorMN;
@@ -1198,44 +1221,44 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
                                   umma_desc_kmajor_sw128(smem_u32(smem + kMnQ + kMnHalf))};
           const uint64_t dqx = umma_desc_kmajor_sw32(smem_u32(smem + kMnQx));
           auto pv = [&](int t) -> bool {
-            const int s = t & 1;
-            if (!mbar_wait(&ms.p_full[s], (t >> 1) & 1, p.status, kA4KernelId) ||
+            const int s = t & 1, slot = t % 3;
+            if (!mbar_wait(&ms.p_full[slot], (t / 3) & 1, p.status, kA4KernelId) ||
                 !mbar_wait(&ms.v_full[s], (t >> 1) & 1, p.status, kA4KernelId))
               return false;
             tc_fence_after();
             const uint64_t dv = umma_desc_mnmajor_sw128(smem_u32(smem + kMnV + s * 2 * kMnHalf), kMnHalf);
 #pragma unroll
             for (int kk = 0; kk < kMnKeys / 16; ++kk)
-              umma_f16_ts(tmem + 256 + 128 * s, tmem + 128 * s + 8 * kk, dv + (kk * 2048 >> 4), idesc_pv,
-                          (t > 1 || kk > 0) ? 1u : 0u);
-            umma_commit(&ms.v_empty[s]);
-            umma_commit(&ms.pv_done[s]);
+              umma_f16_ts(tmem, tmem + 128 + 128 * slot + 8 * kk, dv + (kk * 2048 >> 4), idesc_pv,
+                          (t > 0 || kk > 0) ? 1u : 0u);
+            umma_commit(&ms.pv_done[slot]);
             return true;
           };
           bool ok = true;
           for (int t = 0; t < n_kt && ok; ++t) {
-            const int s = t & 1;
-            // S(t) goes over P(t - 2), which P V(t - 2) has read
+            const int s = t & 1, slot = t % 3;
+            // S(t) goes over P(t - 3), which P V(t - 3) has read
             ok = mbar_wait(&ms.k_full[s], (t >> 1) & 1, p.status, kA4KernelId) &&
-                 (t < 2 || mbar_wait(&ms.pv_done[s], ((t >> 1) - 1) & 1, p.status, kA4KernelId));
+                 (t < 3 || mbar_wait(&ms.pv_done[slot], (t / 3 - 1) & 1, p.status, kA4KernelId));
             if (!ok) break;
             tc_fence_after();
             const uint32_t kst = smem_u32(smem + kMnK + s * 2 * kMnHalf);
             const uint64_t dk[2] = {umma_desc_kmajor_sw128(kst), umma_desc_kmajor_sw128(kst + kMnHalf)};
 #pragma unroll
             for (int kk = 0; kk < kA4HeadDim / 16; ++kk)
-              umma_bf16(tmem + 128 * s, dq[kk >> 2] + 2 * (kk & 3), dk[kk >> 2] + 2 * (kk & 3), idesc_s, kk > 0 ? 1u : 0u);
-            umma_bf16(tmem + 128 * s, dqx, umma_desc_kmajor_sw32(smem_u32(smem + kMnKx + s * kMnExt)), idesc_s, 1u);
-            umma_commit(&ms.k_empty[s]);
-            umma_commit(&ms.s_full[s]);
-            if (t >= 1) ok = pv(t - 1);
+              umma_bf16(tmem + 128 + 128 * slot, dq[kk >> 2] + 2 * (kk & 3), dk[kk >> 2] + 2 * (kk & 3), idesc_s,
+                        kk > 0 ? 1u : 0u);
+            umma_bf16(tmem + 128 + 128 * slot, dqx, umma_desc_kmajor_sw32(smem_u32(smem + kMnKx + s * kMnExt)), idesc_s,
+                      1u);
+            umma_commit(&ms.s_full[slot]);
+            if (t >= 2) ok = pv(t - 2);
           }
+          if (ok && n_kt > 1) ok = pv(n_kt - 2);
           if (ok) pv(n_kt - 1);
           // every arrival of the tensor cores is in before the barriers go
           umma_commit(&ms.mma_done);
           mbar_wait(&ms.mma_done, 0, p.status, kA4KernelId);
         }
-      }
       __syncwarp();
       tc_fence_before();
       __syncthreads();
@@ -1244,7 +1267,7 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 16) {
     tc_fence_after();
     tmem_dealloc(ms.tmem, 512);
   }

@@ -23,12 +23,13 @@ static_assert(kI4Block % 16 == 0, "bulk copies of whole blocks");
 
 // Codes of pair i of a word as bf16 integers code - 8 (exact).  128 + code is
 // a bf16 whose low mantissa bits are the code (the spacing at 128 is 1).
+// (Constants are written as bit patterns: the conversion intrinsics are
+// instructions of their own even for a literal.)
 __device__ __forceinline__ uint32_t i4_pair(uint32_t shifted) {
-  uint32_t m;
+  uint32_t m, r;
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(m) : "r"(shifted), "n"(0x000f000f), "r"(0x43004300u));
-  const __nv_bfloat162 c = *reinterpret_cast<const __nv_bfloat162*>(&m);
-  const __nv_bfloat162 r = __hsub2(c, __floats2bfloat162_rn(136.f, 136.f));
-  return *reinterpret_cast<const uint32_t*>(&r);
+  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(m), "r"(0xC308C308u));  // - 136
+  return r;
 }
 
 }  // namespace fdllm
