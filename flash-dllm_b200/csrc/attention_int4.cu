@@ -54,6 +54,21 @@ struct A4Params {
   int32_t splits, split_pages;     // key splits of split_pages pages each
 };
 
+// Bounded wait on an mbarrier phase: about a second of suspended tries.  Short
+// in place (the rare end is out of line): the roles of the tcgen05 kernel run
+// different code at once, and what does not fit the instruction caches
+// together is fetched again and again.
+__device__ __forceinline__ bool a4_timeout(int32_t* status) {
+  report(status, FDLLM_ERR_TIMEOUT, 0, kA4KernelId);
+  return false;
+}
+__device__ __forceinline__ bool a4_wait(uint64_t* bar, uint32_t parity, int32_t* status) {
+  if (mbar_try_wait(bar, parity)) return true;
+  for (int i = 0; i < 50000; ++i)
+    if (mbar_try_wait_suspend(bar, parity, kWaitSuspendNs)) return true;
+  return a4_timeout(status);
+}
+
 struct A4Item {
   int seq, k_end, m_start, m_len, t_start, rows, mchunk;
 };
@@ -528,21 +543,22 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_int4_few_kernel(const A4P
 // tensor cores' 17 instructions of about 60 clocks, 1024 for the exponentials
 // at 16 a clock and about 900 issue slots of each scheduler).
 //
-// Warps (17): 0-3 and 4-7 softmax of the even and the odd key tiles (thread =
-// tile row; the reference R of a row passes from tile to tile through shared
-// memory, right after a tile's maximum, so the exponentials of consecutive
-// tiles overlap), 8-11 and 12-15 conversion of K and of V (each a 32-key piece
-// of every tile, which it fetches into a ring of its own), 16 the MMA thread.
-// Tensor memory: O and three S tiles with P over them: S(t) is issued two
-// tiles ahead of P V(t).
+// Warps (32): 0-15 softmax, 16-21 and 22-27 conversion of K and of V (the
+// 32-key pieces of the tiles in turn; a warp fetches its own), 28 the MMA
+// thread.  A tile's softmax is shared by two groups of four warps (thread =
+// tile row x 64 keys), two more work on the next tile; the reference R of a row
+// passes from tile to tile through shared memory right after a tile's maximum
+// is known, so the exponentials of consecutive tiles overlap.  Tensor memory:
+// O and three S tiles with P over them: S(t) is issued two tiles ahead of P
+// V(t).
 // Key ranges are split over CTAs as in the other kernel.
 // ---------------------------------------------------------------------------
-constexpr int kMnThreads = 17 * 32;
-constexpr int kMnConv = 8;         // conversion warps
+constexpr int kMnThreads = 1024;
+constexpr int kMnSoft = 16;        // softmax warps
+constexpr int kMnConv = 12;        // conversion warps
 constexpr int kMnKeys = 128;
 constexpr int kMnRows = 128;
 constexpr int kMnScoreRows = 120;  // with scores: rows 120, 121, 122 carry the masked rows' sum
-constexpr int kMnRing = 2;         // raw pieces of a conversion warp
 constexpr int kMnPiece = 32;       // keys of a conversion warp
 constexpr int kMnPieceBytes = kMnPiece * (kI4Row + 4);  // codes, then parameters
 constexpr int kMnHalf = 128 * 128;             // 128 rows x 64 dims (128-byte swizzle)
@@ -553,11 +569,15 @@ constexpr int kMnK = kMnQx + kMnExt;           // 2 stages of two halves; each 1
 constexpr int kMnV = kMnK + 4 * kMnHalf;
 constexpr int kMnKx = kMnV + 4 * kMnHalf;
 constexpr int kMnRaw = kMnKx + 2 * kMnExt;
-constexpr int kMnMisc = kMnRaw + kMnConv * kMnRing * kMnPieceBytes;
-constexpr int kMnMiscBytes = 8 * 1024;
+constexpr int kMnMisc = kMnRaw + kMnConv * kMnPieceBytes;
+constexpr int kMnMiscBytes = 18 * 1024;
 constexpr int kMnSmem = 1024 + kMnMisc + kMnMiscBytes;
 static_assert(kMnK % 1024 == 0 && kMnV % 1024 == 0 && kMnKx % 1024 == 0 && kMnRaw % 128 == 0, "operand alignment");
 static_assert(kMnSmem <= 227 * 1024, "shared memory");
+// of 64 registers a thread at launch
+constexpr int kMnRegsSoft = 72, kMnRegsConv = 56, kMnRegsMisc = 48;
+static_assert(32 * (kMnSoft * kMnRegsSoft + kMnConv * kMnRegsConv + 4 * kMnRegsMisc) <= kMnThreads * 64,
+              "setmaxnreg split");
 constexpr float kMnLazy = 8.f;   // log2 units a contribution may pass the reference by before it moves
 constexpr float kMnRaise = 6.f;  // P is raised by 2^6: with the 8 above, below fp16's 2^16
 constexpr int kMnPartFloats = kMnRows * kA4HeadDim + 2 * kMnRows;
@@ -594,25 +614,21 @@ __device__ __forceinline__ uint64_t umma_desc_kmajor_sw32(uint32_t smem_addr) {
   d |= static_cast<uint64_t>(6u) << 61;
   return d;
 }
-// pairs of fp32 in one instruction
-__device__ __forceinline__ uint64_t pack_f32x2(float x, float y) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-__device__ __forceinline__ void unpack_f32x2(uint64_t v, float& x, float& y) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+// maximum of 32 values
+__device__ __forceinline__ float mn_max32(const float (&v)[32]) {
+  float a[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+  for (int j = 4; j < 28; j += 8)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = max3(a[i], v[j + i], v[j + 4 + i]);
+  return max3(max3(a[0], a[1], v[28]), max3(a[2], a[3], v[29]), fmaxf(v[30], v[31]));
 }
-__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
+
 __device__ __forceinline__ uint8_t* ext_chunk(uint8_t* base, int row, int chunk) {
   return base + row * 32 + ((chunk ^ ((row >> 2) & 1)) << 4);
 }
@@ -640,11 +656,6 @@ __device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
   return r;
 }
-__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
 
 // the parameters of a lane's key, normalised over the warp's 32 keys
 struct MnParams {
@@ -668,10 +679,10 @@ __device__ __forceinline__ MnParams mn_params(const uint8_t* piece, int lane, bo
 // The warp's 32 keys of a K or V block into a tile (rows row0 ..): lane ->
 // key 8 i + lane / 4, 16 bytes of codes = 32 dims, four 16-byte chunks out.
 // The lanes of dims 64 .. 127 take their words in another order, so that a
-// quarter-warp's stores fall into different banks.  (A loop of four short
-// turns: unrolled, the roles' code together overran the instruction caches.)
-template <bool IS_V>
-__device__ __forceinline__ void mn_convert(const uint8_t* piece, uint8_t* tile, int row0, int lane, const MnParams& pm) {
+// quarter-warp's stores fall into different banks.
+// K: base 0.
+__device__ __forceinline__ void mn_convert(const uint8_t* piece, uint8_t* tile, int row0, int lane, uint32_t step_n,
+                                           uint32_t base_n) {
   const int q = lane & 3, r = lane >> 2;
   const int swap = (q >> 1) << 3;
   const uint8_t* src = piece + r * kI4Row + 16 * q;
@@ -679,26 +690,21 @@ __device__ __forceinline__ void mn_convert(const uint8_t* piece, uint8_t* tile, 
   int off[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) off[j] = (((q & 1) * 4 + (j ^ (swap >> 2))) ^ r) << 4;
-  const uint32_t base_bits = IS_V ? pack_f16x2(pm.base, pm.base) : 0u;
-  uint2 a = *reinterpret_cast<const uint2*>(src + swap), b = *reinterpret_cast<const uint2*>(src + (swap ^ 8));
 #pragma unroll 1
   for (int i = 0; i < 4; ++i) {
+    const uint2 a = *reinterpret_cast<const uint2*>(src + swap), b = *reinterpret_cast<const uint2*>(src + (swap ^ 8));
     const uint32_t v[4] = {a.x, a.y, b.x, b.y};
-    src += 8 * kI4Row;
-    if (i < 3) {
-      a = *reinterpret_cast<const uint2*>(src + swap);
-      b = *reinterpret_cast<const uint2*>(src + (swap ^ 8));
-    }
-    const uint32_t step = __shfl_sync(0xffffffffu, pm.step, 8 * i + r);
-    const uint32_t base = IS_V ? __shfl_sync(0xffffffffu, base_bits, 8 * i + r) : 0u;
+    const uint32_t step = __shfl_sync(0xffffffffu, step_n, 8 * i + r);
+    const uint32_t base = __shfl_sync(0xffffffffu, base_n, 8 * i + r);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint32_t hi = v[j] >> 8;
       uint32_t o[4] = {i4_even_f16(v[j]), i4_odd_f16(v[j]), i4_even_f16(hi), i4_odd_f16(hi)};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) o[k] = IS_V ? fma_f16x2(o[k], step, base) : mul_f16x2(o[k], step);
+      for (int k = 0; k < 4; ++k) o[k] = fma_f16x2(o[k], step, base);
       *reinterpret_cast<uint4*>(dst + off[j]) = make_uint4(o[0], o[1], o[2], o[3]);
     }
+    src += 8 * kI4Row;
     dst += 8 * 128;
   }
 }
@@ -732,9 +738,9 @@ __device__ __forceinline__ int64_t mn_row(const A4Params& p, const MnSeq& s, int
 }
 
 struct MnMisc {
-  uint64_t raw_full[kMnConv * kMnRing];  // [conversion warp][stage]
+  uint64_t raw_full[kMnConv];
   uint64_t ev_full[8];             // [tile % 8]
-  uint64_t k_full[2], v_full[2], s_full[3], p_full[3], pv_done[3], r_ready[4][2], mma_done;
+  uint64_t k_full[2], v_full[2], s_full[3], p_full[3], pv_done[3], m_ready[4][2], r_ready[4][4], mma_done;
   uint32_t tmem;
   int32_t last, convert;
   // [tile % 8][32-key piece]: a conversion warp that writes tile t's has seen
@@ -743,13 +749,17 @@ struct MnMisc {
   alignas(16) int32_t ev[8][4];
   float red[4][8];                  // score rows: warp partials
   float q_amax[2][kMnRows], q_sum[2][kMnRows];
+  float q_mul[kMnRows];             // 2^e of the rows
   float score_scale[4];             // scale of the score rows
-  alignas(16) float score[2][3][kMnKeys];
-  float ref[kMnRows];               // R of the last tile that was decided
-  float l[2][kMnRows];              // the two softmax groups' sums
+  alignas(16) float score[4][3][64];
+  // [tile % 4]: the group that writes tile t + 4's has seen S(t + 4), so P V(t + 1),
+  // so both key halves of tile t + 1 have read R and their maxima of tile t
+  float mx[4][2][kMnRows];          // maximum of logit + ev over a key half
+  float ref[4][kMnRows];            // R after the tile
+  float l[4][kMnRows], l_ref[4][kMnRows];  // the softmax groups' sums and their references
 };
 static_assert(sizeof(MnMisc) <= kMnMiscBytes, "misc");
-constexpr int kMnBars = kMnConv * kMnRing + 8 + 22;
+constexpr int kMnBars = kMnConv + 8 + 38;
 static_assert(offsetof(MnMisc, tmem) == kMnBars * 8, "the barriers lie in a row");
 
 // What one row tile of a CTA takes: every role computes the same.
@@ -791,80 +801,88 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
   const int n_tiles = (sq.rows * p.group + tile_rows - 1) / tile_rows;
   if (split * p.split_pages * kI4Page >= sq.k_end || tile0 >= n_tiles) return;
 
-  if (warp == 16) tmem_alloc(&ms.tmem, 512);
+  if (warp == 28) tmem_alloc(&ms.tmem, 512);
   // Every role runs its own loop over the CTA's row tiles (one, unless the
   // hint was low) with two CTA barriers a tile: operands and barriers in place
   // / everyone done.
-  if (warp < 8) {
+  if (warp < kMnSoft) {
     // ------------------------------------------------------- softmax ----
-    const int h = warp >> 2, r = threadIdx.x & 127;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMnRegsSoft));
+    // group: keys 64 hk .. of the tiles of parity par
+    const int grp = warp >> 2, par = grp >> 1, hk = grp & 1, r = threadIdx.x & 127;
     MnTile c;
     for (int tile = tile0; tile < n_tiles && mn_tile(p, sq, tile, c); tile += p.chunks) {
       const int first = c.first, n_splits = c.n_splits, n_kt = c.n_kt, m0 = c.m0, rows = c.rows;
       const bool with_scores = c.with_scores;
       if (threadIdx.x == 0) {
-        for (int s = 0; s < kMnConv * kMnRing; ++s) mbar_init(&ms.raw_full[s], 1);
+        for (int s = 0; s < kMnConv; ++s) mbar_init(&ms.raw_full[s], 1);
         for (int s = 0; s < 8; ++s) mbar_init(&ms.ev_full[s], 4);
         for (int s = 0; s < 2; ++s) {
           mbar_init(&ms.k_full[s], 4);
           mbar_init(&ms.v_full[s], 4);
-          for (int q = 0; q < 4; ++q) mbar_init(&ms.r_ready[q][s], 1);
+          for (int q = 0; q < 4; ++q) {
+            mbar_init(&ms.m_ready[q][s], 2);
+            mbar_init(&ms.r_ready[q][s], 1);
+            mbar_init(&ms.r_ready[q][2 + s], 1);
+          }
         }
         for (int s = 0; s < 3; ++s) {
           mbar_init(&ms.s_full[s], 1);
-          mbar_init(&ms.p_full[s], 4);
+          mbar_init(&ms.p_full[s], 8);
           mbar_init(&ms.pv_done[s], 1);
         }
         mbar_init(&ms.mma_done, 1);
         fence_barrier_init();
       }
       // ---- the query operand ----
-      float row_mul;  // 2^e of the row
-      const bool fill = !(with_scores && r >= kMnScoreRows);  // rows the conversion warps fill instead
-      uint4 v[8];
-      const uint4* src = reinterpret_cast<const uint4*>(p.q + mn_row(p, sq, kvh, m0 + min(r, rows - 1)) + 64 * h);
+      if (grp < 2) {
+        const int h = grp;
+        const bool fill = !(with_scores && r >= kMnScoreRows);  // rows the conversion warps fill instead
+        uint4 v[8];
+        const uint4* src = reinterpret_cast<const uint4*>(p.q + mn_row(p, sq, kvh, m0 + min(r, rows - 1)) + 64 * h);
 #pragma unroll
-      for (int c = 0; c < 8; ++c) v[c] = r < rows ? src[c] : make_uint4(0, 0, 0, 0);
-      uint32_t mag = 0;
-      float sum = 0.f;
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          mag = __vmaxu2(mag, w[k] & 0x7fff7fffu);
-          const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]));
-          sum += f.x + f.y;
-        }
-      }
-      mag = max(mag & 0xffffu, mag >> 16);
-      ms.q_amax[h][r] = __uint_as_float(mag << 16);
-      ms.q_sum[h][r] = sum;
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      // (patterns order as magnitudes: an infinity or NaN keeps e = 126 and stays what it is)
-      const uint32_t both = max(__float_as_uint(ms.q_amax[0][r]), __float_as_uint(ms.q_amax[1][r]));
-      const int e = exponent_of(__uint_as_float(both));
-      const float s = pow2i(-e);
-      row_mul = pow2i(e);
-      if (fill) {
-        uint8_t* row = smem + kMnQ + h * kMnHalf + r * 128;
+        for (int c = 0; c < 8; ++c) v[c] = r < rows ? src[c] : make_uint4(0, 0, 0, 0);
+        uint32_t mag = 0;
+        float sum = 0.f;
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
           const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
-          uint32_t o[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
+            mag = __vmaxu2(mag, w[k] & 0x7fff7fffu);
             const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]));
-            o[k] = pack_f16x2(f.x * s, f.y * s);
+            sum += f.x + f.y;
           }
-          *reinterpret_cast<uint4*>(row + ((c ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
         }
-        if (h == 0) {
-          const float qs = (ms.q_sum[0][r] + ms.q_sum[1][r]) * s;
-          const float qh = __half2float(__float2half_rn(qs)), qm = __half2float(__float2half_rn(qs - qh));
-          const uint32_t a = pack_f16x2(qh, qm);
-          *reinterpret_cast<uint4*>(ext_chunk(smem + kMnQx, r, 0)) = make_uint4(a, a, pack_f16x2(qs - qh - qm, 1.f), 0);
-          *reinterpret_cast<uint4*>(ext_chunk(smem + kMnQx, r, 1)) = make_uint4(0, 0, 0, 0);
+        mag = max(mag & 0xffffu, mag >> 16);
+        ms.q_amax[h][r] = __uint_as_float(mag << 16);
+        ms.q_sum[h][r] = sum;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        // (patterns order as magnitudes: an infinity or NaN keeps e = 126 and stays what it is)
+        const uint32_t both = max(__float_as_uint(ms.q_amax[0][r]), __float_as_uint(ms.q_amax[1][r]));
+        const int e = exponent_of(__uint_as_float(both));
+        const float s = pow2i(-e);
+        if (h == 0) ms.q_mul[r] = pow2i(e);
+        if (fill) {
+          uint8_t* row = smem + kMnQ + h * kMnHalf + r * 128;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+            uint32_t o[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]));
+              o[k] = pack_f16x2(f.x * s, f.y * s);
+            }
+            *reinterpret_cast<uint4*>(row + ((c ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+          }
+          if (h == 0) {
+            const float qs = (ms.q_sum[0][r] + ms.q_sum[1][r]) * s;
+            const float qh = __half2float(__float2half_rn(qs)), qm = __half2float(__float2half_rn(qs - qh));
+            const uint32_t a = pack_f16x2(qh, qm);
+            *reinterpret_cast<uint4*>(ext_chunk(smem + kMnQx, r, 0)) = make_uint4(a, a, pack_f16x2(qs - qh - qm, 1.f), 0);
+            *reinterpret_cast<uint4*>(ext_chunk(smem + kMnQx, r, 1)) = make_uint4(0, 0, 0, 0);
+          }
         }
       }
       fence_proxy_async_smem();
@@ -874,107 +892,106 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
       const uint32_t tmem = ms.tmem;
       const uint32_t tl = static_cast<uint32_t>((warp & 3) * 32) << 16;
       const uint32_t to = tmem + tl;
-      if (with_scores && r >= kMnScoreRows) row_mul = ms.score_scale[0];
+      const bool score_row = with_scores && r >= kMnScoreRows;
+      const float row_mul = score_row ? ms.score_scale[0] : ms.q_mul[r];
       const bool score_warp = with_scores && (warp & 3) == 3;
-      const float log_mul = with_scores && r >= kMnScoreRows ? 0.f : row_mul * p.scale_log2;
-      float ref_l = -INFINITY, l = 0.f;  // the sum of 2^(logit - ref_l + kMnRaise) over this group's tiles
+      const float log_mul = score_row ? 0.f : row_mul * p.scale_log2;
+      float ref_l = -INFINITY, l = 0.f;  // the sum of 2^(logit - ref_l + kMnRaise) over this group's keys
       bool ok = true, range_ok = true;
-      for (int t = h; t < n_kt; t += 2) {
+      for (int t = par; t < n_kt; t += 2) {
         const int slot = t % 3;
         const uint32_t ts = tmem + 128 + 128 * slot + tl;
-        ok = mbar_wait(&ms.s_full[slot], (t / 3) & 1, p.status, kA4KernelId) &&
-             mbar_wait(&ms.ev_full[t & 7], (t >> 3) & 1, p.status, kA4KernelId);
+        ok = a4_wait(&ms.s_full[slot], (t / 3) & 1, p.status) && a4_wait(&ms.ev_full[t & 7], (t >> 3) & 1, p.status);
         if (!ok) break;
         tc_fence_after();
-        // pass 1: logits in log2 units are s * mul (keys past the end -inf);
-        // mt = max (logit + ev)
+        // pass 1: logits in log2 units are s * mul (keys past the end
+        // -infinity); mt = max (logit + ev)
         float mt = -INFINITY;
 #pragma unroll 1
-        for (int g = 0; g < 4; ++g) {
+        for (int g = 2 * hk; g < 2 * hk + 2; ++g) {
           float v[32];
           tmem_ld_32x32b_x32(ts + 32 * g, v);
           const float k = pow2i(ms.ek[t & 7][g]);
           if (score_warp && lane >= 24 && lane < 27) {
-            // lanes 24 .. 26 hold the three parts' logits of all keys
+            // lanes 24 .. 26 hold the three parts' logits
             const float kr = k * row_mul;
 #pragma unroll
             for (int j = 0; j < 32; j += 4)
-              *reinterpret_cast<float4*>(&ms.score[h][lane - 24][32 * g + j]) =
+              *reinterpret_cast<float4*>(&ms.score[grp][lane - 24][32 * (g & 1) + j]) =
                   make_float4(v[j] * kr, v[j + 1] * kr, v[j + 2] * kr, v[j + 3] * kr);
           }
-#pragma unroll
-          for (int j = 4; j < 32; ++j) v[j & 3] = fmaxf(v[j & 3], v[j]);
-          mt = fmaxf(mt, fmaf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), log_mul * k,
-                              static_cast<float>(ms.ev[t & 7][g])));
+          mt = fmaxf(mt, fmaf(mn_max32(v), log_mul * k, static_cast<float>(ms.ev[t & 7][g])));
         }
+        ms.mx[t & 3][hk][r] = mt;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ms.m_ready[warp & 3][par]);
         if (score_warp) {
-          const int n0 = first * kI4Page + t * kMnKeys;
-          __syncwarp();
+          const int n0 = first * kI4Page + t * kMnKeys + 64 * hk;
           unsigned long long* acc = p.score_acc + static_cast<int64_t>(seq) * p.seqlen_max + n0;
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const int n = 32 * g + lane;
+          for (int u = 0; u < 2; ++u) {
+            const int n = 32 * u + lane;
             if (n0 + n < sq.k_end)
-              a4_add_score(acc + n, ms.score[h][0][n] + ms.score[h][1][n] + ms.score[h][2][n], range_ok);
+              a4_add_score(acc + n, ms.score[grp][0][n] + ms.score[grp][1][n] + ms.score[grp][2][n], range_ok);
           }
           __syncwarp();
         }
         // the reference after the tile before, moved if this tile passes it
-        float ref = -INFINITY;
-        if (t > 0) {
-          ok = mbar_wait(&ms.r_ready[warp & 3][(t - 1) & 1], ((t - 1) >> 1) & 1, p.status, kA4KernelId);
-          if (!ok) break;
-          ref = ms.ref[r];
-        }
+        // (both key halves decide the same)
+        ok = a4_wait(&ms.m_ready[warp & 3][par], (t >> 1) & 1, p.status) &&
+             (t == 0 || a4_wait(&ms.r_ready[warp & 3][(t - 1) & 3], ((t - 1) >> 2) & 1, p.status));
+        if (!ok) break;
+        mt = fmaxf(mt, ms.mx[t & 3][hk ^ 1][r]);
+        float ref = t > 0 ? ms.ref[(t - 1) & 3][r] : -INFINITY;
         const bool need = mt > ref + kMnLazy;
-        if (__any_sync(0xffffffffu, need)) {
-          if (t > 0) {
-            // O holds P V of the tiles before
-            ok = mbar_wait(&ms.pv_done[(t - 1) % 3], ((t - 1) / 3) & 1, p.status, kA4KernelId);
-            if (!ok) break;
-            tc_fence_after();
-            const float a = need ? ex2_approx(ref - mt) : 1.f;
+        if (t > 0 && __any_sync(0xffffffffu, need)) {
+          // O holds P V of the tiles before; each key half scales half of its dims
+          ok = a4_wait(&ms.pv_done[(t - 1) % 3], ((t - 1) / 3) & 1, p.status);
+          if (!ok) break;
+          tc_fence_after();
+          const float a = need ? ex2_approx(ref - mt) : 1.f;
 #pragma unroll 1
-            for (int c = 0; c < kA4HeadDim / 16; ++c) {
-              float ov[16];
-              tmem_ld_32x32b_x16(to + 16 * c, ov);
+          for (int c = 0; c < 4; ++c) {
+            float ov[16];
+            tmem_ld_32x32b_x16(to + 64 * hk + 16 * c, ov);
 #pragma unroll
-              for (int j = 0; j < 16; ++j) ov[j] *= a;
-              tmem_st_32x32b_x16(to + 16 * c, ov);
-            }
-            tmem_wait_st();
+            for (int j = 0; j < 16; ++j) ov[j] *= a;
+            tmem_st_32x32b_x16(to + 64 * hk + 16 * c, ov);
           }
-          if (need) ref = mt;
         }
-        ms.ref[r] = ref;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ms.r_ready[warp & 3][t & 1]);
+        if (need) ref = mt;
+        if (hk == 0) {
+          ms.ref[t & 3][r] = ref;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ms.r_ready[warp & 3][t & 3]);
+        }
         if (ref != ref_l) {
           l *= ex2_approx(ref_l - ref);
           ref_l = ref;
         }
         const float base = kMnRaise - (ref == -INFINITY ? 0.f : ref);
         // pass 2: P = 2^(logit + ev - R + kMnRaise)
-        // (P goes over columns that have been read: 32 keys' over 16 columns)
 #pragma unroll 1
-        for (int g = 0; g < 4; ++g) {
+        for (int g = 2 * hk; g < 2 * hk + 2; ++g) {
           float v[32];
           tmem_ld_32x32b_x32(ts + 32 * g, v);
           const int ev = ms.ev[t & 7][g];
           const float shift = base + static_cast<float>(ev);
           const float mul = log_mul * pow2i(ms.ek[t & 7][g]);
           float ps[4] = {0.f, 0.f, 0.f, 0.f};
-          float pw[16];
+          uint32_t pw[16];
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
             const float x = ex2_approx(fmaf(v[j], mul, shift));
             const float y = ex2_approx(fmaf(v[j + 1], mul, shift));
             ps[j & 3] += x;
             ps[(j + 1) & 3] += y;
-            pw[j >> 1] = __uint_as_float(pack_f16x2(x, y));
+            pw[j >> 1] = pack_f16x2(x, y);
           }
           l = fmaf((ps[0] + ps[1]) + (ps[2] + ps[3]), pow2i(-ev), l);
-          tmem_st_32x32b_x16(ts + 16 * g, pw);
+          // P of keys 0 .. 63 in columns 0 .. 31, of keys 64 .. 127 in columns
+          // 64 .. 95: either half writes over logits of its own that it has read
+          tmem_st_32x32b_x16(ts + 64 * hk + 16 * (g & 1), pw);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -983,48 +1000,44 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
       }
       if (score_warp && !__all_sync(0xffffffffu, range_ok) && lane == 0)
         report(p.status, FDLLM_ERR_RANGE, seq, kA4KernelId);
-      // ---- O: this group's half of the dims of row r ----
-      ms.l[h][r] = l;
-      ms.q_amax[h][r] = ref_l;
-      if (ok) mbar_wait(&ms.pv_done[(n_kt - 1) % 3], ((n_kt - 1) / 3) & 1, p.status, kA4KernelId);
+      // ---- O: this group's 32 dims of row r ----
+      ms.l[grp][r] = l;
+      ms.l_ref[grp][r] = ref_l;
+      if (ok) a4_wait(&ms.pv_done[(n_kt - 1) % 3], ((n_kt - 1) / 3) & 1, p.status);
       tc_fence_after();
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+      asm volatile("bar.sync 1, 512;" ::: "memory");
       {
-        const float m_o = ms.ref[r];
+        const float m_o = ms.ref[(n_kt - 1) & 3][r];
         float l_o = 0.f;
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const float rg = ms.q_amax[g][r];
+        for (int g = 0; g < 4; ++g) {
+          const float rg = ms.l_ref[g][r];
           l_o += ms.l[g][r] * (rg == m_o ? 1.f : ex2_approx(rg - m_o));
         }
         const bool direct = n_splits == 1;
         const float inv = direct ? (l_o > 0.f ? 1.f / l_o : (l_o == 0.f ? 0.f : l_o)) : 1.f;
-        __nv_bfloat16* dst = p.o + mn_row(p, sq, kvh, m0 + min(r, rows - 1)) + 64 * h;
-        const int64_t cell = (static_cast<int64_t>(seq) * p.n_kv + kvh) * p.chunks + tile;
-        float* part = direct ? nullptr : p.part + (cell * p.splits + split) * kMnPartFloats;
-#pragma unroll 1
-        for (int c = 0; c < 2; ++c) {
-          float ov[32];
-          tmem_ld_32x32b_x32(to + 64 * h + 32 * c, ov);
-          if (r >= rows) continue;
-          if (direct) {
+        float ov[32];
+        tmem_ld_32x32b_x32(to + 32 * grp, ov);
+        if (r < rows && direct) {
+          __nv_bfloat16* dst = p.o + mn_row(p, sq, kvh, m0 + r) + 32 * grp;
 #pragma unroll
-            for (int j = 0; j < 32; j += 8)
-              *reinterpret_cast<uint4*>(dst + 32 * c + j) =
-                  make_uint4(pack_bf16x2(ov[j] * inv, ov[j + 1] * inv), pack_bf16x2(ov[j + 2] * inv, ov[j + 3] * inv),
-                             pack_bf16x2(ov[j + 4] * inv, ov[j + 5] * inv),
-                             pack_bf16x2(ov[j + 6] * inv, ov[j + 7] * inv));
-          } else {
-            // [dim / 4][row][4]: a warp's stores are 512 contiguous bytes
+          for (int j = 0; j < 32; j += 8)
+            *reinterpret_cast<uint4*>(dst + j) =
+                make_uint4(pack_bf16x2(ov[j] * inv, ov[j + 1] * inv), pack_bf16x2(ov[j + 2] * inv, ov[j + 3] * inv),
+                           pack_bf16x2(ov[j + 4] * inv, ov[j + 5] * inv),
+                           pack_bf16x2(ov[j + 6] * inv, ov[j + 7] * inv));
+        } else if (r < rows) {
+          // [dim / 4][row][4]: a warp's stores are 512 contiguous bytes
+          const int64_t cell = (static_cast<int64_t>(seq) * p.n_kv + kvh) * p.chunks + tile;
+          float* part = p.part + (cell * p.splits + split) * kMnPartFloats;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              __stcg(reinterpret_cast<float4*>(part) + (16 * h + 8 * c + j) * kMnRows + r,
-                     make_float4(ov[4 * j], ov[4 * j + 1], ov[4 * j + 2], ov[4 * j + 3]));
+          for (int j = 0; j < 8; ++j)
+            __stcg(reinterpret_cast<float4*>(part) + (8 * grp + j) * kMnRows + r,
+                   make_float4(ov[4 * j], ov[4 * j + 1], ov[4 * j + 2], ov[4 * j + 3]));
+          if (grp == 0) {
+            __stcg(part + kMnRows * kA4HeadDim + r, m_o);
+            __stcg(part + kMnRows * kA4HeadDim + kMnRows + r, l_o);
           }
-        }
-        if (!direct && r < rows && h == 0) {
-          __stcg(part + kMnRows * kA4HeadDim + r, m_o);
-          __stcg(part + kMnRows * kA4HeadDim + kMnRows + r, l_o);
         }
       }
       // every role is done with this tile: its barriers and buffers are free
@@ -1043,7 +1056,7 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
           if (ms.last) p.part_cnt[cell] = 0;
           __threadfence();
         }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+        asm volatile("bar.sync 1, 512;" ::: "memory");
         if (ms.last) {
           // thread -> (row, 4 dims) units; splits joined in order
           const float* all = p.part + cell * p.splits * kMnPartFloats;
@@ -1060,7 +1073,7 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
             const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
             __nv_bfloat16* dst = p.o + mn_row(p, sq, kvh, m0 + r);
 #pragma unroll 1
-            for (int u = (threadIdx.x >> 7); u < kA4HeadDim / 4; u += 2) {
+            for (int u = (threadIdx.x >> 7); u < kA4HeadDim / 4; u += 4) {
               float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
               for (int k = 0; k < n_splits; ++k) {
@@ -1076,7 +1089,7 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
             }
           }
         }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+        asm volatile("bar.sync 1, 512;" ::: "memory");
       }
     }
     if (p.scores != nullptr && sq.m_len > 0 && tile0 == 0) {
@@ -1087,18 +1100,19 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
         __threadfence();
         ms.convert = done;
       }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (ms.convert) a4_convert_scores(p, seq, min(sq.k_end, p.seqlen_max), 256);
+      asm volatile("bar.sync 1, 512;" ::: "memory");
+      if (ms.convert) a4_convert_scores(p, seq, min(sq.k_end, p.seqlen_max), 512);
     }
-  } else if (warp < 8 + kMnConv) {
+  } else if (warp < kMnSoft + kMnConv) {
     // ---------------------------------------------------- conversion ----
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMnRegsConv));
     MnTile c;
     for (int tile = tile0; tile < n_tiles && mn_tile(p, sq, tile, c); tile += p.chunks) {
       const int first = c.first, n_pages = c.n_pages, n_kt = c.n_kt;
-      if (c.with_scores && warp < 12) {
+      if (c.with_scores && warp < kMnSoft + 4) {
         // rows 120 .. 122: the sum of the masked rows over rows and heads, in
         // three fp16 parts; rows 123 .. 127 zero.  Thread = dim.
-        const int d = threadIdx.x - 256;
+        const int d = threadIdx.x - 32 * kMnSoft;
         float acc = 0.f;
         const int n = sq.m_len * p.group;
 #pragma unroll 8
@@ -1106,7 +1120,7 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
         float mag = fabsf(acc) <= 3.4e38f ? fabsf(acc) : 3.4e38f;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) mag = fmaxf(mag, __shfl_xor_sync(0xffffffffu, mag, o));
-        if (lane == 0) ms.red[warp - 8][0] = mag;
+        if (lane == 0) ms.red[warp - kMnSoft][0] = mag;
         asm volatile("bar.sync 2, 128;" ::: "memory");
         mag = fmaxf(fmaxf(ms.red[0][0], ms.red[1][0]), fmaxf(ms.red[2][0], ms.red[3][0]));
         const int e = exponent_of(mag);
@@ -1126,7 +1140,7 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
         for (int k = 0; k < 3; ++k) {
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) part[k] += __shfl_xor_sync(0xffffffffu, part[k], o);
-          if (lane == 0) ms.red[warp - 8][1 + k] = part[k];
+          if (lane == 0) ms.red[warp - kMnSoft][1 + k] = part[k];
         }
         asm volatile("bar.sync 2, 128;" ::: "memory");
         if (d < 8) {
@@ -1144,36 +1158,37 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
       tc_fence_before();
       __syncthreads();
       tc_fence_after();
-      const bool is_v = warp >= 12;
-      const int w = warp & 3;  // piece
-      uint8_t* ring = smem + kMnRaw + (warp - 8) * (kMnRing * kMnPieceBytes);
-      uint64_t* full = ms.raw_full + (warp - 8) * kMnRing;
-      const uint8_t* cache = is_v ? p.vc : p.kc;
-      // pages of tiles 32 k .. 32 k + 31, one a lane, read ahead of their use
-      auto page_of = [&](int t) -> int {
-        const int j = 2 * t + (w >> 1);
+      // pieces in order, four a tile: this warp's are cw, cw + 6, ...
+      const int cw = (warp - kMnSoft) % (kMnConv / 2);
+      const bool is_v = warp >= kMnSoft + kMnConv / 2;
+      uint8_t* piece = smem + kMnRaw + (warp - kMnSoft) * kMnPieceBytes;
+      uint64_t* full = ms.raw_full + (warp - kMnSoft);
+      const uint8_t* cache = (is_v ? p.vc : p.kc) + static_cast<size_t>(kvh) * kI4Block;
+      const int64_t page_stride = static_cast<int64_t>(p.n_kv) * kI4Block;
+      // pages of this warp's next 32 pieces, one a lane, read ahead of their use
+      auto page_of = [&](int k) -> int {
+        const int j = (cw + 6 * k) >> 1;
         return j < n_pages ? static_cast<int>(a4_page(p, seq, first + j)) : 0;
       };
       int pages = page_of(lane);
-      auto load = [&](int t) {  // this warp's piece of tile t (the whole warp)
-        if ((t & 31) == 0 && t > 0) pages = page_of(t + lane);
-        const int page = __shfl_sync(0xffffffffu, pages, t & 31);
-        if (lane == 0 && 2 * t + (w >> 1) < n_pages) {
-          const int s = t % kMnRing;
-          const uint8_t* block = cache + (static_cast<size_t>(page) * p.n_kv + kvh) * kI4Block;
-          uint8_t* dst = ring + s * kMnPieceBytes;
-          mbar_arrive_expect_tx(&full[s], kMnPieceBytes);
-          bulk_load(dst, block + (w & 1) * (kMnPiece * kI4Row), kMnPiece * kI4Row, &full[s]);
-          bulk_load(dst + kMnPiece * kI4Row, block + kI4Codes + (w & 1) * (kMnPiece * 4), kMnPiece * 4, &full[s]);
+      auto load = [&](int k) {  // this warp's k-th piece (the whole warp)
+        if ((k & 31) == 0 && k > 0) pages = page_of(k + lane);
+        const int page = __shfl_sync(0xffffffffu, pages, k & 31);
+        const int u = cw + 6 * k;
+        if (lane == 0 && (u >> 1) < n_pages) {
+          const uint8_t* block = cache + page * page_stride;
+          mbar_arrive_expect_tx(full, kMnPieceBytes);
+          bulk_load(piece, block + (u & 1) * (kMnPiece * kI4Row), kMnPiece * kI4Row, full);
+          bulk_load(piece + kMnPiece * kI4Row, block + kI4Codes + (u & 1) * (kMnPiece * 4), kMnPiece * 4, full);
         }
       };
-      for (int t = 0; t < min(n_kt, kMnRing); ++t) load(t);
-      for (int t = 0; t < n_kt; ++t) {
-        const int s = t & 1, rs = t % kMnRing;
-        const int j = 2 * t + (w >> 1);
+      static_assert(kMnConv == 12, "six warps each");
+      load(0);
+      for (int k = 0; cw + 6 * k < 4 * n_kt; ++k) {
+        const int u = cw + 6 * k, t = u >> 2, w = u & 3, s = t & 1;
+        const int j = u >> 1;  // page
         const bool has = j < n_pages;
-        if (has && !mbar_wait(&full[rs], (t / kMnRing) & 1, p.status, kA4KernelId)) break;
-        const uint8_t* piece = ring + rs * kMnPieceBytes;
+        if (has && !a4_wait(full, k & 1, p.status)) break;
         const bool valid = has && (first + j) * kI4Page + (w & 1) * kMnPiece + lane < sq.k_end;
         const MnParams pm = mn_params(piece, lane, valid);
         if (is_v) {
@@ -1183,10 +1198,9 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
             mbar_arrive(&ms.ev_full[t & 7]);
           }
           // V's stage is free when P V(t - 2) is done, K's when S(t - 2) is
-          if (t >= 2 && !mbar_wait(&ms.pv_done[(t - 2) % 3], ((t - 2) / 3) & 1, p.status, kA4KernelId)) break;
-          mn_convert<true>(piece, smem + kMnV + s * 2 * kMnHalf, kMnPiece * w, lane, pm);
+          if (t >= 2 && !a4_wait(&ms.pv_done[(t - 2) % 3], ((t - 2) / 3) & 1, p.status)) break;
         } else {
-          if (t >= 2 && !mbar_wait(&ms.s_full[(t - 2) % 3], ((t - 2) / 3) & 1, p.status, kA4KernelId)) break;
+          if (t >= 2 && !a4_wait(&ms.s_full[(t - 2) % 3], ((t - 2) / 3) & 1, p.status)) break;
           if (lane == 0) ms.ek[t & 7][w] = pm.e;
           const float bh = __half2float(__float2half_rn(pm.base));
           uint8_t* kx = smem + kMnKx + s * kMnExt;
@@ -1194,12 +1208,13 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
           *reinterpret_cast<uint4*>(ext_chunk(kx, kMnPiece * w + lane, 0)) =
               make_uint4(hh, ll, pack_f16x2(bh, valid ? 0.f : -INFINITY), 0);
           *reinterpret_cast<uint4*>(ext_chunk(kx, kMnPiece * w + lane, 1)) = make_uint4(0, 0, 0, 0);
-          mn_convert<false>(piece, smem + kMnK + s * 2 * kMnHalf, kMnPiece * w, lane, pm);
         }
+        mn_convert(piece, smem + (is_v ? kMnV : kMnK) + s * 2 * kMnHalf, kMnPiece * w, lane, pm.step,
+                   is_v ? pack_f16x2(pm.base, pm.base) : 0u);
         fence_proxy_async_smem();
         __syncwarp();  // (and every lane has read the raw stage)
         if (lane == 0) mbar_arrive(is_v ? &ms.v_full[s] : &ms.k_full[s]);
-        if (t + kMnRing < n_kt) load(t + kMnRing);
+        load(k + 1);
       }
       tc_fence_before();
       __syncthreads();
@@ -1207,6 +1222,7 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
     }
   } else {
     // ----------------------------------------------------------- MMA ----
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMnRegsMisc));
     MnTile c;
     for (int tile = tile0; tile < n_tiles && mn_tile(p, sq, tile, c); tile += p.chunks) {
       const int n_kt = c.n_kt;
@@ -1214,7 +1230,7 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
       __syncthreads();
       tc_fence_after();
       const uint32_t tmem = ms.tmem;
-        if (lane == 0) {
+        if (warp == 28 && lane == 0) {
           constexpr uint32_t idesc_s = umma_idesc_f16(128, kMnKeys);
           constexpr uint32_t idesc_pv = umma_idesc_f16(128, kA4HeadDim) | kUmmaBMajorMN;
           const uint64_t dq[2] = {umma_desc_kmajor_sw128(smem_u32(smem + kMnQ)),
@@ -1222,14 +1238,14 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
           const uint64_t dqx = umma_desc_kmajor_sw32(smem_u32(smem + kMnQx));
           auto pv = [&](int t) -> bool {
             const int s = t & 1, slot = t % 3;
-            if (!mbar_wait(&ms.p_full[slot], (t / 3) & 1, p.status, kA4KernelId) ||
-                !mbar_wait(&ms.v_full[s], (t >> 1) & 1, p.status, kA4KernelId))
+            if (!a4_wait(&ms.p_full[slot], (t / 3) & 1, p.status) ||
+                !a4_wait(&ms.v_full[s], (t >> 1) & 1, p.status))
               return false;
             tc_fence_after();
             const uint64_t dv = umma_desc_mnmajor_sw128(smem_u32(smem + kMnV + s * 2 * kMnHalf), kMnHalf);
 #pragma unroll
             for (int kk = 0; kk < kMnKeys / 16; ++kk)
-              umma_f16_ts(tmem, tmem + 128 + 128 * slot + 8 * kk, dv + (kk * 2048 >> 4), idesc_pv,
+              umma_f16_ts(tmem, tmem + 128 + 128 * slot + 8 * kk + (kk & 4) * 8, dv + (kk * 2048 >> 4), idesc_pv,
                           (t > 0 || kk > 0) ? 1u : 0u);
             umma_commit(&ms.pv_done[slot]);
             return true;
@@ -1238,8 +1254,8 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
           for (int t = 0; t < n_kt && ok; ++t) {
             const int s = t & 1, slot = t % 3;
             // S(t) goes over P(t - 3), which P V(t - 3) has read
-            ok = mbar_wait(&ms.k_full[s], (t >> 1) & 1, p.status, kA4KernelId) &&
-                 (t < 3 || mbar_wait(&ms.pv_done[slot], (t / 3 - 1) & 1, p.status, kA4KernelId));
+            ok = a4_wait(&ms.k_full[s], (t >> 1) & 1, p.status) &&
+                 (t < 3 || a4_wait(&ms.pv_done[slot], (t / 3 - 1) & 1, p.status));
             if (!ok) break;
             tc_fence_after();
             const uint32_t kst = smem_u32(smem + kMnK + s * 2 * kMnHalf);
@@ -1257,7 +1273,7 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
           if (ok) pv(n_kt - 1);
           // every arrival of the tensor cores is in before the barriers go
           umma_commit(&ms.mma_done);
-          mbar_wait(&ms.mma_done, 0, p.status, kA4KernelId);
+          a4_wait(&ms.mma_done, 0, p.status);
         }
       __syncwarp();
       tc_fence_before();
@@ -1267,7 +1283,7 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 16) {
+  if (warp == 28) {
     tc_fence_after();
     tmem_dealloc(ms.tmem, 512);
   }
