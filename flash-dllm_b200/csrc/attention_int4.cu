@@ -550,7 +550,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_int4_few_kernel(const A4P
 // passes from tile to tile through shared memory right after a tile's maximum
 // is known, so the exponentials of consecutive tiles overlap.  Tensor memory:
 // O and three S tiles with P over them: S(t) is issued two tiles ahead of P
-// V(t).
+// V(t).  Warp 29 works out V's exponents ahead of V's conversion.
 // Key ranges are split over CTAs as in the other kernel.
 // ---------------------------------------------------------------------------
 constexpr int kMnThreads = 1024;
@@ -619,6 +619,25 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+// pairs of fp32 in one instruction
+__device__ __forceinline__ uint64_t pack_f32x2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpack_f32x2(uint64_t v, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 // maximum of 32 values
 __device__ __forceinline__ float mn_max32(const float (&v)[32]) {
   float a[4] = {v[0], v[1], v[2], v[3]};
@@ -663,13 +682,17 @@ struct MnParams {
   float base;        // normalised, fp32
   int e;             // exponent of the piece
 };
-__device__ __forceinline__ MnParams mn_params(const uint8_t* piece, int lane, bool valid) {
-  MnParams r;
-  const uint32_t pr = valid ? reinterpret_cast<const uint32_t*>(piece + kMnPiece * kI4Row)[lane] : 0u;
+// exponent of the largest value of the warp's 32 groups
+__device__ __forceinline__ int mn_exponent(uint32_t pr) {
   const float step = __uint_as_float(pr << 16), low = __uint_as_float(pr & 0xffff0000u);
   const float mag = fmaxf(fabsf(low), fabsf(fmaf(15.f, step, low)));
   // (a NaN group says nothing about the others' size)
-  r.e = __reduce_max_sync(0xffffffffu, mag <= 3.4e38f ? exponent_of(mag) : -100);
+  return __reduce_max_sync(0xffffffffu, mag <= 3.4e38f ? exponent_of(mag) : -100);
+}
+__device__ __forceinline__ MnParams mn_params(uint32_t pr) {
+  MnParams r;
+  r.e = mn_exponent(pr);
+  const float step = __uint_as_float(pr << 16), low = __uint_as_float(pr & 0xffff0000u);
   const float s = pow2i(-r.e);
   r.step = pack_f16x2(step * s, step * s);
   r.base = fmaf(8.f, step, low) * s;
@@ -679,21 +702,28 @@ __device__ __forceinline__ MnParams mn_params(const uint8_t* piece, int lane, bo
 // The warp's 32 keys of a K or V block into a tile (rows row0 ..): lane ->
 // key 8 i + lane / 4, 16 bytes of codes = 32 dims, four 16-byte chunks out.
 // The lanes of dims 64 .. 127 take their words in another order, so that a
-// quarter-warp's stores fall into different banks.
-// K: base 0.
-__device__ __forceinline__ void mn_convert(const uint8_t* piece, uint8_t* tile, int row0, int lane, uint32_t step_n,
-                                           uint32_t base_n) {
+// quarter-warp's stores fall into different banks.  The codes are taken into
+// registers first: the next piece's copy is under way while they are converted.
+__device__ __forceinline__ void mn_codes(const uint8_t* piece, int lane, uint2 (&a)[4], uint2 (&b)[4]) {
+  const int swap = ((lane & 3) >> 1) << 3;
+  const uint8_t* src = piece + (lane >> 2) * kI4Row + 16 * (lane & 3);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    a[i] = *reinterpret_cast<const uint2*>(src + i * 8 * kI4Row + swap);
+    b[i] = *reinterpret_cast<const uint2*>(src + i * 8 * kI4Row + (swap ^ 8));
+  }
+}
+// value = (code - 8) * step + base; K: base 0
+__device__ __forceinline__ void mn_convert(const uint2 (&a)[4], const uint2 (&b)[4], uint8_t* tile, int row0, int lane,
+                                           uint32_t step_n, uint32_t base_n) {
   const int q = lane & 3, r = lane >> 2;
-  const int swap = (q >> 1) << 3;
-  const uint8_t* src = piece + r * kI4Row + 16 * q;
   uint8_t* dst = tile + (q >> 1) * kMnHalf + (row0 + r) * 128;  // (row0 a multiple of 8)
   int off[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) off[j] = (((q & 1) * 4 + (j ^ (swap >> 2))) ^ r) << 4;
-#pragma unroll 1
+  for (int j = 0; j < 4; ++j) off[j] = (((q & 1) * 4 + (j ^ (q & 2))) ^ r) << 4;
+#pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint2 a = *reinterpret_cast<const uint2*>(src + swap), b = *reinterpret_cast<const uint2*>(src + (swap ^ 8));
-    const uint32_t v[4] = {a.x, a.y, b.x, b.y};
+    const uint32_t v[4] = {a[i].x, a[i].y, b[i].x, b[i].y};
     const uint32_t step = __shfl_sync(0xffffffffu, step_n, 8 * i + r);
     const uint32_t base = __shfl_sync(0xffffffffu, base_n, 8 * i + r);
 #pragma unroll
@@ -702,10 +732,8 @@ __device__ __forceinline__ void mn_convert(const uint8_t* piece, uint8_t* tile, 
       uint32_t o[4] = {i4_even_f16(v[j]), i4_odd_f16(v[j]), i4_even_f16(hi), i4_odd_f16(hi)};
 #pragma unroll
       for (int k = 0; k < 4; ++k) o[k] = fma_f16x2(o[k], step, base);
-      *reinterpret_cast<uint4*>(dst + off[j]) = make_uint4(o[0], o[1], o[2], o[3]);
+      *reinterpret_cast<uint4*>(dst + i * 8 * 128 + off[j]) = make_uint4(o[0], o[1], o[2], o[3]);
     }
-    src += 8 * kI4Row;
-    dst += 8 * 128;
   }
 }
 
@@ -743,8 +771,8 @@ struct MnMisc {
   uint64_t k_full[2], v_full[2], s_full[3], p_full[3], pv_done[3], m_ready[4][2], r_ready[4][4], mma_done;
   uint32_t tmem;
   int32_t last, convert;
-  // [tile % 8][32-key piece]: a conversion warp that writes tile t's has seen
-  // S(t - 2), so P V(t - 5), so the softmax of every tile up to t - 5
+  // [tile % 8][32-key piece]: who writes tile t's has seen S(t - 2), so P V(t - 5),
+  // so the softmax of every tile up to t - 5
   alignas(16) int32_t ek[8][4];
   alignas(16) int32_t ev[8][4];
   float red[4][8];                  // score rows: warp partials
@@ -814,9 +842,13 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
     for (int tile = tile0; tile < n_tiles && mn_tile(p, sq, tile, c); tile += p.chunks) {
       const int first = c.first, n_splits = c.n_splits, n_kt = c.n_kt, m0 = c.m0, rows = c.rows;
       const bool with_scores = c.with_scores;
+      // Warps of 32 tile rows: those beyond the rows have nothing to do, the
+      // last one at least takes the score rows' logits.
+      const int row_warps = (rows + 31) / 32;
+      const int p_warps = 2 * (row_warps + (with_scores && row_warps < 4 ? 1 : 0));
       if (threadIdx.x == 0) {
         for (int s = 0; s < kMnConv; ++s) mbar_init(&ms.raw_full[s], 1);
-        for (int s = 0; s < 8; ++s) mbar_init(&ms.ev_full[s], 4);
+        for (int s = 0; s < 8; ++s) mbar_init(&ms.ev_full[s], 1);
         for (int s = 0; s < 2; ++s) {
           mbar_init(&ms.k_full[s], 4);
           mbar_init(&ms.v_full[s], 4);
@@ -828,7 +860,7 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
         }
         for (int s = 0; s < 3; ++s) {
           mbar_init(&ms.s_full[s], 1);
-          mbar_init(&ms.p_full[s], 8);
+          mbar_init(&ms.p_full[s], p_warps);
           mbar_init(&ms.pv_done[s], 1);
         }
         mbar_init(&ms.mma_done, 1);
@@ -897,8 +929,9 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
       const bool score_warp = with_scores && (warp & 3) == 3;
       const float log_mul = score_row ? 0.f : row_mul * p.scale_log2;
       float ref_l = -INFINITY, l = 0.f;  // the sum of 2^(logit - ref_l + kMnRaise) over this group's keys
+      const bool soft = (warp & 3) < row_warps;
       bool ok = true, range_ok = true;
-      for (int t = par; t < n_kt; t += 2) {
+      for (int t = soft || score_warp ? par : n_kt; t < n_kt; t += 2) {
         const int slot = t % 3;
         const uint32_t ts = tmem + 128 + 128 * slot + tl;
         ok = a4_wait(&ms.s_full[slot], (t / 3) & 1, p.status) && a4_wait(&ms.ev_full[t & 7], (t >> 3) & 1, p.status);
@@ -922,10 +955,13 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
           }
           mt = fmaxf(mt, fmaf(mn_max32(v), log_mul * k, static_cast<float>(ms.ev[t & 7][g])));
         }
-        ms.mx[t & 3][hk][r] = mt;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ms.m_ready[warp & 3][par]);
+        if (soft) {
+          ms.mx[t & 3][hk][r] = mt;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ms.m_ready[warp & 3][par]);
+        }
         if (score_warp) {
+          __syncwarp();
           const int n0 = first * kI4Page + t * kMnKeys + 64 * hk;
           unsigned long long* acc = p.score_acc + static_cast<int64_t>(seq) * p.seqlen_max + n0;
 #pragma unroll
@@ -935,6 +971,11 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
               a4_add_score(acc + n, ms.score[grp][0][n] + ms.score[grp][1][n] + ms.score[grp][2][n], range_ok);
           }
           __syncwarp();
+        }
+        if (!soft) {
+          tc_fence_before();
+          if (lane == 0) mbar_arrive(&ms.p_full[slot]);  // S is read
+          continue;
         }
         // the reference after the tile before, moved if this tile passes it
         // (both key halves decide the same)
@@ -978,17 +1019,21 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
           const int ev = ms.ev[t & 7][g];
           const float shift = base + static_cast<float>(ev);
           const float mul = log_mul * pow2i(ms.ek[t & 7][g]);
-          float ps[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint64_t shift2 = pack_f32x2(shift, shift), mul2 = pack_f32x2(mul, mul);
+          uint64_t ps[2] = {0ull, 0ull};  // (zero pairs)
           uint32_t pw[16];
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
-            const float x = ex2_approx(fmaf(v[j], mul, shift));
-            const float y = ex2_approx(fmaf(v[j + 1], mul, shift));
-            ps[j & 3] += x;
-            ps[(j + 1) & 3] += y;
+            float x, y;
+            unpack_f32x2(fma_f32x2(pack_f32x2(v[j], v[j + 1]), mul2, shift2), x, y);
+            x = ex2_approx(x);
+            y = ex2_approx(y);
+            ps[(j >> 1) & 1] = add_f32x2(ps[(j >> 1) & 1], pack_f32x2(x, y));
             pw[j >> 1] = pack_f16x2(x, y);
           }
-          l = fmaf((ps[0] + ps[1]) + (ps[2] + ps[3]), pow2i(-ev), l);
+          float x, y;
+          unpack_f32x2(add_f32x2(ps[0], ps[1]), x, y);
+          l = fmaf(x + y, pow2i(-ev), l);
           // P of keys 0 .. 63 in columns 0 .. 31, of keys 64 .. 127 in columns
           // 64 .. 95: either half writes over logits of its own that it has read
           tmem_st_32x32b_x16(ts + 64 * hk + 16 * (g & 1), pw);
@@ -1189,14 +1234,13 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
         const int j = u >> 1;  // page
         const bool has = j < n_pages;
         if (has && !a4_wait(full, k & 1, p.status)) break;
-        const bool valid = has && (first + j) * kI4Page + (w & 1) * kMnPiece + lane < sq.k_end;
-        const MnParams pm = mn_params(piece, lane, valid);
+        const bool valid = has && (first + j) * kI4Page + (u & 1) * kMnPiece + lane < sq.k_end;
+        const MnParams pm = mn_params(valid ? reinterpret_cast<const uint32_t*>(piece + kMnPiece * kI4Row)[lane] : 0u);
+        uint2 ca[4], cb[4];
+        mn_codes(piece, lane, ca, cb);
+        __syncwarp();  // every lane has read the piece
+        load(k + 1);
         if (is_v) {
-          // (the exponents go out before V's stage is free: P needs them)
-          if (lane == 0) {
-            ms.ev[t & 7][w] = pm.e;
-            mbar_arrive(&ms.ev_full[t & 7]);
-          }
           // V's stage is free when P V(t - 2) is done, K's when S(t - 2) is
           if (t >= 2 && !a4_wait(&ms.pv_done[(t - 2) % 3], ((t - 2) / 3) & 1, p.status)) break;
         } else {
@@ -1209,12 +1253,11 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
               make_uint4(hh, ll, pack_f16x2(bh, valid ? 0.f : -INFINITY), 0);
           *reinterpret_cast<uint4*>(ext_chunk(kx, kMnPiece * w + lane, 1)) = make_uint4(0, 0, 0, 0);
         }
-        mn_convert(piece, smem + (is_v ? kMnV : kMnK) + s * 2 * kMnHalf, kMnPiece * w, lane, pm.step,
+        mn_convert(ca, cb, smem + (is_v ? kMnV : kMnK) + s * 2 * kMnHalf, kMnPiece * w, lane, pm.step,
                    is_v ? pack_f16x2(pm.base, pm.base) : 0u);
         fence_proxy_async_smem();
-        __syncwarp();  // (and every lane has read the raw stage)
+        __syncwarp();
         if (lane == 0) mbar_arrive(is_v ? &ms.v_full[s] : &ms.k_full[s]);
-        load(k + 1);
       }
       tc_fence_before();
       __syncthreads();
@@ -1230,47 +1273,91 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
       __syncthreads();
       tc_fence_after();
       const uint32_t tmem = ms.tmem;
+      if (warp == 29) {
+        // the exponents of V's pieces, ahead of their conversion: P needs
+        // them while V's stage is not free yet
+        const int first = c.first, n_pages = c.n_pages;
+        const uint8_t* pairs = p.vc + static_cast<size_t>(kvh) * kI4Block + kI4Codes + lane * 4;
+        const int64_t page_stride = static_cast<int64_t>(p.n_kv) * kI4Block;
+        // pages 32 k .. 32 k + 31, one a lane; a tile's parameters are read
+        // while the tile before waits
+        auto page_of = [&](int j) -> int { return j < n_pages ? static_cast<int>(a4_page(p, seq, first + j)) : 0; };
+        int pages = page_of(lane);
+        uint32_t pr[4];
+        auto read = [&](int t) {
+          if (((2 * t) & 31) == 0 && t > 0) pages = page_of(2 * t + lane);
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int j = 2 * t + (g >> 1);
+            const int page = __shfl_sync(0xffffffffu, pages, j & 31);
+            const bool valid = j < n_pages && (first + j) * kI4Page + (g & 1) * kMnPiece + lane < sq.k_end;
+            pr[g] = valid ? __ldg(reinterpret_cast<const uint32_t*>(pairs + page * page_stride + (g & 1) * kMnPiece * 4))
+                          : 0u;
+          }
+        };
+        read(0);
+        for (int t = 0; t < n_kt; ++t) {
+          int e[4];
+#pragma unroll
+          for (int g = 0; g < 4; ++g) e[g] = mn_exponent(pr[g]);
+          if (t + 1 < n_kt) read(t + 1);
+          // (the slot of tile t - 8 is free: S(t) comes after P V(t - 3).  No
+          // earlier phase would do: it must not pass before this wait sees it)
+          if (!a4_wait(&ms.s_full[t % 3], (t / 3) & 1, p.status)) break;
+          if (lane == 0) {
+            *reinterpret_cast<int4*>(ms.ev[t & 7]) = make_int4(e[0], e[1], e[2], e[3]);
+            mbar_arrive(&ms.ev_full[t & 7]);
+          }
+        }
+      }
         if (warp == 28 && lane == 0) {
           constexpr uint32_t idesc_s = umma_idesc_f16(128, kMnKeys);
           constexpr uint32_t idesc_pv = umma_idesc_f16(128, kA4HeadDim) | kUmmaBMajorMN;
           const uint64_t dq[2] = {umma_desc_kmajor_sw128(smem_u32(smem + kMnQ)),
                                   umma_desc_kmajor_sw128(smem_u32(smem + kMnQ + kMnHalf))};
           const uint64_t dqx = umma_desc_kmajor_sw32(smem_u32(smem + kMnQx));
-          auto pv = [&](int t) -> bool {
-            const int s = t & 1, slot = t % 3;
-            if (!a4_wait(&ms.p_full[slot], (t / 3) & 1, p.status) ||
-                !a4_wait(&ms.v_full[s], (t >> 1) & 1, p.status))
-              return false;
-            tc_fence_after();
-            const uint64_t dv = umma_desc_mnmajor_sw128(smem_u32(smem + kMnV + s * 2 * kMnHalf), kMnHalf);
+          // Whichever of the next P V and the next S is ready goes first (P V,
+          // when both are): issued in a fixed order, each would wait for the
+          // tail of the one before it.
+          int ns = 0, np = 0;  // the next S and P V
+          int idle = 0;
+          while (np < n_kt) {
+            if (np < ns && mbar_test(&ms.p_full[np % 3], (np / 3) & 1) && mbar_test(&ms.v_full[np & 1], (np >> 1) & 1)) {
+              tc_fence_after();
+              const int slot = np % 3;
+              const uint64_t dv = umma_desc_mnmajor_sw128(smem_u32(smem + kMnV + (np & 1) * 2 * kMnHalf), kMnHalf);
 #pragma unroll
-            for (int kk = 0; kk < kMnKeys / 16; ++kk)
-              umma_f16_ts(tmem, tmem + 128 + 128 * slot + 8 * kk + (kk & 4) * 8, dv + (kk * 2048 >> 4), idesc_pv,
-                          (t > 0 || kk > 0) ? 1u : 0u);
-            umma_commit(&ms.pv_done[slot]);
-            return true;
-          };
-          bool ok = true;
-          for (int t = 0; t < n_kt && ok; ++t) {
-            const int s = t & 1, slot = t % 3;
-            // S(t) goes over P(t - 3), which P V(t - 3) has read
-            ok = a4_wait(&ms.k_full[s], (t >> 1) & 1, p.status) &&
-                 (t < 3 || a4_wait(&ms.pv_done[slot], (t / 3 - 1) & 1, p.status));
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t kst = smem_u32(smem + kMnK + s * 2 * kMnHalf);
-            const uint64_t dk[2] = {umma_desc_kmajor_sw128(kst), umma_desc_kmajor_sw128(kst + kMnHalf)};
+              for (int kk = 0; kk < kMnKeys / 16; ++kk)
+                umma_f16_ts(tmem, tmem + 128 + 128 * slot + 8 * kk + (kk & 4) * 8, dv + (kk * 2048 >> 4), idesc_pv,
+                            (np > 0 || kk > 0) ? 1u : 0u);
+              umma_commit(&ms.pv_done[slot]);
+              ++np;
+              idle = 0;
+            } else if (ns < n_kt && mbar_test(&ms.k_full[ns & 1], (ns >> 1) & 1) &&
+                       // S(t) goes over P(t - 3), which P V(t - 3) has read
+                       (ns < 3 || mbar_test(&ms.pv_done[ns % 3], (ns / 3 - 1) & 1))) {
+              tc_fence_after();
+              const int s = ns & 1, slot = ns % 3;
+              const uint32_t kst = smem_u32(smem + kMnK + s * 2 * kMnHalf);
+              const uint64_t dk[2] = {umma_desc_kmajor_sw128(kst), umma_desc_kmajor_sw128(kst + kMnHalf)};
 #pragma unroll
-            for (int kk = 0; kk < kA4HeadDim / 16; ++kk)
-              umma_bf16(tmem + 128 + 128 * slot, dq[kk >> 2] + 2 * (kk & 3), dk[kk >> 2] + 2 * (kk & 3), idesc_s,
-                        kk > 0 ? 1u : 0u);
-            umma_bf16(tmem + 128 + 128 * slot, dqx, umma_desc_kmajor_sw32(smem_u32(smem + kMnKx + s * kMnExt)), idesc_s,
-                      1u);
-            umma_commit(&ms.s_full[slot]);
-            if (t >= 2) ok = pv(t - 2);
+              for (int kk = 0; kk < kA4HeadDim / 16; ++kk)
+                umma_bf16(tmem + 128 + 128 * slot, dq[kk >> 2] + 2 * (kk & 3), dk[kk >> 2] + 2 * (kk & 3), idesc_s,
+                          kk > 0 ? 1u : 0u);
+              umma_bf16(tmem + 128 + 128 * slot, dqx, umma_desc_kmajor_sw32(smem_u32(smem + kMnKx + s * kMnExt)),
+                        idesc_s, 1u);
+              umma_commit(&ms.s_full[slot]);
+              ++ns;
+              idle = 0;
+            } else {
+              // (bounded by a count of polls, some tenths of a second: reading
+              // the global timer takes longer than a poll)
+              if (++idle > (1 << 24)) {
+                a4_timeout(p.status);
+                break;
+              }
+            }
           }
-          if (ok && n_kt > 1) ok = pv(n_kt - 2);
-          if (ok) pv(n_kt - 1);
           // every arrival of the tensor cores is in before the barriers go
           umma_commit(&ms.mma_done);
           a4_wait(&ms.mma_done, 0, p.status);
