@@ -132,36 +132,57 @@ __device__ __forceinline__ void a4_convert_scores(const A4Params& p, int seq, in
 // Few rows: mma.sync with keys in the M dimension.
 //
 // A warp takes one page of one head at a time: S^T = K Q^T as four 16-key x
-// 8-row tiles, O^T += V^T P^T as eight 16-dim x 8-row tiles, so a chunk is 8
-// query rows (rows x heads of the group, in that order) and no instruction is
-// spent on padding up to 64 or 128 of them.  K codes go from shared memory to
-// A fragments with one 16-byte load per lane and key (a lane's four words are
-// 32 consecutive dims: the sum over dims may take them in any order, so the
-// query fragments are laid out to match), V codes with one 8-byte load per
-// lane and key (a lane owns 16 consecutive dims of O).  P^T becomes the B
-// operand by one 8x8 transpose per tile.  Bound by the cache bytes (136 per
-// token and head) and, close behind, by the issue slots of the conversion to
-// bf16 (11 instructions per 8 codes).
+// 8-row tiles, O^T += V^T P^T as eight 16-dim x 8-row tiles, so a chunk is up
+// to 8 query rows (rows x heads of the group, in that order) and no
+// instruction is spent on padding up to 64 or 128 of them.  K codes go from
+// shared memory to A fragments with one 16-byte load per lane and key (a
+// lane's four words are 32 consecutive dims: the sum over dims may take them in
+// any order, so the query fragments are laid out to match), V codes with one
+// 8-byte load per lane and key (a lane owns 16 consecutive dims of O).  P^T
+// becomes the B operand by one 8x8 transpose per tile.
+//
+// The codes are operands as they lie: a masked nibble at the foot of a half
+// word is the fp16 subnormal code * 2^-24, one nibble higher it is code *
+// 2^-20, and products with subnormals are exact.  Eight codes cost five
+// instructions (a shift, four masks).  The other operands are fp16 then: a
+// query row is divided by a power of two (and every second pair of dims by 16
+// more) so that its largest value lies in [2^13, 2^14), which drops what is
+// 2^-37 of it; p_n s_n is taken relative to the largest p_n v_n so far, v being
+// the power of two at the largest value of a page (so 2^-39 of it is dropped,
+// and the rest is rounded by 2^-12).
 //
 // The eight warps of a CTA take pages round robin, each with its own ring of
-// bulk copies and its own running maximum, and are joined in shared memory.
+// three blocks (K and V of a page in turn) filled by bulk copies and its own
+// running maximum, and are joined in shared memory.  Two CTAs share an SM.
 // Long key ranges are split over CTAs; the last one to finish joins the
 // partial results in split order, so the result does not depend on timing.
+//
+// kE: logit columns of a lane that are used.  A fragment's lane holds columns
+// 2 t and 2 t + 1; with up to four rows they all go to the even columns, and
+// the softmax is half the instructions.
 // ---------------------------------------------------------------------------
 constexpr int kFewWarps = 8;
 constexpr int kFewThreads = kFewWarps * 32;
+constexpr int kFewCtas = 2;   // per SM
 constexpr int kFewStages = 3;
-constexpr int kFewRows = 8;  // rows x group heads of a chunk
-constexpr int kFewStageBytes = 2 * kI4Block;
-constexpr int kFewRing = kFewWarps * kFewStages * kFewStageBytes;
+constexpr int kFewRows = 8;   // rows x group heads of a chunk, at most
+constexpr int kFewRing = kFewWarps * kFewStages * kI4Block;
 constexpr int kFewPartFloats = kFewRows * kA4HeadDim + 2 * kFewRows;
-constexpr int kFewSmem = kFewRing + 512;
-static_assert(kFewSmem <= 227 * 1024, "shared memory");
+constexpr int kFewSmem = kFewRing + kFewWarps * kFewStages * 8;
+static_assert(kFewCtas * (kFewSmem + 2048) <= 228 * 1024, "shared memory");
 static_assert(kFewWarps * kFewPartFloats * 4 <= kFewRing, "the warps' results fit the ring");
+constexpr int kFewRaise = 18;  // p s 2^(18 - ev) < 2^15: a step is below 2^(ev + 1) / 16
 
-__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+// 2^e for |e| <= 126
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((127 + e) << 23); }
+// exponent of a magnitude, held to what pow2i takes (0 and denormals: the least)
+__device__ __forceinline__ int exponent_of(float mag) {
+  const int e = static_cast<int>((__float_as_uint(mag) >> 23) & 255u) - 127;
+  return max(-100, min(e, 126));
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -170,13 +191,24 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 
-__global__ void __launch_bounds__(kFewThreads, 1) attn_int4_few_kernel(const A4Params p) {
+template <int kE>
+__global__ void __launch_bounds__(kFewThreads, kFewCtas) attn_int4_few_kernel(const A4Params p) {
+  constexpr int kRows = 4 * kE;
   extern __shared__ __align__(128) uint8_t smem[];
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kFewRing);  // [warps][stages]
   __shared__ int s_last, s_convert;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + kFewRing) + warp * kFewStages;
+  uint8_t* ring = smem + warp * (kFewStages * kI4Block);
+  if (lane == 0)
+    for (int s = 0; s < kFewStages; ++s) mbar_init(&bar[s], 1);
+  if (threadIdx.x == 0) s_convert = -1;
+  fence_barrier_init();
   pdl_wait();
   pdl_launch_dependents();
   const int item_id = blockIdx.x / p.chunks;
@@ -190,17 +222,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_int4_few_kernel(const A4P
   int n_splits = (seq_pages + p.split_pages - 1) / p.split_pages;
   const int cta_splits = n_splits;
   const bool scores_on = p.scores != nullptr && it.m_len > 0 && it.mchunk >= 0;
-  uint8_t* ring = smem + warp * (kFewStages * kFewStageBytes);
-  uint64_t* bar = bars + warp * kFewStages;
-  if (lane == 0)
-    for (int s = 0; s < kFewStages; ++s) mbar_init(&bar[s], 1);
-  if (threadIdx.x == 0) s_convert = -1;
-  fence_barrier_init();
   __syncthreads();
 
   const int m_all = it.rows * p.group;
-  const int n_chunks = (m_all + kFewRows - 1) / kFewRows;
-  uint32_t use = 0;  // ring uses of this warp so far
+  const int n_chunks = (m_all + kRows - 1) / kRows;
+  int slot = 0;           // of the next block to be read
+  uint32_t parity = 0;    // of its barrier
   bool range_ok = true;
   for (int chunk = blockIdx.x % p.chunks; chunk < n_chunks; chunk += p.chunks) {
     int n_pages = min(p.split_pages, seq_pages - first);  // of this CTA
@@ -213,59 +240,105 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_int4_few_kernel(const A4P
       n_splits = 1;
     }
     const int n_mine = n_pages > warp ? (n_pages - warp + kFewWarps - 1) / kFewWarps : 0;  // of this warp
-    auto load = [&](int j) {  // the warp's j-th page of this chunk (one lane)
-      const uint32_t s = (use + j) % kFewStages;
-      const int64_t page = a4_page(p, it.seq, first + warp + j * kFewWarps);
-      const size_t off = (static_cast<size_t>(page) * p.n_kv + kvh) * kI4Block;
-      mbar_arrive_expect_tx(&bar[s], kFewStageBytes);
-      bulk_load(ring + s * kFewStageBytes, p.kc + off, kI4Block, &bar[s]);
-      bulk_load(ring + s * kFewStageBytes + kI4Block, p.vc + off, kI4Block, &bar[s]);
+    // block b of the warp: K (even) or V (odd) of its page b / 2, into slot s;
+    // the pages of the next 32 are looked up by the lanes at once
+    int64_t ids = 0;
+    auto load = [&](int b, int s) {
+      const int j = b >> 1;
+      if ((b & 63) == 0 && j + lane < n_mine) ids = a4_page(p, it.seq, first + warp + (j + lane) * kFewWarps);
+      const int64_t page = __shfl_sync(0xffffffffu, ids, j & 31);
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&bar[s], kI4Block);
+        bulk_load(ring + s * kI4Block, ((b & 1) ? p.vc : p.kc) + (page * p.n_kv + kvh) * kI4Block, kI4Block, &bar[s]);
+      }
     };
-    if (lane == 0)
-      for (int j = 0; j < min(n_mine, kFewStages); ++j) load(j);
-
-    // query fragments: row g of the chunk, dims 32 t .. 32 t + 31
-    uint32_t qf[16];
     {
-      const int m = chunk * kFewRows + g;
+      int s = slot;
+      for (int b = 0; b < min(2 * n_mine, kFewStages); ++b) {
+        load(b, s);
+        s = s == kFewStages - 1 ? 0 : s + 1;
+      }
+    }
+
+    // query fragments: column g of the tile, dims 32 t .. 32 t + 31
+    uint32_t qf[16];
+    float qs = 0.f, qmax = 0.f;  // sum and largest magnitude of the row
+    {
+      const int mr = kE == 2 ? g : g >> 1;
+      const int m = chunk * kRows + mr;
+      const bool have = m < m_all && (kE == 2 || (g & 1) == 0);
+      const int mm = min(m, m_all - 1);
       const uint4* src = reinterpret_cast<const uint4*>(
-          p.q + (static_cast<int64_t>(a4_row(it, min(m, m_all - 1) / p.group)) * p.n_heads + kvh * p.group +
-                 min(m, m_all - 1) % p.group) * kA4HeadDim + 32 * t);
+          p.q + (static_cast<int64_t>(a4_row(it, mm / p.group)) * p.n_heads + kvh * p.group + mm % p.group) * kA4HeadDim +
+          32 * t);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint4 v = m < m_all ? src[j] : make_uint4(0, 0, 0, 0);
+        const uint4 v = have ? src[j] : make_uint4(0, 0, 0, 0);
         qf[4 * j] = v.x;
         qf[4 * j + 1] = v.y;
         qf[4 * j + 2] = v.z;
         qf[4 * j + 3] = v.w;
       }
     }
-    float qs = 0.f;  // sum of row g
+    bool fin = true;
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
       const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&qf[j]));
       qs += f.x + f.y;
+      fin = fin && fabsf(f.x) <= 3.4e38f && fabsf(f.y) <= 3.4e38f;
+      qmax = fmaxf(qmax, fmaxf(fabsf(f.x), fabsf(f.y)));
     }
-    qs += __shfl_xor_sync(0xffffffffu, qs, 1);
-    qs += __shfl_xor_sync(0xffffffffu, qs, 2);
-    const float qsum[2] = {__shfl_sync(0xffffffffu, qs, 8 * t), __shfl_sync(0xffffffffu, qs, 8 * t + 4)};
-    // this lane's two rows: 2 t, 2 t + 1 of the chunk; masked ones count into the scores
-    bool is_m[2];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) is_m[e] = chunk * kFewRows + 2 * t + e < it.m_len * p.group;
-    const bool chunk_scores = scores_on && chunk * kFewRows < it.m_len * p.group;
+    for (int o = 1; o < 4; o <<= 1) {
+      qs += __shfl_xor_sync(0xffffffffu, qs, o);
+      qmax = fmaxf(qmax, __shfl_xor_sync(0xffffffffu, qmax, o));
+    }
+    // a query with a NaN or an infinity has no weights: NaN through the base's term
+    if (__shfl_xor_sync(0xffffffffu, fin ? 0 : 1, 1) | __shfl_xor_sync(0xffffffffu, fin ? 0 : 1, 2) |
+        __shfl_xor_sync(0xffffffffu, fin ? 0 : 1, 3) | (fin ? 0 : 1))
+      qs = __int_as_float(0x7fc00000);
+    const int eq = min(exponent_of(qmax) - 13, 102);  // (2^(24 + eq) is a number)
+    {
+      const float down = pow2i(-eq), down16 = down * 0.0625f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&qf[j]));
+        const float d = (j & 1) ? down16 : down;
+        qf[j] = pack_half2(f.x * d, f.y * d);
+      }
+    }
+    // logits are kept divided by 2^(24 + eq)
+    const float qsn = qs * pow2i(-max(min(eq + 24, 126), -126));
+    float qsum[kE], up[kE], mul[kE];
+#pragma unroll
+    for (int e = 0; e < kE; ++e) {
+      qsum[e] = __shfl_sync(0xffffffffu, qsn, 8 * t + 4 * e);
+      up[e] = pow2i(24 + __shfl_sync(0xffffffffu, eq, 8 * t + 4 * e));
+      mul[e] = up[e] * p.scale_log2;
+    }
+    // this lane's rows of the chunk; masked ones count into the scores
+    bool is_m[kE];
+#pragma unroll
+    for (int e = 0; e < kE; ++e) is_m[e] = chunk * kRows + kE * t + e < it.m_len * p.group;
+    const bool chunk_scores = scores_on && chunk * kRows < it.m_len * p.group;
 
     float acc[8][4];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
-    float mx[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, pb[2] = {0.f, 0.f};
+    float mx[kE], l[kE], pb[kE];  // reference, sum, bases' part of O
+#pragma unroll
+    for (int e = 0; e < kE; ++e) {
+      mx[e] = -INFINITY;
+      l[e] = 0.f;
+      pb[e] = 0.f;
+    }
+    bool live = true;
     for (int j = 0; j < n_mine; ++j) {
-      const uint32_t s = (use + j) % kFewStages;
-      if (!mbar_wait(&bar[s], ((use + j) / kFewStages) & 1, p.status, kA4KernelId)) break;  // (recorded)
-      const uint8_t* kb = ring + s * kFewStageBytes;
-      const uint8_t* vb = kb + kI4Block;
+      live = live && mbar_wait(&bar[slot], parity, p.status, kA4KernelId);  // (recorded)
+      if (!live) break;
+      const uint8_t* kb = ring + slot * kI4Block;
       const int n0 = (first + warp + j * kFewWarps) * kI4Page;
       const bool whole = n0 + kI4Page <= it.k_end;  // uniform
       float sc[4][4];
@@ -278,88 +351,120 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_int4_few_kernel(const A4P
         const uint32_t a0[4] = {wa.x, wa.y, wa.z, wa.w}, a1[4] = {wb.x, wb.y, wb.z, wb.w};
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
-          const int sh = 8 * (ks & 1);
-          const uint32_t a[4] = {i4_pair(a0[ks >> 1] >> sh), i4_pair(a1[ks >> 1] >> sh),
-                                 i4_pair(a0[ks >> 1] >> (sh + 4)), i4_pair(a1[ks >> 1] >> (sh + 4))};
-          mma_bf16(sc[mt], a, qf[2 * ks], qf[2 * ks + 1]);
+          const uint32_t x = (ks & 1) ? a0[ks >> 1] >> 8 : a0[ks >> 1], y = (ks & 1) ? a1[ks >> 1] >> 8 : a1[ks >> 1];
+          const uint32_t a[4] = {x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u};
+          mma_f16(sc[mt], a, qf[2 * ks], qf[2 * ks + 1]);
         }
       }
-      // raw logits of keys mt * 16 + g (+ 8), rows 2 t, 2 t + 1
+      // logits of keys mt * 16 + g (+ 8)
       const uint32_t* kp = reinterpret_cast<const uint32_t*>(kb + kI4Codes);
-      float pm[2] = {-INFINITY, -INFINITY};
+      float pm[kE];
+#pragma unroll
+      for (int e = 0; e < kE; ++e) pm[e] = -INFINITY;
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
           const int key = mt * 16 + 8 * hh + g;
           const uint32_t pr = kp[key];
-          const float st = __uint_as_float(pr << 16), base = fmaf(8.f, st, __uint_as_float(pr & 0xffff0000u));
+          const float st = __uint_as_float(pr << 16), low = __uint_as_float(pr & 0xffff0000u);
           const bool in = whole || n0 + key < it.k_end;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float raw = fmaf(st, sc[mt][2 * hh + e], base * qsum[e]);
+          for (int e = 0; e < kE; ++e) {
+            const float raw = fmaf(st, sc[mt][2 * hh + e], low * qsum[e]);
             sc[mt][2 * hh + e] = in ? raw : -INFINITY;  // (a select: what lies past the end may be NaN)
             pm[e] = fmaxf(pm[e], sc[mt][2 * hh + e]);
           }
         }
+      __syncwarp();  // every lane has read K
+      if (2 * j + kFewStages < 2 * n_mine) load(2 * j + kFewStages, slot);
+      if (++slot == kFewStages) {
+        slot = 0;
+        parity ^= 1;
+      }
       if (chunk_scores) {
         unsigned long long* sacc = p.score_acc + static_cast<int64_t>(it.seq) * p.seqlen_max + n0;
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
           for (int hh = 0; hh < 2; ++hh) {
-            float v = (is_m[0] ? sc[mt][2 * hh] : 0.f) + (is_m[1] ? sc[mt][2 * hh + 1] : 0.f);
+            float v = 0.f;
+#pragma unroll
+            for (int e = 0; e < kE; ++e) v += is_m[e] ? sc[mt][2 * hh + e] * up[e] : 0.f;
             v += __shfl_xor_sync(0xffffffffu, v, 1);
             v += __shfl_xor_sync(0xffffffffu, v, 2);
             const int key = mt * 16 + 8 * hh + g;
             if (t == mt && n0 + key < it.k_end) a4_add_score(sacc + key, v, range_ok);
           }
       }
+      live = mbar_wait(&bar[slot], parity, p.status, kA4KernelId);
+      if (!live) break;
+      const uint8_t* vb = ring + slot * kI4Block;
+      const uint32_t* vp = reinterpret_cast<const uint32_t*>(vb + kI4Codes);
+      // the exponent of the page's largest value
+      uint32_t mag = 0;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t pr = vp[lane + 32 * k];
+        const float m = fmaxf(__uint_as_float(pr << 16) * 16.f, fabsf(__uint_as_float(pr & 0xffff0000u)));
+        if (whole || n0 + lane + 32 * k < it.k_end) mag = max(mag, __float_as_uint(m));
+      }
+      const int ev = exponent_of(__uint_as_float(__reduce_max_sync(0xffffffffu, mag)));
+      const float vn = pow2i(-ev);
+      float ref[kE];
+      bool grow = false;
+#pragma unroll
+      for (int e = 0; e < kE; ++e) {
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) pm[e] = fmaxf(pm[e], __shfl_xor_sync(0xffffffffu, pm[e], o));
-        pm[e] = fmaxf(mx[e], pm[e] * p.scale_log2);
+        pm[e] = fmaxf(mx[e], fmaf(pm[e], mul[e], static_cast<float>(ev)));
+        ref[e] = pm[e] == -INFINITY ? 0.f : pm[e];
+        grow = grow || pm[e] > mx[e];
       }
-      const float ref[2] = {pm[0] == -INFINITY ? 0.f : pm[0], pm[1] == -INFINITY ? 0.f : pm[1]};
-      if (__any_sync(0xffffffffu, pm[0] > mx[0] || pm[1] > mx[1])) {
-        const float al[2] = {ex2_approx(mx[0] - ref[0]), ex2_approx(mx[1] - ref[1])};
+      if (__any_sync(0xffffffffu, grow)) {
+        float al[2] = {0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
+        for (int e = 0; e < kE; ++e) {
+          al[e] = ex2_approx(mx[e] - ref[e]);
           l[e] *= al[e];
           pb[e] *= al[e];
           mx[e] = pm[e];
         }
 #pragma unroll
-        for (int jj = 0; jj < 8; ++jj) {
-          acc[jj][0] *= al[0];
-          acc[jj][1] *= al[1];
-          acc[jj][2] *= al[0];
-          acc[jj][3] *= al[1];
-        }
+        for (int jj = 0; jj < 8; ++jj)
+#pragma unroll
+          for (int e = 0; e < kE; ++e) {
+            acc[jj][e] *= al[e];
+            acc[jj][2 + e] *= al[e];
+          }
       }
-      const uint32_t* vp = reinterpret_cast<const uint32_t*>(vb + kI4Codes);
       uint32_t bf[4][2];
+      float lp[kE];
+#pragma unroll
+      for (int e = 0; e < kE; ++e) {
+        lp[e] = 0.f;
+        ref[e] = static_cast<float>(ev) - ref[e];
+      }
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
           const int key = mt * 16 + 8 * hh + g;
-          const uint32_t pr = vp[key];
-          const bool in = whole || n0 + key < it.k_end;
-          // past the end p is 0, but 0 times a NaN step is not
-          const float st = in ? __uint_as_float(pr << 16) : 0.f;
-          const float base = in ? fmaf(8.f, st, __uint_as_float(pr & 0xffff0000u)) : 0.f;
-          float w[2];
+          uint32_t pr = vp[key];
+          if (!whole && n0 + key >= it.k_end) pr = 0;  // p is 0 there, but 0 times a NaN step is not
+          const float st = __uint_as_float(pr << 16) * vn, low = __uint_as_float(pr & 0xffff0000u) * vn;
+          float w[2] = {0.f, 0.f};
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float x = ex2_approx(fmaf(sc[mt][2 * hh + e], p.scale_log2, -ref[e]));
-            l[e] += x;
-            pb[e] = fmaf(x, base, pb[e]);
-            w[e] = x * st;
+          for (int e = 0; e < kE; ++e) {
+            const float x = ex2_approx(fmaf(sc[mt][2 * hh + e], mul[e], ref[e]));
+            lp[e] += x;
+            pb[e] = fmaf(x, low, pb[e]);
+            w[e] = x * (st * static_cast<float>(1 << kFewRaise));
           }
-          bf[mt][hh] = transpose8x8(pack_bf16x2(w[0], w[1]));
+          bf[mt][hh] = transpose8x8(pack_half2(w[0], w[1]));
         }
+#pragma unroll
+      for (int e = 0; e < kE; ++e) l[e] = fmaf(lp[e], vn, l[e]);
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
         const uint8_t* vr = vb + (mt * 16 + 2 * t) * kI4Row + 8 * g;
@@ -369,26 +474,35 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_int4_few_kernel(const A4P
         const uint2 k3 = *reinterpret_cast<const uint2*>(vr + 9 * kI4Row);
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          const uint32_t lo0 = __byte_perm(w ? k0.y : k0.x, w ? k1.y : k1.x, 0x5410);
-          const uint32_t hi0 = __byte_perm(w ? k0.y : k0.x, w ? k1.y : k1.x, 0x7632);
-          const uint32_t lo1 = __byte_perm(w ? k2.y : k2.x, w ? k3.y : k3.x, 0x5410);
-          const uint32_t hi1 = __byte_perm(w ? k2.y : k2.x, w ? k3.y : k3.x, 0x7632);
+          uint32_t lo0 = __byte_perm(w ? k0.y : k0.x, w ? k1.y : k1.x, 0x5410);
+          uint32_t hi0 = __byte_perm(w ? k0.y : k0.x, w ? k1.y : k1.x, 0x7632);
+          uint32_t lo1 = __byte_perm(w ? k2.y : k2.x, w ? k3.y : k3.x, 0x5410);
+          uint32_t hi1 = __byte_perm(w ? k2.y : k2.x, w ? k3.y : k3.x, 0x7632);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint32_t a[4] = {i4_pair(lo0 >> (4 * i)), i4_pair(hi0 >> (4 * i)), i4_pair(lo1 >> (4 * i)),
-                                   i4_pair(hi1 >> (4 * i))};
-            mma_bf16(acc[4 * w + i], a, bf[mt][0], bf[mt][1]);
+            if (i == 2) {
+              lo0 >>= 8;
+              hi0 >>= 8;
+              lo1 >>= 8;
+              hi1 >>= 8;
+            }
+            const uint32_t m = (i & 1) ? 0x00f000f0u : 0x000f000fu;
+            const uint32_t a[4] = {lo0 & m, hi0 & m, lo1 & m, hi1 & m};
+            mma_f16(acc[4 * w + i], a, bf[mt][0], bf[mt][1]);
           }
         }
       }
-      __syncwarp();  // every lane has read the stage
-      if (lane == 0 && j + kFewStages < n_mine) load(j + kFewStages);
+      __syncwarp();  // every lane has read V
+      if (2 * j + 1 + kFewStages < 2 * n_mine) load(2 * j + 1 + kFewStages, slot);
+      if (++slot == kFewStages) {
+        slot = 0;
+        parity ^= 1;
+      }
     }
-    use += n_mine;
 
-    // join the warps: (m, l) and the unnormalised O rows, through the ring
+    // join the warps: (reference, l) and the unnormalised O rows, through the ring
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
+    for (int e = 0; e < kE; ++e)
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) {
         l[e] += __shfl_xor_sync(0xffffffffu, l[e], o);
@@ -398,21 +512,23 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_int4_few_kernel(const A4P
     float* mine = reinterpret_cast<float*>(smem) + warp * kFewPartFloats;
     if (g == 0) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        mine[2 * t + e] = mx[e];
-        mine[kFewRows + 2 * t + e] = l[e];
+      for (int e = 0; e < kE; ++e) {
+        mine[kE * t + e] = mx[e];
+        mine[kFewRows + kE * t + e] = l[e];
       }
     }
-    // O of row 2 t + e, dims 16 g + 8 w + 2 i + {0, 1}
+    // O of the lane's rows, dims 16 g + 8 w + 2 i + {0, 1}; codes were 2^-24 and
+    // (odd i) 2^-20 of themselves
+    constexpr float kUp = static_cast<float>(1 << (24 - kFewRaise)), kUp16 = kUp / 16.f;
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
+    for (int e = 0; e < kE; ++e)
 #pragma unroll
       for (int w = 0; w < 2; ++w)
 #pragma unroll
         for (int i = 0; i < 4; i += 2)
-          *reinterpret_cast<float4*>(mine + 2 * kFewRows + (2 * t + e) * kA4HeadDim + 16 * g + 8 * w + 2 * i) =
-              make_float4(acc[4 * w + i][e] + pb[e], acc[4 * w + i][2 + e] + pb[e], acc[4 * w + i + 1][e] + pb[e],
-                          acc[4 * w + i + 1][2 + e] + pb[e]);
+          *reinterpret_cast<float4*>(mine + 2 * kFewRows + (kE * t + e) * kA4HeadDim + 16 * g + 8 * w + 2 * i) =
+              make_float4(fmaf(acc[4 * w + i][e], kUp, pb[e]), fmaf(acc[4 * w + i][2 + e], kUp, pb[e]),
+                          fmaf(acc[4 * w + i + 1][e], kUp16, pb[e]), fmaf(acc[4 * w + i + 1][2 + e], kUp16, pb[e]));
     __syncthreads();
     // thread -> row r, dims 4 c .. 4 c + 3
     const int r = threadIdx.x >> 5, c = threadIdx.x & 31;
@@ -434,14 +550,14 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_int4_few_kernel(const A4P
       O.z = fmaf(f, v.z, O.z);
       O.w = fmaf(f, v.w, O.w);
     }
-    const int m = chunk * kFewRows + r;
-    bool write = m < m_all;
+    const int m = chunk * kRows + r;
+    bool write = r < kRows && m < m_all;
     if (n_splits > 1) {
       // chunk of an item of a head: its splits' results side by side
       const int64_t cell = (static_cast<int64_t>(item_id) * p.n_kv + kvh) * p.chunks + chunk;
       float* out = p.part + (cell * p.splits + split) * kFewPartFloats;
-      __stcg(reinterpret_cast<float4*>(out + 2 * kFewRows + r * kA4HeadDim) + c, O);
-      if (c == 0) {
+      if (write) __stcg(reinterpret_cast<float4*>(out + 2 * kFewRows + r * kA4HeadDim) + c, O);
+      if (write && c == 0) {
         __stcg(out + r, M);
         __stcg(out + kFewRows + r, L);
       }
@@ -496,7 +612,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) attn_int4_few_kernel(const A4P
         const int32_t* e = p.plan + kA4PlanHeader + (item_id - it.mchunk +
                                                      p.plan[p.plan[3] + kA4PlanSeq * it.seq] + i) * kA4PlanItem;
         const int rows = e[3] + e[5];
-        ctas += min(p.chunks, (rows * p.group + kFewRows - 1) / kFewRows);
+        ctas += min(p.chunks, (rows * p.group + kRows - 1) / kRows);
       }
       if (atomicAdd(p.score_cnt + it.seq, 1) == ctas * p.n_kv * cta_splits - 1) {
         p.score_cnt[it.seq] = 0;
@@ -581,14 +697,6 @@ static_assert(32 * (kMnSoft * kMnRegsSoft + kMnConv * kMnRegsConv + 4 * kMnRegsM
 constexpr float kMnLazy = 8.f;   // log2 units a contribution may pass the reference by before it moves
 constexpr float kMnRaise = 6.f;  // P is raised by 2^6: with the 8 above, below fp16's 2^16
 constexpr int kMnPartFloats = kMnRows * kA4HeadDim + 2 * kMnRows;
-
-// 2^e for |e| <= 126
-__device__ __forceinline__ float pow2i(int e) { return __int_as_float((127 + e) << 23); }
-// exponent of a magnitude, held to what pow2i takes (0 and denormals: the least)
-__device__ __forceinline__ int exponent_of(float mag) {
-  const int e = static_cast<int>((__float_as_uint(mag) >> 23) & 255u) - 127;
-  return max(-100, min(e, 126));
-}
 
 // fp16 operands (kind::f16, fp32 accumulate); the A operand in shared or in tensor memory
 __host__ __device__ constexpr uint32_t umma_idesc_f16(int M, int N) {
@@ -1380,6 +1488,7 @@ namespace {
 
 struct A4Plan {
   bool many;        // the tcgen05 kernel
+  bool narrow;      // few rows: at most four to a chunk
   int batch;        // many: sequences
   int chunks, splits, split_pages;
 };
@@ -1394,13 +1503,23 @@ constexpr int kFewMaxRows = 16;
 A4Plan a4_plan_few(int items, int rows, int group, int n_kv, int seqlen_max, int kv_splits) {
   A4Plan pl{};
   const int pages = (seqlen_max + kI4Page - 1) / kI4Page;
-  pl.chunks = (rows * group + kFewRows - 1) / kFewRows;
+  pl.narrow = rows * group <= kFewRows / 2;
+  const int chunk_rows = pl.narrow ? kFewRows / 2 : kFewRows;
+  pl.chunks = (rows * group + chunk_rows - 1) / chunk_rows;
   int s = kv_splits;
   if (s <= 0) {
     const long long ctas = static_cast<long long>(items) * pl.chunks * n_kv;
-    const long long want = (2ll * sm_count() + ctas - 1) / ctas;
-    const long long most = (pages + 2 * kFewWarps - 1) / (2 * kFewWarps);
-    s = static_cast<int>(want < most ? want : most);
+    const int slots = kFewCtas * sm_count();
+    long long best = 0;
+    for (int k = 1; k <= pages && k <= slots; ++k) {
+      const long long waves = (ctas * k + slots - 1) / slots;
+      const int rounds = ((pages + k - 1) / k + kFewWarps - 1) / kFewWarps;
+      const long long cost = waves * (rounds + 1) + (k > 1 ? 1 : 0);
+      if (k == 1 || cost < best) {
+        best = cost;
+        s = k;
+      }
+    }
   }
   if (s > pages) s = pages;
   if (s > 1024) s = 1024;
@@ -1557,7 +1676,9 @@ extern "C" int fdllm_attn_cache_int4(const void* q, void* o, const void* k_cache
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return FDLLM_ERR_CUDA;
   if (!attr[dev]) {
-    if (cudaFuncSetAttribute(attn_int4_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem) !=
+    if (cudaFuncSetAttribute(attn_int4_few_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem) !=
+            cudaSuccess ||
+        cudaFuncSetAttribute(attn_int4_few_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem) !=
             cudaSuccess ||
         cudaFuncSetAttribute(attn_int4_many_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMnSmem) !=
             cudaSuccess)
@@ -1573,7 +1694,8 @@ extern "C" int fdllm_attn_cache_int4(const void* q, void* o, const void* k_cache
   }
   const dim3 grid(static_cast<unsigned>(max_items) * pl.chunks, static_cast<unsigned>(n_kv_heads),
                   static_cast<unsigned>(pl.splits));
-  if (launch_ex(attn_int4_few_kernel, grid, dim3(kFewThreads), kFewSmem, stream, 1, pdl_enabled(), p) != cudaSuccess)
+  if (launch_ex(pl.narrow ? attn_int4_few_kernel<1> : attn_int4_few_kernel<2>, grid, dim3(kFewThreads), kFewSmem, stream,
+                1, pdl_enabled(), p) != cudaSuccess)
     return FDLLM_ERR_CUDA;
   return cudaPeekAtLastError() == cudaSuccess ? FDLLM_OK : FDLLM_ERR_CUDA;
 }
