@@ -1498,7 +1498,7 @@ struct A4Plan {
 // item, and the longest cache.  One CTA runs per SM and its eight warps take a
 // page each, so keys are split until the grid covers the SMs twice, and no
 // further than two pages per warp.
-constexpr int kFewMaxRows = 16;
+constexpr int kFewMaxRows = 32;
 
 A4Plan a4_plan_few(int items, int rows, int group, int n_kv, int seqlen_max, int kv_splits) {
   A4Plan pl{};

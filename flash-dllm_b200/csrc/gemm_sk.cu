@@ -1360,6 +1360,8 @@ int fdllm_gemm_int8(const void* a, const float* a_scale, const void* w, const fl
   for (const void* x : ptrs)
     if (x == nullptr || !aligned16(x)) return FDLLM_ERR_ARG;
   if (a_scale == nullptr || (residual != nullptr && !aligned16(residual))) return FDLLM_ERR_ARG;
+  if (gemv_int8_rows(n_rows, static_cast<int64_t>(n_cols) * k_dim))
+    return gemv_int8(a, a_scale, w, w_scale, out, residual, n_rows, n_cols, k_dim, ld_out, ld_res, false, stream);
   GemmParams p{};
   p.out0 = static_cast<__nv_bfloat16*>(out);
   p.res = static_cast<const __nv_bfloat16*>(residual);
@@ -1384,6 +1386,8 @@ int fdllm_gemm_swiglu_int8(const void* a, const float* a_scale, const void* w_ga
   for (const void* x : ptrs)
     if (x == nullptr || !aligned16(x)) return FDLLM_ERR_ARG;
   if (a_scale == nullptr) return FDLLM_ERR_ARG;
+  if (gemv_int8_rows(n_rows, static_cast<int64_t>(hidden) * 2 * k_dim))
+    return gemv_int8(a, a_scale, w_gate_up, w_scale, out, nullptr, n_rows, hidden, k_dim, ld_out, 0, true, stream);
   GemmParams p{};
   p.out0 = static_cast<__nv_bfloat16*>(out);
   p.ld_out = ld_out;

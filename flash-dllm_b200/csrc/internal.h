@@ -73,4 +73,15 @@ int launch_qkv_sk(const void* xn, const void* wq, const void* wk, const void* wv
                   int kv_by_slot, cudaStream_t stream);
 size_t qkv_sk_ws_bytes(int32_t n_rows, int32_t d_model);
 
+// int8 products of a few rows (gemv_int8.cu); n: output columns.  Up to four
+// rows it is ahead of the tensor cores at every size but the largest (126464 x
+// 4096 at four rows: 107 us against 101); up to eight while the weights are few
+// (50 M: 16.9 us against 18.3; 100 M: 31.2 against 28.6).
+inline bool gemv_int8_rows(int32_t rows, int64_t weights) {
+  return rows <= 4 || (rows <= 8 && weights <= (int64_t(1) << 26));
+}
+int gemv_int8(const void* a, const float* a_scale, const void* w, const float* w_scale, void* out,
+              const void* residual, int32_t rows, int32_t n, int32_t k, int64_t ld_out, int64_t ld_res, bool swiglu,
+              cudaStream_t stream);
+
 }  // namespace fdllm

@@ -189,6 +189,26 @@ def test_linear_swiglu_int8(rows, h, k, plan, gemm_plan):
     assert ((y - ref).abs() <= tol * (1 + 2 * U8)).all()
 
 
+@pytest.mark.parametrize("rows,n,k", [(1, 8, 131056), (2, 16, 16), (3, 1032, 4112), (4, 40, 8176), (5, 264, 8208),
+                                      (6, 8, 32), (8, 2056, 528), (8, 16392, 4096)])
+def test_linear_int8_few_rows(rows, n, k):
+    """Up to eight rows: every count, and K that ends inside a step; the same
+    rows among more (another kernel) are the same integers and scales."""
+    from flash_dllm_b200 import ops
+    g = _gen(rows + n)
+    a, w = _int8(g, 12, k), _int8(g, n, k)
+    sa, sw = torch.rand(12, device="cuda", generator=g) + 0.01, torch.rand(n, device="cuda", generator=g) * 1e-3
+    y = ops.linear_int8(a[:rows], sa[:rows], w, sw)
+    ref, tol = _linear_ref(a, sa, w, sw)
+    assert ((y.double() - ref[:rows]).abs() <= tol[:rows]).all()
+    assert ((ops.linear_int8(a, sa, w, sw).double() - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("rows,h,k", [(2, 128, 16), (3, 256, 4112), (4, 128, 1040), (7, 1024, 272), (8, 128, 12288)])
+def test_linear_swiglu_int8_few_rows(rows, h, k, gemm_plan):
+    test_linear_swiglu_int8(rows, h, k, {}, gemm_plan)
+
+
 # ------------------------------------------------------ append to a cache --
 
 def _append_case(seed, seqs, tokens, h, hk, length, bits, table=True):
