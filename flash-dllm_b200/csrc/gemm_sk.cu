@@ -1096,7 +1096,26 @@ int g2_max_pairs_for(int epi, int ksub) {
 // request) for 64-row single CTAs, one 64-K box elsewhere.
 //
 // I8: k_dim counts pairs of int8 (the 2-byte columns of the tensor maps); a
-// last box that reaches past it is zero-filled by the loads.
+// last box that reaches past it is zero-filled by the loads.  The products
+// take half the time per k-block and the fix-ups as long as ever, so the int8
+// plan differs (rows x columns x K, us):
+//   - single CTAs with 128-column tiles while those fit the grid once, with up
+//     to 384 rows or K up to 8192 (256x4096x4096: 13.8 against a pair's 20.9;
+//     384x4096x12288 28.9, 31.7; but 512x4096x12288 33.3, 31.7), and up to 256
+//     rows while they fit it twice (256x12288x4096 22.0, 23.7; but
+//     256x24576x4096 38.2, 34.1);
+//   - 128 x 256 tiles, one whole tile a CTA, where they nearly fill one wave
+//     and K is up to 8192 (384x12288x4096: 22.4 against 28.7 and 28.8;
+//     1024x4096x4096 20.2, 24.3; but 1024x4096x12288 51.5, 44.4);
+//   - a group's CTAs are cut to a number that splits its tiles at the same
+//     places (whole or half tiles a CTA, or whole CTAs a tile) if that leaves
+//     out less than 3 in 20: fewer pieces and no CTA that adds to two tiles
+//     (16x4096x4096: 10.6 against 12.4; 512x12288x4096 29.3, 34.5).  Where the
+//     fix-ups are little of the whole, all SMs stay in: up to 128 rows with
+//     eight k-blocks a CTA and more (16x24576x4096: 23.2 against 24.9), pairs
+//     with two tiles each and more or more than 512 rows (2048x4096x12288:
+//     74.3 against 81.4);
+//   - no piece is under four k-blocks (100x1024x1024: 11.3 against 17.1).
 GemmPlan plan_gemm(int epi, int32_t n_rows, int32_t n_cols, int32_t k_dim, int32_t d_model, bool i8 = false) {
   GemmPlan pl{};
   const GemmOverride& ov = gemm_override();
@@ -1111,7 +1130,19 @@ GemmPlan plan_gemm(int epi, int32_t n_rows, int32_t n_cols, int32_t k_dim, int32
                                ((out_cols + (epi == kEpiSwiglu ? 63 : 127)) / (epi == kEpiSwiglu ? 64 : 128));
     if (tiles128 <= sm_count() && 5 * tiles128 >= 4ll * sm_count()) dp = true;
   }
-  pl.pair = ov.pair < 0 ? (n_rows > kGBM && !dp) : ov.pair != 0;
+  const bool i8_auto = i8 && ov.pair < 0 && ov.dp == 0 && ov.bn == 0 && ov.grid == 0;
+  bool one_wave256 = false, single = false;
+  if (i8_auto && n_rows > kGBM) {
+    const long long m = (n_rows + kGBM - 1) / kGBM, sms = sm_count();
+    const int cols128 = epi == kEpiSwiglu ? 64 : 128;
+    const long long tiles128 = m * ((out_cols + cols128 - 1) / cols128);
+    const long long tiles256 = m * ((out_cols + 2 * cols128 - 1) / (2 * cols128));
+    one_wave256 = n_rows > 2 * kGBM && k_dim <= 4096 && tiles256 <= sms && 6 * tiles256 >= 5 * sms;
+    single = !one_wave256 && ((tiles128 <= sms && (n_rows <= 384 || k_dim <= 4096)) ||
+                              (n_rows <= 2 * kGBM && tiles128 <= 2 * sms));
+    dp = one_wave256 || (dp && single);
+  }
+  pl.pair = ov.pair < 0 ? (n_rows > kGBM && !dp && !single) : ov.pair != 0;
   if (epi == kEpiQkv && d_model % 256 != 0) pl.pair = false;  // a pair tile holds two heads of one projection
   int bn;
   if (pl.pair) {
@@ -1119,7 +1150,7 @@ GemmPlan plan_gemm(int epi, int32_t n_rows, int32_t n_cols, int32_t k_dim, int32
     pl.xrows = kGBM;
     pl.m_tiles = (n_rows + 2 * kGBM - 1) / (2 * kGBM);
   } else {
-    bn = ov.bn == 128 || ov.bn == 256 ? ov.bn : 128;
+    bn = ov.bn == 128 || ov.bn == 256 ? ov.bn : one_wave256 ? 256 : 128;
     if (epi == kEpiQkv && d_model % bn != 0) bn = 128;
     pl.xrows = n_rows <= 64 ? 64 : kGBM;
     pl.m_tiles = (n_rows + kGBM - 1) / kGBM;
@@ -1150,6 +1181,17 @@ GemmPlan plan_gemm(int epi, int32_t n_rows, int32_t n_cols, int32_t k_dim, int32
   // tiles fit the grid
   const int tiles_per_group = pl.groups > 1 ? pl.n_tiles : pl.m_tiles * pl.n_tiles;
   if (dp && tiles_per_group <= per_group) per_group = tiles_per_group;
+  // (pieces of at least four k-blocks: below that the join is all of the time)
+  if (i8_auto && !dp && iters < 4ll * per_group) per_group = static_cast<int>(std::max(1ll, iters / 4));
+  bool even = false;  // CTAs' ranges meet at whole, half, ... tiles
+  if (i8_auto && !dp &&
+      (pl.pair ? pl.m_tiles <= 2 && tiles_per_group < 2 * per_group : pl.m_tiles > 1 || iters < 8ll * per_group)) {
+    for (int c = per_group; !even && 20 * c >= 17 * per_group; --c)
+      if ((2 * tiles_per_group) % c == 0 || c % tiles_per_group == 0) {
+        per_group = c;
+        even = true;
+      }
+  }
   // CTA pairs: whole-tile waves plus a stream-K region of the remaining
   // tiles (split first, so only the last whole tile's epilogue follows the
   // last MMA; measured 4 and 3 us faster for the QKV and MLP GEMMs at 512
@@ -1159,7 +1201,7 @@ GemmPlan plan_gemm(int epi, int32_t n_rows, int32_t n_cols, int32_t k_dim, int32
   // k-blocks than CTAs: every CTA's range must be non-empty).  dp = 2: all
   // tiles stream-K.
   int sk_tiles = tiles_per_group;
-  if (pl.pair && ov.dp != 2 && tiles_per_group >= per_group) {
+  if (pl.pair && ov.dp != 2 && !even && tiles_per_group >= per_group) {
     sk_tiles = tiles_per_group % per_group;
     if (sk_tiles > 0 && (8 * sk_tiles < per_group || static_cast<long long>(sk_tiles) * pl.kbt < per_group))
       sk_tiles += per_group;
