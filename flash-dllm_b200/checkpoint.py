@@ -103,10 +103,12 @@ def config_from_json(path: str) -> LLaDAConfigB200:
 
 
 @torch.no_grad()
-def load_model(path: str, device="cuda", dtype=torch.bfloat16, fuse_mlp: bool = True) -> LLaDAModelB200:
+def load_model(path: str, device="cuda", dtype=torch.bfloat16, fuse_mlp: bool = True,
+               int8: bool = False) -> LLaDAModelB200:
     """LLaDAModelB200 with the weights of the checkpoint directory `path`
     (every parameter must be present, none may be left over), cast to
-    `dtype` on `device`; the MLP weights are stacked for the fused GEMM."""
+    `dtype` on `device`; the MLP weights are stacked for the fused GEMM.
+    `int8` adds 8-bit copies of the projections (`LLaDAModelB200.quantize_int8`)."""
     cfg = config_from_json(path)
     with torch.device("meta"):
         model = LLaDAModelB200(cfg, device="meta", dtype=dtype)
@@ -127,6 +129,8 @@ def load_model(path: str, device="cuda", dtype=torch.bfloat16, fuse_mlp: bool = 
         raise KeyError(f"checkpoint lacks {len(missing)} tensors, e.g. {missing[:3]}")
     if fuse_mlp:
         model.fuse_mlp_weights()
+    if int8:
+        model.quantize_int8()
     return model.eval()
 
 
@@ -137,10 +141,10 @@ def load_tokenizer(path: str, trust_remote_code: bool = True):
     return AutoTokenizer.from_pretrained(path, trust_remote_code=trust_remote_code)
 
 
-def from_pretrained(path: str, device="cuda", dtype=torch.bfloat16, tokenizer: bool = True
+def from_pretrained(path: str, device="cuda", dtype=torch.bfloat16, tokenizer: bool = True, int8: bool = False
                     ) -> Tuple[LLaDAModelB200, Optional[object]]:
     """(model, tokenizer or None) from a local LLaDA checkpoint directory."""
-    model = load_model(path, device=device, dtype=dtype)
+    model = load_model(path, device=device, dtype=dtype, int8=int8)
     return model, (load_tokenizer(path) if tokenizer else None)
 
 

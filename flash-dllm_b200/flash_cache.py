@@ -28,11 +28,22 @@ alone at several of those shapes).  The
 environment variable ``FDLLM_OWN_GEMMS`` (a comma list of ``attn_out``,
 ``mlp``, ``ff_out``, ``lm_head``, ``all`` or ``none``) forces the choice for
 comparisons (``lm_head``: the model's LM head, in ``model.py``).
+
+Two options, each on its own or together:
+- 8-bit projections (``quantize_block_int8``): QKV, ``attn_out``, the MLP and
+  ``ff_out`` as int8 products with a scale per token and per output channel,
+  the tokens quantised behind the norms.  The verify forward, whose task is to
+  check drafts, keeps the bf16 weights.
+- a 4-bit cache (``k_cache`` / ``v_cache`` from ``ops.int4_cache``): Q and K are
+  rotated and K and V quantised on the way into the pages, attention reads the
+  4-bit pages, and the verify attention the keys and values they stand for.
 """
 from __future__ import annotations
 
+import itertools
 import math
 import os
+from typing import NamedTuple
 
 import torch
 
@@ -132,6 +143,39 @@ class _PlanCache:
 _PLANS = _PlanCache()
 
 
+class Int8Weights(NamedTuple):
+    """A block's projections as int8 [n, k] with an fp32 scale per row."""
+    qkv: torch.Tensor         # [q; k; v]
+    qkv_scale: torch.Tensor
+    attn_out: torch.Tensor
+    attn_out_scale: torch.Tensor
+    ffup: torch.Tensor        # [ff_proj; up_proj]
+    ffup_scale: torch.Tensor
+    ff_out: torch.Tensor
+    ff_out_scale: torch.Tensor
+    version: int              # distinct for every quantisation (graphs captured with other weights are stale)
+
+
+_INT8_VERSIONS = itertools.count(1)
+
+
+@torch.no_grad()
+def quantize_block_int8(block) -> None:
+    """Set ``block.int8_weights`` from the block's bf16 weights: from then on
+    its Flash-Cache forwards run 8-bit products.  The bf16 weights stay (the
+    verify forward uses them); call again after changing them, and delete the
+    attribute to go back."""
+    linears = [getattr(block, n) for n in ("q_proj", "k_proj", "v_proj", "attn_out", "ff_proj", "up_proj", "ff_out")]
+    if not all(_plain_linear(m) for m in linears):
+        raise TypeError("8-bit projections need bf16 Linear modules without bias")
+    if not isinstance(block.dropout, torch.nn.Identity) or not isinstance(block.act, torch.nn.SiLU):
+        raise TypeError("8-bit projections need a block without dropout and with SiLU")
+    wq, wk, wv, wo, wg, wu, wf = (m.weight.detach() for m in linears)
+    block.int8_weights = Int8Weights(*ops.quantize_int8(torch.cat([wq, wk, wv], 0)), *ops.quantize_int8(wo),
+                                     *ops.quantize_int8(torch.cat([wg, wu], 0)), *ops.quantize_int8(wf),
+                                     next(_INT8_VERSIONS))
+
+
 def flash_fused_elastic_cache(self, x: torch.Tensor, block_idx, positions, lengths, softmax_scale: float = None):
     query_pos_flat, key_pos_flat, rotary_emb_pos, _info, attn_scores, attn_mask = positions
     (_start_layer, query_verify_blocks, query_masked_blocks, query_tracked_blocks, _query_blocks, active_batch,
@@ -142,27 +186,58 @@ def flash_fused_elastic_cache(self, x: torch.Tensor, block_idx, positions, lengt
     softmax_scale = softmax_scale or (1.0 / math.sqrt(head_dim))
     x = x.contiguous()
     n_rows = x.shape[0]
-    x_normed = ops.rmsnorm(x, _norm_weight(self.attn_norm), _eps(self.attn_norm))
-    att = torch.empty_like(x)
-    q = torch.empty_like(x)
+    int8 = None if verify else getattr(self, "int8_weights", None)
+    four_bits = getattr(self.k_cache, "dtype", None) == torch.uint8  # ops.int4_cache
     sin, cos = rotary_emb_pos
     wq, wk, wv = self.q_proj.weight, self.k_proj.weight, self.v_proj.weight
+    att = torch.empty_like(x)
+    if int8 is None:
+        x_normed = ops.rmsnorm(x, _norm_weight(self.attn_norm), _eps(self.attn_norm))
+        q = torch.empty_like(x)
 
     if verify:
         k1 = torch.empty_like(x)
         v1 = torch.empty_like(x)
         ops.verify_qkv(x_normed, wq, wk, wv, query_pos_flat, sin, cos, q, k1, v1, n_heads)
-        ops.verify_attn(q, k1, v1, att, self.k_cache, self.v_cache, key_pos_flat, attn_mask, query_verify_blocks,
+        k_cache, v_cache = self.k_cache, self.v_cache
+        if four_bits:
+            if key_pos_flat.numel() > 0:  # the gathered keys as bf16 rows of their own
+                k_cache, v_cache = ops.read_cache_int4(k_cache, v_cache, key_pos_flat, max_length)
+                key_pos_flat = torch.arange(key_pos_flat.numel(), device=x.device)
+            else:
+                k_cache, v_cache = k1, v1  # (nothing is read)
+        ops.verify_attn(q, k1, v1, att, k_cache, v_cache, key_pos_flat, attn_mask, query_verify_blocks,
                         2 * block_m, n_heads, softmax_scale, max_keys=max_length)
     else:
         if n_rows > 0:
-            ops.qkv_rope_cache(x_normed, wq, wk, wv, query_pos_flat, sin, cos, q, self.k_cache, self.v_cache,
-                               n_heads)
+            if int8 is not None:
+                a, a_scale = ops.rmsnorm_int8(x, _norm_weight(self.attn_norm), _eps(self.attn_norm))
+                qkv = ops.linear_int8(a, a_scale, int8.qkv, int8.qkv_scale)
+                q, k1, v1 = qkv[:, :d_model], qkv[:, d_model:2 * d_model], qkv[:, 2 * d_model:]
+            elif four_bits:
+                q, k1, v1 = (torch.nn.functional.linear(x_normed, w) for w in (wq, wk, wv))
+            if int8 is not None or four_bits:
+                q = ops.rope_append(q, k1, v1, query_pos_flat, sin, cos, self.k_cache, self.v_cache, n_heads,
+                                    n_heads, max_length)
+            else:
+                ops.qkv_rope_cache(x_normed, wq, wk, wv, query_pos_flat, sin, cos, q, self.k_cache, self.v_cache,
+                                   n_heads)
             plan, cap = _PLANS.get(query_masked_blocks, query_tracked_blocks, n_rows, len(active_batch), block_m,
                                    max_length, x.device)
             scores = attn_scores if block_idx > 1 else None
-            ops.attn_cache(q, att, self.k_cache, self.v_cache, plan, cap, scores, 1.0 / (block_m * n_heads),
-                           n_heads, max_length, softmax_scale, items_hint=-(-n_rows // 64))
+            if four_bits:
+                ops.attn_cache_int4(q, att, self.k_cache, self.v_cache, plan, cap, scores, 1.0 / (block_m * n_heads),
+                                    n_heads, n_heads, max_length, softmax_scale,
+                                    rows_hint=-(-n_rows // max(1, len(active_batch))))
+            else:
+                ops.attn_cache(q, att, self.k_cache, self.v_cache, plan, cap, scores, 1.0 / (block_m * n_heads),
+                               n_heads, max_length, softmax_scale, items_hint=-(-n_rows // 64))
+
+    if int8 is not None:
+        og_x = ops.linear_int8(*ops.quantize_int8(att), int8.attn_out, int8.attn_out_scale, residual=x)
+        a, a_scale = ops.rmsnorm_int8(og_x, _norm_weight(self.ff_norm), _eps(self.ff_norm))
+        h = ops.linear_swiglu_int8(a, a_scale, int8.ffup, int8.ffup_scale)
+        return ops.linear_int8(*ops.quantize_int8(h), int8.ff_out, int8.ff_out_scale, residual=og_x).unsqueeze(0)
 
     # Residual adds: into the GEMM epilogue (C = x + att W^T, one bf16 rounding
     # of the sum instead of two) when the projection is a plain bias-free

@@ -26,6 +26,10 @@ caches, score buffer, RoPE tables and graphs live in a per-model session
 (one per batch size / slot length), so a later call of the same shape zeroes
 the caches and replays the graphs an earlier call captured.
 
+``kv_bits=4`` keeps the KV caches in 4 bits (3.76 times less memory and
+reading than bf16); a model with 8-bit projections
+(``LLaDAModelB200.quantize_int8``) is run as such.
+
 ``min_keep`` (default 1, the reference) forces a minimum number of accepted
 tokens per step; ``trace`` (a list) receives the per-step decisions.
 """
@@ -168,11 +172,14 @@ class _Session:
     and scores instead of allocating them, so forwards captured by an earlier
     call replay unchanged."""
 
-    def __init__(self, model, B: int, L: int, head_dim: int, use_graphs: bool):
+    def __init__(self, model, B: int, L: int, head_dim: int, use_graphs: bool, kv_bits: int):
         dev, cfg = model.device, model.config
-        self.caches = [(torch.zeros((L * B, cfg.d_model), dtype=model.dtype, device=dev),
-                        torch.zeros((L * B, cfg.d_model), dtype=model.dtype, device=dev))
-                       for _ in model.model.transformer.blocks]
+        blocks = model.model.transformer.blocks
+        if kv_bits == 4:
+            self.caches = [ops.int4_cache(L * B // ops.PAGE, cfg.n_heads, dev) for _ in blocks]
+        else:
+            self.caches = [(torch.zeros((L * B, cfg.d_model), dtype=model.dtype, device=dev),
+                            torch.zeros((L * B, cfg.d_model), dtype=model.dtype, device=dev)) for _ in blocks]
         self.attn_scores = torch.zeros(B * L, dtype=torch.float32, device=dev)
         sin, cos = get_rotary_embedding(L, head_dim, cfg.rope_theta, dev)
         self.rotary = [sin.repeat(B, 1).contiguous(), cos.repeat(B, 1).contiguous()]
@@ -192,13 +199,15 @@ class _Session:
 _SESSIONS = weakref.WeakKeyDictionary()
 
 
-def _session(model, B: int, L: int, head_dim: int, use_graphs: bool) -> _Session:
-    key = (B, L, model.dtype, str(model.device), use_graphs)
+def _session(model, B: int, L: int, head_dim: int, use_graphs: bool, kv_bits: int = 16) -> _Session:
+    int8 = tuple(b.int8_weights.version if getattr(b, "int8_weights", None) is not None else 0
+                 for b in model.model.transformer.blocks)
+    key = (B, L, model.dtype, str(model.device), use_graphs, kv_bits, int8)
     held = _SESSIONS.get(model)
     if held is None or held[0] != key:
         held = (key, None)
         _SESSIONS[model] = held  # drop the previous shape's buffers first
-        held = (key, _Session(model, B, L, head_dim, use_graphs))
+        held = (key, _Session(model, B, L, head_dim, use_graphs, kv_bits))
         _SESSIONS[model] = held
     sess = held[1]
     sess.reset(model)
@@ -247,7 +256,8 @@ def generate_with_Flash_dLLM(model, prompts, prompt_lengths, batch_size, respons
                              mask_id=126336, threshold=0.9, gamma=0.9, track_num=4, mask_num=4, eos_id=126081,
                              verify=False, sliding_window=True, is_instruct=True, tokenizer=None, stop_tokens=None,
                              min_keep: int = 1, trace: Optional[list] = None, max_steps: Optional[int] = None,
-                             step_hook=None, record=None, stats: Optional[dict] = None, use_graphs: bool = True):
+                             step_hook=None, record=None, stats: Optional[dict] = None, use_graphs: bool = True,
+                             kv_bits: int = 16):
     """Returns ``(responses, num_tokens, max_num_tokens)`` like the reference;
     ``responses[i]`` is the decoded text (token ids when ``tokenizer`` is
     None) and ``n_steps[i]`` counts the steps of prompt ``i``.  ``max_steps``
@@ -255,7 +265,8 @@ def generate_with_Flash_dLLM(model, prompts, prompt_lengths, batch_size, respons
     ``record(verify, x_query, query_pos, key_pos, logits, logit_rows,
     attn_scores)`` sees every forward (tests replay it through the oracle);
     ``stats`` (a dict) accumulates ``h2d_bytes`` / ``d2h_bytes`` / ``steps``;
-    ``use_graphs`` replays repeated forward shapes as CUDA graphs."""
+    ``use_graphs`` replays repeated forward shapes as CUDA graphs; ``kv_bits``:
+    16 (bf16 caches) or 4 (``ops.int4_cache``; heads of 128)."""
     dev = model.device
     cfg = model.config
     io = stats if stats is not None else {}
@@ -276,6 +287,10 @@ def generate_with_Flash_dLLM(model, prompts, prompt_lengths, batch_size, respons
 
     d_model, n_heads, n_layers = cfg.d_model, cfg.n_heads, cfg.n_layers
     head_dim = d_model // n_heads
+    if kv_bits not in (16, 4):
+        raise ValueError(f"kv_bits must be 16 or 4, got {kv_bits}")
+    if kv_bits == 4 and head_dim != ops.HEAD_DIM:
+        raise ValueError(f"the 4-bit cache holds heads of {ops.HEAD_DIM}, not {head_dim}")
     bm, bn = block_length, 128
     L = ((max(prompt_lengths) + gen_length + bm) // bn + 1) * bn
     B = batch_size
@@ -284,7 +299,7 @@ def generate_with_Flash_dLLM(model, prompts, prompt_lengths, batch_size, respons
     x = torch.full((B * L,), mask_id, dtype=torch.long, device=dev)
     x_draft = torch.full((B * L,), mask_id, dtype=torch.long, device=dev)
     full_pos = torch.arange(B * L, device=dev).reshape(B, L)
-    sess = _session(model, B, L, head_dim, use_graphs)
+    sess = _session(model, B, L, head_dim, use_graphs, kv_bits)
     attn_scores = sess.attn_scores
     rotary_emb_pos = sess.rotary
     empty_i32, empty_i64 = sess.empty_i32, sess.empty_i64

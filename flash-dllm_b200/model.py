@@ -21,7 +21,7 @@ import torch
 from torch import nn
 
 from . import ops
-from .flash_cache import flash_fused_elastic_cache, use_own
+from .flash_cache import flash_fused_elastic_cache, quantize_block_int8, use_own
 
 
 @dataclasses.dataclass
@@ -136,6 +136,13 @@ class LLaDAModelB200(nn.Module):
         """``LLaDABlockB200.fuse_mlp_weights`` on every block."""
         for blk in self.model.transformer.blocks:
             blk.fuse_mlp_weights()
+
+    def quantize_int8(self) -> "LLaDAModelB200":
+        """8-bit projections in every block from now on (``quantize_block_int8``:
+        the LM head and the verify forwards stay bf16)."""
+        for blk in self.model.transformer.blocks:
+            quantize_block_int8(blk)
+        return self
 
     @torch.no_grad()
     def forward(self, input_ids: torch.Tensor, use_cache: bool = True, lengths=None, positions=None,
