@@ -342,19 +342,29 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) attn_int4_few_kernel(co
       const int n0 = (first + warp + j * kFewWarps) * kI4Page;
       const bool whole = n0 + kI4Page <= it.k_end;  // uniform
       float sc[4][4];
+      {  // the four tiles in step: their chains of products overlap
+        uint32_t w[8][4];
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sc[mt][e] = 0.f;
-        const uint4 wa = *reinterpret_cast<const uint4*>(kb + (mt * 16 + g) * kI4Row + 16 * t);
-        const uint4 wb = *reinterpret_cast<const uint4*>(kb + (mt * 16 + 8 + g) * kI4Row + 16 * t);
-        const uint32_t a0[4] = {wa.x, wa.y, wa.z, wa.w}, a1[4] = {wb.x, wb.y, wb.z, wb.w};
-#pragma unroll
-        for (int ks = 0; ks < 8; ++ks) {
-          const uint32_t x = (ks & 1) ? a0[ks >> 1] >> 8 : a0[ks >> 1], y = (ks & 1) ? a1[ks >> 1] >> 8 : a1[ks >> 1];
-          const uint32_t a[4] = {x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u};
-          mma_f16(sc[mt], a, qf[2 * ks], qf[2 * ks + 1]);
+        for (int h = 0; h < 8; ++h) {
+          const uint4 v = *reinterpret_cast<const uint4*>(kb + (8 * h + g) * kI4Row + 16 * t);
+          w[h][0] = v.x;
+          w[h][1] = v.y;
+          w[h][2] = v.z;
+          w[h][3] = v.w;
         }
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[h][e] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            const uint32_t x = (ks & 1) ? w[2 * h][ks >> 1] >> 8 : w[2 * h][ks >> 1];
+            const uint32_t y = (ks & 1) ? w[2 * h + 1][ks >> 1] >> 8 : w[2 * h + 1][ks >> 1];
+            const uint32_t a[4] = {x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u};
+            mma_f16(sc[h], a, qf[2 * ks], qf[2 * ks + 1]);
+          }
       }
       // logits of keys mt * 16 + g (+ 8)
       const uint32_t* kp = reinterpret_cast<const uint32_t*>(kb + kI4Codes);
