@@ -886,7 +886,7 @@ __device__ __forceinline__ int64_t mn_row(const A4Params& p, const MnSeq& s, int
 struct MnMisc {
   uint64_t raw_full[kMnConv];
   uint64_t ev_full[8];             // [tile % 8]
-  uint64_t k_full[2], v_full[2], s_full[3], p_full[3], pv_done[3], m_ready[4][2], r_ready[4][4], mma_done;
+  uint64_t k_full[2], v_full[2], s_full[3], p_full[3], pv_done[3], mma_done;
   uint32_t tmem;
   int32_t last, convert;
   // [tile % 8][32-key piece]: who writes tile t's has seen S(t - 2), so P V(t - 5),
@@ -897,15 +897,14 @@ struct MnMisc {
   float q_amax[2][kMnRows], q_sum[2][kMnRows];
   float q_mul[kMnRows];             // 2^e of the rows
   float score_scale[4];             // scale of the score rows
-  alignas(16) float score[4][3][64];
-  // [tile % 4]: the group that writes tile t + 4's has seen S(t + 4), so P V(t + 1),
-  // so both key halves of tile t + 1 have read R and their maxima of tile t
-  float mx[4][2][kMnRows];          // maximum of logit + ev over a key half
-  float ref[4][kMnRows];            // R after the tile
-  float l[4][kMnRows], l_ref[4][kMnRows];  // the softmax groups' sums and their references
+  alignas(16) float score[4][3][32];
+  // [tile % 2]: a thread writes tile t + 2's after the barrier of tile t + 1,
+  // which the others of its row reach with tile t's read
+  alignas(16) float mx[2][kMnRows][4];  // maximum of logit + ev over a key quarter
+  float l[4][kMnRows];              // the key quarters' sums
 };
 static_assert(sizeof(MnMisc) <= kMnMiscBytes, "misc");
-constexpr int kMnBars = kMnConv + 8 + 38;
+constexpr int kMnBars = kMnConv + 8 + 14;
 static_assert(offsetof(MnMisc, tmem) == kMnBars * 8, "the barriers lie in a row");
 
 // What one row tile of a CTA takes: every role computes the same.
@@ -954,8 +953,8 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
   if (warp < kMnSoft) {
     // ------------------------------------------------------- softmax ----
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMnRegsSoft));
-    // group: keys 64 hk .. of the tiles of parity par
-    const int grp = warp >> 2, par = grp >> 1, hk = grp & 1, r = threadIdx.x & 127;
+    // thread: tile row r, keys 32 grp .. of every tile
+    const int grp = warp >> 2, r = threadIdx.x & 127;
     MnTile c;
     for (int tile = tile0; tile < n_tiles && mn_tile(p, sq, tile, c); tile += p.chunks) {
       const int first = c.first, n_splits = c.n_splits, n_kt = c.n_kt, m0 = c.m0, rows = c.rows;
@@ -963,18 +962,13 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
       // Warps of 32 tile rows: those beyond the rows have nothing to do, the
       // last one at least takes the score rows' logits.
       const int row_warps = (rows + 31) / 32;
-      const int p_warps = 2 * (row_warps + (with_scores && row_warps < 4 ? 1 : 0));
+      const int p_warps = 4 * (row_warps + (with_scores && row_warps < 4 ? 1 : 0));
       if (threadIdx.x == 0) {
         for (int s = 0; s < kMnConv; ++s) mbar_init(&ms.raw_full[s], 1);
         for (int s = 0; s < 8; ++s) mbar_init(&ms.ev_full[s], 1);
         for (int s = 0; s < 2; ++s) {
           mbar_init(&ms.k_full[s], 4);
           mbar_init(&ms.v_full[s], 4);
-          for (int q = 0; q < 4; ++q) {
-            mbar_init(&ms.m_ready[q][s], 2);
-            mbar_init(&ms.r_ready[q][s], 1);
-            mbar_init(&ms.r_ready[q][2 + s], 1);
-          }
         }
         for (int s = 0; s < 3; ++s) {
           mbar_init(&ms.s_full[s], 1);
@@ -1046,48 +1040,35 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
       const float row_mul = score_row ? ms.score_scale[0] : ms.q_mul[r];
       const bool score_warp = with_scores && (warp & 3) == 3;
       const float log_mul = score_row ? 0.f : row_mul * p.scale_log2;
-      float ref_l = -INFINITY, l = 0.f;  // the sum of 2^(logit - ref_l + kMnRaise) over this group's keys
+      float ref = -INFINITY, l = 0.f;  // R, and the sum of 2^(logit - R + kMnRaise) over this thread's keys
       const bool soft = (warp & 3) < row_warps;
+      // A wait that ran out is recorded; the warp goes on without waiting (what
+      // it computes is not used), as the others meet it at named barriers.
       bool ok = true, range_ok = true;
-      for (int t = soft || score_warp ? par : n_kt; t < n_kt; t += 2) {
+      for (int t = soft || score_warp ? 0 : n_kt; t < n_kt; ++t) {
         const int slot = t % 3;
-        const uint32_t ts = tmem + 128 + 128 * slot + tl;
-        ok = a4_wait(&ms.s_full[slot], (t / 3) & 1, p.status) && a4_wait(&ms.ev_full[t & 7], (t >> 3) & 1, p.status);
-        if (!ok) break;
+        const uint32_t ts = tmem + 128 + 128 * slot + 32 * grp + tl;
+        ok = ok && a4_wait(&ms.s_full[slot], (t / 3) & 1, p.status) && a4_wait(&ms.ev_full[t & 7], (t >> 3) & 1, p.status);
         tc_fence_after();
-        // pass 1: logits in log2 units are s * mul (keys past the end
-        // -infinity); mt = max (logit + ev)
-        float mt = -INFINITY;
-#pragma unroll 1
-        for (int g = 2 * hk; g < 2 * hk + 2; ++g) {
-          float v[32];
-          tmem_ld_32x32b_x32(ts + 32 * g, v);
-          const float k = pow2i(ms.ek[t & 7][g]);
-          if (score_warp && lane >= 24 && lane < 27) {
-            // lanes 24 .. 26 hold the three parts' logits
+        // logits in log2 units are v * mul (keys past the end -infinity)
+        float v[32];
+        tmem_ld_32x32b_x32(ts, v);
+        const float k = pow2i(ms.ek[t & 7][grp]);
+        const int ev = ms.ev[t & 7][grp];
+        if (score_warp) {
+          // lanes 24 .. 26 hold the three parts' logits
+          if (lane >= 24 && lane < 27) {
             const float kr = k * row_mul;
 #pragma unroll
             for (int j = 0; j < 32; j += 4)
-              *reinterpret_cast<float4*>(&ms.score[grp][lane - 24][32 * (g & 1) + j]) =
+              *reinterpret_cast<float4*>(&ms.score[grp][lane - 24][j]) =
                   make_float4(v[j] * kr, v[j + 1] * kr, v[j + 2] * kr, v[j + 3] * kr);
           }
-          mt = fmaxf(mt, fmaf(mn_max32(v), log_mul * k, static_cast<float>(ms.ev[t & 7][g])));
-        }
-        if (soft) {
-          ms.mx[t & 3][hk][r] = mt;
           __syncwarp();
-          if (lane == 0) mbar_arrive(&ms.m_ready[warp & 3][par]);
-        }
-        if (score_warp) {
-          __syncwarp();
-          const int n0 = first * kI4Page + t * kMnKeys + 64 * hk;
-          unsigned long long* acc = p.score_acc + static_cast<int64_t>(seq) * p.seqlen_max + n0;
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int n = 32 * u + lane;
-            if (n0 + n < sq.k_end)
-              a4_add_score(acc + n, ms.score[grp][0][n] + ms.score[grp][1][n] + ms.score[grp][2][n], range_ok);
-          }
+          const int n = first * kI4Page + t * kMnKeys + 32 * grp + lane;
+          if (n < sq.k_end)
+            a4_add_score(p.score_acc + static_cast<int64_t>(seq) * p.seqlen_max + n,
+                         ms.score[grp][0][lane] + ms.score[grp][1][lane] + ms.score[grp][2][lane], range_ok);
           __syncwarp();
         }
         if (!soft) {
@@ -1095,67 +1076,53 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
           if (lane == 0) mbar_arrive(&ms.p_full[slot]);  // S is read
           continue;
         }
-        // the reference after the tile before, moved if this tile passes it
-        // (both key halves decide the same)
-        ok = a4_wait(&ms.m_ready[warp & 3][par], (t >> 1) & 1, p.status) &&
-             (t == 0 || a4_wait(&ms.r_ready[warp & 3][(t - 1) & 3], ((t - 1) >> 2) & 1, p.status));
-        if (!ok) break;
-        mt = fmaxf(mt, ms.mx[t & 3][hk ^ 1][r]);
-        float ref = t > 0 ? ms.ref[(t - 1) & 3][r] : -INFINITY;
+        const float mul = log_mul * k;
+        ms.mx[t & 1][r][grp] = fmaf(mn_max32(v), mul, static_cast<float>(ev));
+        asm volatile("bar.sync %0, 128;" ::"r"(3 + (warp & 3)) : "memory");
+        const float4 m4 = *reinterpret_cast<const float4*>(ms.mx[t & 1][r]);
+        const float mt = fmaxf(max3(m4.x, m4.y, m4.z), m4.w);
+        // the reference moves if this tile passes it (a row's four threads
+        // decide the same)
         const bool need = mt > ref + kMnLazy;
-        if (t > 0 && __any_sync(0xffffffffu, need)) {
-          // O holds P V of the tiles before; each key half scales half of its dims
-          ok = a4_wait(&ms.pv_done[(t - 1) % 3], ((t - 1) / 3) & 1, p.status);
-          if (!ok) break;
-          tc_fence_after();
+        if (__any_sync(0xffffffffu, need)) {
           const float a = need ? ex2_approx(ref - mt) : 1.f;
+          if (t > 0) {
+            // O holds P V of the tiles before; each key quarter scales a quarter of its dims
+            ok = ok && a4_wait(&ms.pv_done[(t - 1) % 3], ((t - 1) / 3) & 1, p.status);
+            tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            float ov[16];
-            tmem_ld_32x32b_x16(to + 64 * hk + 16 * c, ov);
+            for (int c = 0; c < 2; ++c) {
+              float ov[16];
+              tmem_ld_32x32b_x16(to + 32 * grp + 16 * c, ov);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) ov[j] *= a;
-            tmem_st_32x32b_x16(to + 64 * hk + 16 * c, ov);
+              for (int j = 0; j < 16; ++j) ov[j] *= a;
+              tmem_st_32x32b_x16(to + 32 * grp + 16 * c, ov);
+            }
+          }
+          if (need) {
+            ref = mt;
+            l *= a;
           }
         }
-        if (need) ref = mt;
-        if (hk == 0) {
-          ms.ref[t & 3][r] = ref;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&ms.r_ready[warp & 3][t & 3]);
-        }
-        if (ref != ref_l) {
-          l *= ex2_approx(ref_l - ref);
-          ref_l = ref;
-        }
-        const float base = kMnRaise - (ref == -INFINITY ? 0.f : ref);
-        // pass 2: P = 2^(logit + ev - R + kMnRaise)
-#pragma unroll 1
-        for (int g = 2 * hk; g < 2 * hk + 2; ++g) {
-          float v[32];
-          tmem_ld_32x32b_x32(ts + 32 * g, v);
-          const int ev = ms.ev[t & 7][g];
-          const float shift = base + static_cast<float>(ev);
-          const float mul = log_mul * pow2i(ms.ek[t & 7][g]);
-          const uint64_t shift2 = pack_f32x2(shift, shift), mul2 = pack_f32x2(mul, mul);
-          uint64_t ps[2] = {0ull, 0ull};  // (zero pairs)
-          uint32_t pw[16];
+        // P = 2^(logit + ev - R + kMnRaise)
+        const float shift = kMnRaise - (ref == -INFINITY ? 0.f : ref) + static_cast<float>(ev);
+        const uint64_t shift2 = pack_f32x2(shift, shift), mul2 = pack_f32x2(mul, mul);
+        uint64_t ps[2] = {0ull, 0ull};  // (zero pairs)
+        uint32_t pw[16];
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            float x, y;
-            unpack_f32x2(fma_f32x2(pack_f32x2(v[j], v[j + 1]), mul2, shift2), x, y);
-            x = ex2_approx(x);
-            y = ex2_approx(y);
-            ps[(j >> 1) & 1] = add_f32x2(ps[(j >> 1) & 1], pack_f32x2(x, y));
-            pw[j >> 1] = pack_f16x2(x, y);
-          }
+        for (int j = 0; j < 32; j += 2) {
           float x, y;
-          unpack_f32x2(add_f32x2(ps[0], ps[1]), x, y);
-          l = fmaf(x + y, pow2i(-ev), l);
-          // P of keys 0 .. 63 in columns 0 .. 31, of keys 64 .. 127 in columns
-          // 64 .. 95: either half writes over logits of its own that it has read
-          tmem_st_32x32b_x16(ts + 64 * hk + 16 * (g & 1), pw);
+          unpack_f32x2(fma_f32x2(pack_f32x2(v[j], v[j + 1]), mul2, shift2), x, y);
+          x = ex2_approx(x);
+          y = ex2_approx(y);
+          ps[(j >> 1) & 1] = add_f32x2(ps[(j >> 1) & 1], pack_f32x2(x, y));
+          pw[j >> 1] = pack_f16x2(x, y);
         }
+        float x, y;
+        unpack_f32x2(add_f32x2(ps[0], ps[1]), x, y);
+        l = fmaf(x + y, pow2i(-ev), l);
+        // over the first half of the logits that this thread has read
+        tmem_st_32x32b_x16(ts, pw);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -1165,18 +1132,11 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
         report(p.status, FDLLM_ERR_RANGE, seq, kA4KernelId);
       // ---- O: this group's 32 dims of row r ----
       ms.l[grp][r] = l;
-      ms.l_ref[grp][r] = ref_l;
       if (ok) a4_wait(&ms.pv_done[(n_kt - 1) % 3], ((n_kt - 1) / 3) & 1, p.status);
       tc_fence_after();
       asm volatile("bar.sync 1, 512;" ::: "memory");
       {
-        const float m_o = ms.ref[(n_kt - 1) & 3][r];
-        float l_o = 0.f;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const float rg = ms.l_ref[g][r];
-          l_o += ms.l[g][r] * (rg == m_o ? 1.f : ex2_approx(rg - m_o));
-        }
+        const float l_o = (ms.l[0][r] + ms.l[1][r]) + (ms.l[2][r] + ms.l[3][r]);
         const bool direct = n_splits == 1;
         const float inv = direct ? (l_o > 0.f ? 1.f / l_o : (l_o == 0.f ? 0.f : l_o)) : 1.f;
         float ov[32];
@@ -1198,7 +1158,7 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
             __stcg(reinterpret_cast<float4*>(part) + (8 * grp + j) * kMnRows + r,
                    make_float4(ov[4 * j], ov[4 * j + 1], ov[4 * j + 2], ov[4 * j + 3]));
           if (grp == 0) {
-            __stcg(part + kMnRows * kA4HeadDim + r, m_o);
+            __stcg(part + kMnRows * kA4HeadDim + r, ref);
             __stcg(part + kMnRows * kA4HeadDim + kMnRows + r, l_o);
           }
         }
@@ -1419,9 +1379,9 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
 #pragma unroll
           for (int g = 0; g < 4; ++g) e[g] = mn_exponent(pr[g]);
           if (t + 1 < n_kt) read(t + 1);
-          // (the slot of tile t - 8 is free: S(t) comes after P V(t - 3).  No
-          // earlier phase would do: it must not pass before this wait sees it)
-          if (!a4_wait(&ms.s_full[t % 3], (t / 3) & 1, p.status)) break;
+          // (with P V(t - 3) done, tile t - 8's are read; the phase cannot pass
+          // before this wait sees it, as P V(t) needs what follows)
+          if (t >= 3 && !a4_wait(&ms.pv_done[t % 3], (t / 3 - 1) & 1, p.status)) break;
           if (lane == 0) {
             *reinterpret_cast<int4*>(ms.ev[t & 7]) = make_int4(e[0], e[1], e[2], e[3]);
             mbar_arrive(&ms.ev_full[t & 7]);
@@ -1446,7 +1406,7 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
               const uint64_t dv = umma_desc_mnmajor_sw128(smem_u32(smem + kMnV + (np & 1) * 2 * kMnHalf), kMnHalf);
 #pragma unroll
               for (int kk = 0; kk < kMnKeys / 16; ++kk)
-                umma_f16_ts(tmem, tmem + 128 + 128 * slot + 8 * kk + (kk & 4) * 8, dv + (kk * 2048 >> 4), idesc_pv,
+                umma_f16_ts(tmem, tmem + 128 + 128 * slot + 32 * (kk >> 1) + 8 * (kk & 1), dv + (kk * 2048 >> 4), idesc_pv,
                             (np > 0 || kk > 0) ? 1u : 0u);
               umma_commit(&ms.pv_done[slot]);
               ++np;
