@@ -56,8 +56,8 @@ SIGNATURES = {
     "fdllm_rope_append": (_int, [_p, _p, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32,
                                  _i64, _p, _i32, _i32, _p]),
     "fdllm_read_cache_int4": (_int, [_p, _p, _p, _p, _p, _i32, _i32, _i32, _i64, _p, _i32, _i32, _p]),
-    "fdllm_attn_int4_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p]),
-    "fdllm_attn_cache_int4": (_int, [_p, _p, _p, _p, _p, _i32, _p, _f32, _i32, _i32, _i32, _i32, _i64, _f32, _i32,
+    "fdllm_attn_int4_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p]),
+    "fdllm_attn_cache_int4": (_int, [_p, _p, _p, _p, _p, _i32, _i32, _p, _f32, _i32, _i32, _i32, _i32, _i64, _f32, _i32,
                                      _i32, _p, _i32, _i32, _p, _sz, _p, _sz, _p]),
     "fdllm_verify_attn": (_int, [_p, _p, _p, _p, _p, _p, _p, _i64, _p, _p, _i32, _i32, _i32, _i32, _i32, _i64,
                                  _f32, _i32, _p, _sz, _p]),

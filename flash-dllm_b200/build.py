@@ -53,7 +53,7 @@ def _binding_cmd() -> list:
     # compiler that links its own statically would not)
     return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
             "-DTORCH_EXTENSION_NAME=_torch_ops", *[f"-I{p}" for p in inc], BINDING_SRC, "-o", BINDING,
-            *[f"-L{p}" for p in libs], "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda",
+            *[f"-L{p}" for p in libs], "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-lc10", "-lc10_cuda",
             f"-L{PKG}", f"-l:{os.path.basename(LIB)}", "-Wl,-rpath,$ORIGIN"]
 
 

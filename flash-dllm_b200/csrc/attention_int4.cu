@@ -50,6 +50,7 @@ struct A4Params {
   int32_t seqlen_max, pages_per_seq;
   int32_t max_items, n_rows;
   int32_t batch;                   // sequences the page table (or the cache) holds
+  int32_t n_seqs;                  // sequences the plan was made for
   int32_t chunks;                  // query chunks of an item that have CTAs of their own
   int32_t splits, split_pages;     // key splits of split_pages pages each
 };
@@ -73,8 +74,16 @@ struct A4Item {
   int seq, k_end, m_start, m_len, t_start, rows, mchunk;
 };
 
+// The plan is of as many sequences as the host took it for (what follows from
+// that number, the grid and where the plan ends, holds).
+__device__ __forceinline__ bool a4_plan_ok(const A4Params& p) {
+  if (p.plan[1] == p.n_seqs) return true;
+  if (threadIdx.x == 0) report(p.status, FDLLM_ERR_TABLE, p.plan[1], kA4KernelId);
+  return false;
+}
+
 __device__ __forceinline__ bool a4_load_item(const A4Params& p, int id, A4Item& it) {
-  if (id >= p.max_items || id >= p.plan[0]) return false;
+  if (!a4_plan_ok(p) || id >= p.max_items || id >= p.plan[0]) return false;
   const int4* e = reinterpret_cast<const int4*>(p.plan + kA4PlanHeader + id * kA4PlanItem);
   const int4 e0 = e[0], e1 = e[1];
   it.seq = e0.x;
@@ -860,7 +869,7 @@ struct MnSeq {
   int k_end, m_start, m_len, t_start, rows;
 };
 __device__ __forceinline__ bool mn_load_seq(const A4Params& p, int seq, MnSeq& s) {
-  if (p.plan[0] <= 0 || seq >= p.plan[1]) return false;
+  if (!a4_plan_ok(p) || p.plan[0] <= 0) return false;
   const int4* e = reinterpret_cast<const int4*>(p.plan + p.plan[3] + seq * kA4PlanSeq);
   const int4 e0 = e[0], e1 = e[1];
   s.k_end = e0.z;
@@ -1553,59 +1562,58 @@ A4Workspace a4_workspace(int32_t max_items, int32_t n_kv, int32_t seqlen_max, co
   return w;
 }
 
-bool a4_args_ok(int32_t n_rows, int32_t max_items, int32_t n_heads, int32_t n_kv, int32_t seqlen_max,
+bool a4_args_ok(int32_t n_rows, int32_t max_items, int32_t n_seqs, int32_t n_heads, int32_t n_kv, int32_t seqlen_max,
                 int32_t kv_splits, int32_t rows_hint) {
-  return n_rows >= 0 && max_items >= 0 && n_kv > 0 && n_heads > 0 && n_heads % n_kv == 0 && n_kv <= 65535 &&
+  return n_rows >= 0 && n_seqs > 0 && max_items >= n_seqs && n_kv > 0 && n_heads > 0 && n_heads % n_kv == 0 && n_kv <= 65535 &&
          n_heads / n_kv <= 64 && seqlen_max > 0 && kv_splits >= 0 && rows_hint >= 0;
 }
 
-A4Plan a4_plan(int32_t n_rows, int32_t max_items, int32_t n_heads, int32_t n_kv, int32_t seqlen_max,
+A4Plan a4_plan(int32_t n_rows, int32_t max_items, int32_t n_seqs, int32_t n_heads, int32_t n_kv, int32_t seqlen_max,
                int32_t kv_splits, int32_t rows_hint, bool scores) {
-  const int row_items = (n_rows + kA4ItemRows - 1) / kA4ItemRows;  // max_items = row_items + sequences
-  const int items = max_items - row_items > row_items ? max_items - row_items : row_items;
-  const int batch = max_items > row_items ? max_items - row_items : 1;
+  const int items = std::max(n_seqs, max_items - n_seqs);  // (the capacity: an item per 64 rows and one a sequence)
   const int seq_rows = rows_hint > 0 && rows_hint < n_rows ? rows_hint : n_rows;
   if (static_cast<long long>(seq_rows) * (n_heads / n_kv) > kFewMaxRows)
-    return a4_plan_many(batch, seq_rows, n_heads / n_kv, n_kv, seqlen_max, kv_splits, scores);
+    return a4_plan_many(n_seqs, seq_rows, n_heads / n_kv, n_kv, seqlen_max, kv_splits, scores);
   const int rows = seq_rows < kA4ItemRows ? seq_rows : kA4ItemRows;
-  return a4_plan_few(items > 0 ? items : 1, rows, n_heads / n_kv, n_kv, seqlen_max, kv_splits);
+  return a4_plan_few(items, rows, n_heads / n_kv, n_kv, seqlen_max, kv_splits);
 }
 
 }  // namespace
 }  // namespace fdllm
 
-extern "C" size_t fdllm_attn_int4_workspace_bytes(int32_t n_rows, int32_t max_items, int32_t n_heads,
-                                                  int32_t n_kv_heads, int32_t seqlen_max, int32_t kv_splits,
+extern "C" size_t fdllm_attn_int4_workspace_bytes(int32_t n_rows, int32_t max_items, int32_t n_seqs,
+                                                  int32_t n_heads, int32_t n_kv_heads, int32_t seqlen_max, int32_t kv_splits,
                                                   int32_t rows_hint, int32_t scores, size_t* scratch_bytes) {
   using namespace fdllm;
   if (scratch_bytes != nullptr) *scratch_bytes = 0;
-  if (!a4_args_ok(n_rows, max_items, n_heads, n_kv_heads, seqlen_max, kv_splits, rows_hint)) return 0;
-  const A4Plan pl = a4_plan(n_rows, max_items, n_heads, n_kv_heads, seqlen_max, kv_splits, rows_hint, scores != 0);
+  if (!a4_args_ok(n_rows, max_items, n_seqs, n_heads, n_kv_heads, seqlen_max, kv_splits, rows_hint)) return 0;
+  const A4Plan pl = a4_plan(n_rows, max_items, n_seqs, n_heads, n_kv_heads, seqlen_max, kv_splits, rows_hint, scores != 0);
   const A4Workspace w = a4_workspace(max_items, n_kv_heads, seqlen_max, pl, scores != 0);
   if (scratch_bytes != nullptr) *scratch_bytes = w.scratch;
   return w.total;
 }
 
 extern "C" int fdllm_attn_cache_int4(const void* q, void* o, const void* k_cache, const void* v_cache,
-                                     const void* plan, int32_t max_items, float* attn_scores, float score_scale,
+                                     const void* plan, int32_t max_items, int32_t n_seqs, float* attn_scores,
+                                     float score_scale,
                                      int32_t n_rows, int32_t n_heads, int32_t n_kv_heads, int32_t seqlen_max,
                                      int64_t n_pages, float softmax_scale, int32_t kv_splits, int32_t rows_hint,
                                      const int32_t* page_table, int32_t batch, int32_t pages_per_seq, void* workspace,
                                      size_t workspace_bytes, void* scratch, size_t scratch_bytes,
                                      cudaStream_t stream) {
   using namespace fdllm;
-  if (!a4_args_ok(n_rows, max_items, n_heads, n_kv_heads, seqlen_max, kv_splits, rows_hint) || n_pages <= 0 ||
+  if (!a4_args_ok(n_rows, max_items, n_seqs, n_heads, n_kv_heads, seqlen_max, kv_splits, rows_hint) || n_pages <= 0 ||
       n_pages > (int64_t(1) << 31) || !(softmax_scale > 0.f))
     return FDLLM_ERR_ARG;
   if (page_table != nullptr ? (batch <= 0 || pages_per_seq <= 0 ||
                                static_cast<int64_t>(pages_per_seq) * kI4Page < seqlen_max)
                             : seqlen_max % kI4Page != 0)
     return FDLLM_ERR_ARG;
-  if (max_items == 0 || n_rows == 0) return FDLLM_OK;
+  if (n_rows == 0) return FDLLM_OK;
   const void* ptrs[] = {q, o, k_cache, v_cache, plan};
   for (const void* x : ptrs)
     if (x == nullptr || !aligned16(x)) return FDLLM_ERR_ARG;
-  const A4Plan pl = a4_plan(n_rows, max_items, n_heads, n_kv_heads, seqlen_max, kv_splits, rows_hint,
+  const A4Plan pl = a4_plan(n_rows, max_items, n_seqs, n_heads, n_kv_heads, seqlen_max, kv_splits, rows_hint,
                             attn_scores != nullptr);
   const A4Workspace w = a4_workspace(max_items, n_kv_heads, seqlen_max, pl, attn_scores != nullptr);
   if (w.total > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < w.total))
@@ -1638,6 +1646,7 @@ extern "C" int fdllm_attn_cache_int4(const void* q, void* o, const void* k_cache
   p.seqlen_max = seqlen_max;
   p.max_items = max_items;
   p.n_rows = n_rows;
+  p.n_seqs = n_seqs;
   p.batch = page_table != nullptr ? batch : static_cast<int32_t>(std::min<int64_t>(n_pages / p.pages_per_seq, 1 << 20));
   p.chunks = pl.chunks;
   p.splits = pl.splits;

@@ -1385,7 +1385,9 @@ int fdllm_gemm_bf16(const void* a, const void* w, void* out, const void* residua
 }
 
 size_t fdllm_gemm_int8_workspace_bytes(int32_t n_rows, int32_t n_cols, int32_t k_dim, int32_t swiglu) {
-  if (n_rows <= 0 || n_cols <= 0 || k_dim <= 0) return fdllm::kGFlagBytes;
+  if (n_rows <= 0 || n_cols <= 0 || k_dim <= 0 ||
+      fdllm::gemv_int8_rows(n_rows, static_cast<int64_t>(n_cols) * k_dim))
+    return 0;
   return fdllm::gemm_ws_bytes(
       fdllm::plan_gemm(swiglu ? fdllm::kEpiSwiglu : fdllm::kEpiStore, n_rows, n_cols, (k_dim + 1) / 2, 0, true));
 }

@@ -11,6 +11,7 @@
 // FdllmError for a status of the library (the class is registered by ops.py).
 // Every call runs on the device of its tensors, on torch's current stream
 // there.
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -141,6 +142,12 @@ struct Call {
   }
 };
 
+// (the allocator itself: at::empty's way through the dispatcher costs as much
+// again as the allocation, at up to three outputs a call)
+Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
+
 int32_t i32(int64_t v, const char* name) {
   TORCH_CHECK_VALUE(v >= 0 && v <= INT32_MAX, name, " is out of range: ", v);
   return static_cast<int32_t>(v);
@@ -152,8 +159,8 @@ void* opt_ptr(const OptTensor& t) { return t.has_value() ? t->data_ptr() : nullp
 std::tuple<Tensor, Tensor> quantize_int8(const Tensor& x) {
   Call c(x, "quantize_int8");
   const int64_t ld = c.rows(x, "x", -1, -1);
-  Tensor codes = at::empty(x.sizes(), x.options().dtype(at::kChar));
-  Tensor scale = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
+  Tensor codes = empty(x.sizes(), at::kChar, x);
+  Tensor scale = empty({x.size(0)}, at::kFloat, x);
   check_status("fdllm_quantize_int8",
                fdllm_quantize_int8(x.data_ptr(), ld, codes.data_ptr(), static_cast<float*>(scale.data_ptr()),
                                    i32(x.size(0), "rows"), i32(x.size(1), "dim"), c.stream));
@@ -165,8 +172,8 @@ std::tuple<Tensor, Tensor> rmsnorm_int8(const Tensor& x, const Tensor& weight, d
   c.plain(x, "x", at::kBFloat16, 2);
   c.plain(weight, "weight", at::kBFloat16, 1);
   TORCH_CHECK_VALUE(weight.size(0) == x.size(1), "weight must have ", x.size(1), " values, got ", weight.size(0));
-  Tensor codes = at::empty(x.sizes(), x.options().dtype(at::kChar));
-  Tensor scale = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
+  Tensor codes = empty(x.sizes(), at::kChar, x);
+  Tensor scale = empty({x.size(0)}, at::kFloat, x);
   check_status("fdllm_rmsnorm_int8",
                fdllm_rmsnorm_int8(x.data_ptr(), weight.data_ptr(), codes.data_ptr(),
                                   static_cast<float*>(scale.data_ptr()), i32(x.size(0), "rows"),
@@ -195,7 +202,7 @@ Tensor linear_int8(const Tensor& a, const Tensor& a_scale, const Tensor& w, cons
   Call c(a, "linear_int8");
   const Int8Shape s = int8_operands(c, a, a_scale, w, w_scale);
   const int64_t ld_res = residual.has_value() ? c.rows(*residual, "residual", s.rows, s.n) : 0;
-  Tensor y = out.has_value() ? *out : at::empty({s.rows, s.n}, a.options().dtype(at::kBFloat16));
+  Tensor y = out.has_value() ? *out : empty({s.rows, s.n}, at::kBFloat16, a);
   const int64_t ld_out = out.has_value() ? c.rows(y, "out", s.rows, s.n) : s.n;
   size_t size = 0;
   void* ws = workspaces().get(a.device(), c.stream, "int8", fdllm_gemm_int8_workspace_bytes(s.rows, s.n, s.k, 0),
@@ -211,7 +218,7 @@ Tensor linear_swiglu_int8(const Tensor& a, const Tensor& a_scale, const Tensor& 
   Call c(a, "linear_swiglu_int8");
   const Int8Shape s = int8_operands(c, a, a_scale, w, w_scale);
   TORCH_CHECK_VALUE(s.n % 2 == 0, "w_gate_up must be [2H, K]");
-  Tensor y = at::empty({s.rows, s.n / 2}, a.options().dtype(at::kBFloat16));
+  Tensor y = empty({s.rows, s.n / 2}, at::kBFloat16, a);
   size_t size = 0;
   void* ws = workspaces().get(a.device(), c.stream, "int8", fdllm_gemm_int8_workspace_bytes(s.rows, s.n, s.k, 1),
                               kGemmFlagBytes, &size);
@@ -293,7 +300,7 @@ Tensor rope_append(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
     TORCH_CHECK_VALUE(out.size(0) == rows && out.size(1) == n_heads * kHead, "q_out must be [", rows, ", ",
                       n_heads * kHead, "], got ", out.sizes());
   } else if (sin.has_value()) {
-    out = at::empty({rows, n_heads * kHead}, q.options());
+    out = empty({rows, n_heads * kHead}, at::kBFloat16, q);
   }
   check_status("fdllm_rope_append",
                fdllm_rope_append(q.data_ptr(), k.data_ptr(), v.data_ptr(), ldq, ldk, ldv,
@@ -313,8 +320,8 @@ std::tuple<Tensor, Tensor> read_cache_int4(const Tensor& k_cache, const Tensor& 
   const int64_t n_pages = int4_pages(c, k_cache, v_cache, hk);
   c.plain(slots, "slots", at::kLong, 1);
   const Pages pt = page_table(c, table, seqlen_max);
-  const auto opts = k_cache.options().dtype(at::kBFloat16);
-  Tensor k = at::empty({slots.size(0), hk * kHead}, opts), v = at::empty({slots.size(0), hk * kHead}, opts);
+  Tensor k = empty({slots.size(0), hk * kHead}, at::kBFloat16, slots);
+  Tensor v = empty({slots.size(0), hk * kHead}, at::kBFloat16, slots);
   check_status("fdllm_read_cache_int4",
                fdllm_read_cache_int4(k_cache.data_ptr(), v_cache.data_ptr(),
                                      static_cast<const int64_t*>(slots.data_ptr()), k.data_ptr(), v.data_ptr(),
@@ -338,25 +345,26 @@ void attn_cache_int4(const Tensor& q, const Tensor& o, const Tensor& k_cache, co
   const int64_t n_pages = int4_pages(c, k_cache, v_cache, n_kv_heads);
   c.plain(plan, "plan", at::kInt, 1);
   const Pages pt = page_table(c, table, seqlen_max);
-  TORCH_CHECK_VALUE(capacity >= 0 && plan.numel() >= 8 + 8 * capacity, "plan is smaller than its capacity");
-  const int64_t rows = q.size(0);
+  // (a plan holds a header, its capacity in items and a record per sequence, 8 words each)
+  const int64_t rows = q.size(0), n_seqs = plan.numel() / 8 - 1 - capacity;
+  TORCH_CHECK_VALUE(plan.numel() % 8 == 0 && capacity > 0 && n_seqs > 0 && n_seqs <= capacity,
+                    "plan and capacity are not of one plan_cache_attention");
   if (scores.has_value()) {
     c.plain(*scores, "attn_scores", at::kFloat, -1);
-    // (the plan's sequences: its capacity minus an item per 64 rows)
-    TORCH_CHECK_VALUE(scores->numel() >= (capacity - (rows + 63) / 64) * seqlen_max,
+    TORCH_CHECK_VALUE(scores->numel() >= n_seqs * seqlen_max,
                       "attn_scores must be [batch * seqlen_max]");
   }
-  const int32_t r = i32(rows, "rows"), cap = i32(capacity, "capacity"), h = i32(n_heads, "n_heads"),
+  const int32_t r = i32(rows, "rows"), cap = i32(capacity, "capacity"), seqs = i32(n_seqs, "sequences"), h = i32(n_heads, "n_heads"),
                 hk = i32(n_kv_heads, "n_kv_heads"), len = static_cast<int32_t>(seqlen_max),
                 splits = i32(kv_splits, "kv_splits"), hint = i32(rows_hint, "rows_hint");
   size_t scratch_bytes = 0, ws_size = 0, scratch_size = 0;
   const size_t ws_bytes =
-      fdllm_attn_int4_workspace_bytes(r, cap, h, hk, len, splits, hint, scores.has_value(), &scratch_bytes);
+      fdllm_attn_int4_workspace_bytes(r, cap, seqs, h, hk, len, splits, hint, scores.has_value(), &scratch_bytes);
   void* ws = workspaces().get(q.device(), c.stream, "attn4", ws_bytes, ws_bytes, &ws_size);
   void* scratch = workspaces().get(q.device(), c.stream, "attn4s", scratch_bytes, 0, &scratch_size);
   check_status("fdllm_attn_cache_int4",
                fdllm_attn_cache_int4(q.data_ptr(), o.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-                                     plan.data_ptr(), cap, static_cast<float*>(opt_ptr(scores)),
+                                     plan.data_ptr(), cap, seqs, static_cast<float*>(opt_ptr(scores)),
                                      static_cast<float>(score_scale), r, h, hk, len, n_pages,
                                      static_cast<float>(softmax_scale), splits, hint, pt.table, pt.batch, pt.per_seq,
                                      ws, ws_size, scratch, scratch_size, c.stream));

@@ -138,9 +138,10 @@ int fdllm_rmsnorm_int8(const void* x, const void* weight, void* codes, float* sc
  *   out[r, c] = bf16(float(sum_k a[r, k] * w[c, k]) * a_scale[r] * w_scale[c] (+ residual[r, c]))
  * a int8 [n_rows, k_dim], w int8 [n_cols, k_dim] (both contiguous), scales fp32, out / residual bf16 with
  * row strides ld_out / ld_res elements (residual may be NULL).  The sum is an exact 32-bit integer,
- * rounded to fp32 once.  n_cols a multiple of 8, k_dim a multiple of 16 and at most 131056.  The
- * stream-K tcgen05 GEMM of fdllm_gemm_bf16 with kind::i8 instructions; workspace as there, its first
- * 4096 bytes (the flags) zero before first use. */
+ * rounded to fp32 once.  n_cols a multiple of 8, k_dim a multiple of 16 and at most 131056.  Up to eight
+ * rows a dp4a kernel without a workspace (the size is 0), above the stream-K tcgen05 GEMM of
+ * fdllm_gemm_bf16 with kind::i8 instructions; workspace as there, its first 4096 bytes (the flags) zero
+ * before first use. */
 size_t fdllm_gemm_int8_workspace_bytes(int32_t n_rows, int32_t n_cols, int32_t k_dim, int32_t swiglu);
 int fdllm_gemm_int8(const void* a, const float* a_scale, const void* w, const float* w_scale, void* out,
                     const void* residual, int32_t n_rows, int32_t n_cols, int32_t k_dim, int64_t ld_out,
@@ -279,7 +280,8 @@ int fdllm_read_cache_int4(const void* k_cache, const void* v_cache, const int64_
 
 /* fdllm_attn_cache over the 4-bit cache.  q, o bf16 [n_rows, n_heads * 128]; n_heads a multiple of
  * n_kv_heads (query head h reads kv head h / (n_heads / n_kv_heads); at most 64 per kv head); plan and
- * max_items as for fdllm_attn_cache; page_table int32 [batch, pages_per_seq] or NULL (sequence b owns
+ * max_items as for fdllm_attn_cache, n_seqs the plan's batch_size (a plan of another one is reported as
+ * FDLLM_ERR_TABLE and nothing is computed); page_table int32 [batch, pages_per_seq] or NULL (sequence b owns
  * pages [b * seqlen_max / 64, ...), seqlen_max a multiple of 64); a page outside the cache is reported as
  * FDLLM_ERR_INDEX and read as page 0.  attn_scores and score_scale as there.
  *   rows_hint  rows of one sequence the caller expects at most (0: unknown): chooses the kernel and the
@@ -288,12 +290,12 @@ int fdllm_read_cache_int4(const void* k_cache, const void* v_cache, const int64_
  * The sizes of the workspace (returned) and of the scratch (*scratch_bytes) depend on the arguments as
  * passed here.  The workspace is zero before first use and every call leaves it zero (zero it again after
  * a call whose device status reported an error); the scratch may hold anything. */
-size_t fdllm_attn_int4_workspace_bytes(int32_t n_rows, int32_t max_items, int32_t n_heads, int32_t n_kv_heads,
-                                       int32_t seqlen_max, int32_t kv_splits, int32_t rows_hint, int32_t scores,
-                                       size_t* scratch_bytes);
+size_t fdllm_attn_int4_workspace_bytes(int32_t n_rows, int32_t max_items, int32_t n_seqs, int32_t n_heads,
+                                       int32_t n_kv_heads, int32_t seqlen_max, int32_t kv_splits, int32_t rows_hint,
+                                       int32_t scores, size_t* scratch_bytes);
 int fdllm_attn_cache_int4(const void* q, void* o, const void* k_cache, const void* v_cache, const void* plan,
-                          int32_t max_items, float* attn_scores, float score_scale, int32_t n_rows, int32_t n_heads,
-                          int32_t n_kv_heads, int32_t seqlen_max, int64_t n_pages, float softmax_scale,
+                          int32_t max_items, int32_t n_seqs, float* attn_scores, float score_scale, int32_t n_rows,
+                          int32_t n_heads, int32_t n_kv_heads, int32_t seqlen_max, int64_t n_pages, float softmax_scale,
                           int32_t kv_splits, int32_t rows_hint, const int32_t* page_table, int32_t batch,
                           int32_t pages_per_seq, void* workspace, size_t workspace_bytes, void* scratch, size_t scratch_bytes,
                           cudaStream_t stream);

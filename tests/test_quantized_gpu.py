@@ -486,6 +486,43 @@ def test_attn_cache_int4_plan_of_another_shape_is_reported():
         check_device_status()
 
 
+@pytest.mark.parametrize("rows", [1, 40])
+def test_attn_cache_int4_rows_behind_the_last_sequence(rows):
+    """More rows than the plan was made for: all its sequences are computed,
+    the rows behind them stay."""
+    from flash_dllm_b200 import ops
+    from flash_dllm_b200._lib import check_device_status
+    q, caches, pt, spans, mb, tb, B, L = _attention_case(9, [(200, rows, 0), (150, rows, 0), (64, rows, 0)], 2, 2, 200)
+    plan, cap = ops.plan_cache_attention(mb, tb, q.shape[0], B, 64, L, q.device)
+    more = torch.cat([q, torch.full((150, 256), float("nan"), device="cuda", dtype=q.dtype)])
+    out, sc = torch.full_like(more, 5.0), torch.zeros(B * L, device="cuda")
+    ops.attn_cache_int4(more, out, *caches, plan, cap, sc, 1.0, 2, 2, L, 128 ** -0.5, rows_hint=rows, page_table=pt)
+    check_device_status()
+    assert (out[q.shape[0]:] == 5).all()
+    ref = torch.full_like(q, 5.0)  # (q has rows of its own behind the last sequence)
+    sc_ref = torch.zeros_like(sc)
+    ops.attn_cache_int4(q, ref, *caches, plan, cap, sc_ref, 1.0, 2, 2, L, 128 ** -0.5, rows_hint=rows, page_table=pt)
+    assert torch.equal(out[:q.shape[0]], ref) and torch.equal(sc, sc_ref)
+
+
+def test_attn_cache_int4_plan_and_capacity_go_together():
+    from flash_dllm_b200 import ops
+    from flash_dllm_b200._lib import FdllmError, check_device_status
+    q, caches, pt, spans, mb, tb, B, L = _attention_case(9, [(200, 3, 0), (150, 3, 0)], 2, 2, 200)
+    plan, cap = ops.plan_cache_attention(mb, tb, q.shape[0], B, 64, L, q.device)
+    out = torch.full_like(q, 5.0)
+    args = (None, 1.0, 2, 2, L, 0.1)
+    for p, c in ((plan[:-4], cap), (plan, 0), (plan, 10 ** 6), (plan[:8], cap)):
+        with pytest.raises(ValueError, match="plan"):
+            ops.attn_cache_int4(q, out, *caches, p.contiguous(), c, *args, page_table=pt)
+    # consistent sizes, but not this plan's: found on the device
+    for c, hint in ((cap + 1, 1), (cap + 1, 40)):
+        ops.attn_cache_int4(q, out, *caches, plan, c, *args, rows_hint=hint, page_table=pt)
+        with pytest.raises(FdllmError):
+            check_device_status()
+    assert (out == 5).all()
+
+
 # ------------------------------------------------- streams, graphs, a run --
 
 def _step(ops, st):
