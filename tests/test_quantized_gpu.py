@@ -209,6 +209,27 @@ def test_linear_swiglu_int8_few_rows(rows, h, k, gemm_plan):
     test_linear_swiglu_int8(rows, h, k, {}, gemm_plan)
 
 
+@pytest.mark.parametrize("rows", [1, 6, 30, 200])
+@pytest.mark.parametrize("norm", [False, True])
+def test_linear_int8_of_codes_made_just_before(rows, norm):
+    """Both operands quantised right before the product (products of
+    activations): nothing of them is read before it is written."""
+    from flash_dllm_b200 import ops
+    g = _gen(rows)
+    one = torch.ones(1024, device="cuda", dtype=torch.bfloat16)
+    xs = [_randn(g, 520, 1024).bfloat16() for _ in range(6)]
+    ys, refs = [], []
+    for i in range(30):
+        a, sa = ops.quantize_int8(xs[i % 6][:rows])
+        w, sw = ops.rmsnorm_int8(xs[(i + 1) % 6], one, 1e-5) if norm else ops.quantize_int8(xs[(i + 1) % 6])
+        ys.append(ops.linear_int8(a, sa, w, sw))
+        refs.append((a, sa, w, sw))
+        del a, sa, w, sw
+    for y, r in zip(ys, refs):
+        ref, tol = _linear_ref(*r)
+        assert ((y.double() - ref).abs() <= tol).all()
+
+
 # ------------------------------------------------------ append to a cache --
 
 def _append_case(seed, seqs, tokens, h, hk, length, bits, table=True):
