@@ -906,6 +906,7 @@ struct MnMisc {
   float q_amax[2][kMnRows], q_sum[2][kMnRows];
   float q_mul[kMnRows];             // 2^e of the rows
   float score_scale[4];             // scale of the score rows
+  float row_sum[2][kA4HeadDim];
   alignas(16) float score[4][3][32];
   // [tile % 2]: a thread writes tile t + 2's after the barrier of tile t + 1,
   // which the others of its row reach with tile t's read
@@ -913,8 +914,8 @@ struct MnMisc {
   float l[4][kMnRows];              // the key quarters' sums
 };
 static_assert(sizeof(MnMisc) <= kMnMiscBytes, "misc");
-constexpr int kMnBars = kMnConv + 8 + 14;
-static_assert(offsetof(MnMisc, tmem) == kMnBars * 8, "the barriers lie in a row");
+constexpr int kMnBars = 8 + 14;
+static_assert(offsetof(MnMisc, tmem) - offsetof(MnMisc, ev_full) == kMnBars * 8, "the barriers lie in a row");
 
 // What one row tile of a CTA takes: every role computes the same.
 struct MnTile {
@@ -973,7 +974,6 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
       const int row_warps = (rows + 31) / 32;
       const int p_warps = 4 * (row_warps + (with_scores && row_warps < 4 ? 1 : 0));
       if (threadIdx.x == 0) {
-        for (int s = 0; s < kMnConv; ++s) mbar_init(&ms.raw_full[s], 1);
         for (int s = 0; s < 8; ++s) mbar_init(&ms.ev_full[s], 1);
         for (int s = 0; s < 2; ++s) {
           mbar_init(&ms.k_full[s], 4);
@@ -1173,12 +1173,12 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
         }
       }
       // every role is done with this tile: its barriers and buffers are free
-      __threadfence();
+      if (n_splits > 1 || with_scores) __threadfence();  // (partial results, column sums)
       tc_fence_before();
       __syncthreads();
       tc_fence_after();
       if (threadIdx.x == 0) {
-        uint64_t* b = ms.raw_full;  // every barrier, in a row
+        uint64_t* b = ms.ev_full;  // every barrier but the conversion warps' own, in a row
         for (int i = 0; i < kMnBars; ++i) mbar_inval(b + i);
       }
       if (n_splits > 1) {
@@ -1241,14 +1241,50 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
     MnTile c;
     for (int tile = tile0; tile < n_tiles && mn_tile(p, sq, tile, c); tile += p.chunks) {
       const int first = c.first, n_pages = c.n_pages, n_kt = c.n_kt;
-      if (c.with_scores && warp < kMnSoft + 4) {
-        // rows 120 .. 122: the sum of the masked rows over rows and heads, in
-        // three fp16 parts; rows 123 .. 127 zero.  Thread = dim.
-        const int d = threadIdx.x - 32 * kMnSoft;
-        float acc = 0.f;
+      // pieces in order, four a tile: this warp's are cw, cw + 6, ...
+      const int cw = (warp - kMnSoft) % (kMnConv / 2);
+      const bool is_v = warp >= kMnSoft + kMnConv / 2;
+      uint8_t* piece = smem + kMnRaw + (warp - kMnSoft) * kMnPieceBytes;
+      uint64_t* full = ms.raw_full + (warp - kMnSoft);  // (this warp's alone)
+      if (lane == 0) mbar_init(full, 1);
+      fence_barrier_init();
+      __syncwarp();
+      const uint8_t* cache = (is_v ? p.vc : p.kc) + static_cast<size_t>(kvh) * kI4Block;
+      const int64_t page_stride = static_cast<int64_t>(p.n_kv) * kI4Block;
+      // pages of this warp's next 32 pieces, one a lane, read ahead of their use
+      auto page_of = [&](int k) -> int {
+        const int j = (cw + 6 * k) >> 1;
+        return j < n_pages ? static_cast<int>(a4_page(p, seq, first + j)) : 0;
+      };
+      int pages = page_of(lane);
+      auto load = [&](int k) {  // this warp's k-th piece (the whole warp)
+        if ((k & 31) == 0 && k > 0) pages = page_of(k + lane);
+        const int page = __shfl_sync(0xffffffffu, pages, k & 31);
+        const int u = cw + 6 * k;
+        if (lane == 0 && (u >> 1) < n_pages) {
+          const uint8_t* block = cache + page * page_stride;
+          mbar_arrive_expect_tx(full, kMnPieceBytes);
+          bulk_load(piece, block + (u & 1) * (kMnPiece * kI4Row), kMnPiece * kI4Row, full);
+          bulk_load(piece + kMnPiece * kI4Row, block + kI4Codes + (u & 1) * (kMnPiece * 4), kMnPiece * 4, full);
+        }
+      };
+      static_assert(kMnConv == 12, "six warps each");
+      load(0);  // on its way while the query operand is laid out
+      float row_sum = 0.f;
+      if (c.with_scores) {
+        // the sum of the masked rows over rows and heads, a third of them to
+        // each four warps; thread = dim
+        const int third = (warp - kMnSoft) >> 2, d = threadIdx.x & 127;
         const int n = sq.m_len * p.group;
 #pragma unroll 8
-        for (int m = 0; m < n; ++m) acc += __bfloat162float(p.q[mn_row(p, sq, kvh, m) + d]);
+        for (int m = third; m < n; m += 3) row_sum += __bfloat162float(p.q[mn_row(p, sq, kvh, m) + d]);
+        if (third > 0) ms.row_sum[third - 1][d] = row_sum;
+        asm volatile("bar.sync 7, 384;" ::: "memory");
+      }
+      if (c.with_scores && warp < kMnSoft + 4) {
+        // rows 120 .. 122: that sum in three fp16 parts; rows 123 .. 127 zero
+        const int d = threadIdx.x - 32 * kMnSoft;
+        const float acc = row_sum + ms.row_sum[0][d] + ms.row_sum[1][d];
         float mag = fabsf(acc) <= 3.4e38f ? fabsf(acc) : 3.4e38f;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) mag = fmaxf(mag, __shfl_xor_sync(0xffffffffu, mag, o));
@@ -1290,32 +1326,6 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
       tc_fence_before();
       __syncthreads();
       tc_fence_after();
-      // pieces in order, four a tile: this warp's are cw, cw + 6, ...
-      const int cw = (warp - kMnSoft) % (kMnConv / 2);
-      const bool is_v = warp >= kMnSoft + kMnConv / 2;
-      uint8_t* piece = smem + kMnRaw + (warp - kMnSoft) * kMnPieceBytes;
-      uint64_t* full = ms.raw_full + (warp - kMnSoft);
-      const uint8_t* cache = (is_v ? p.vc : p.kc) + static_cast<size_t>(kvh) * kI4Block;
-      const int64_t page_stride = static_cast<int64_t>(p.n_kv) * kI4Block;
-      // pages of this warp's next 32 pieces, one a lane, read ahead of their use
-      auto page_of = [&](int k) -> int {
-        const int j = (cw + 6 * k) >> 1;
-        return j < n_pages ? static_cast<int>(a4_page(p, seq, first + j)) : 0;
-      };
-      int pages = page_of(lane);
-      auto load = [&](int k) {  // this warp's k-th piece (the whole warp)
-        if ((k & 31) == 0 && k > 0) pages = page_of(k + lane);
-        const int page = __shfl_sync(0xffffffffu, pages, k & 31);
-        const int u = cw + 6 * k;
-        if (lane == 0 && (u >> 1) < n_pages) {
-          const uint8_t* block = cache + page * page_stride;
-          mbar_arrive_expect_tx(full, kMnPieceBytes);
-          bulk_load(piece, block + (u & 1) * (kMnPiece * kI4Row), kMnPiece * kI4Row, full);
-          bulk_load(piece + kMnPiece * kI4Row, block + kI4Codes + (u & 1) * (kMnPiece * 4), kMnPiece * 4, full);
-        }
-      };
-      static_assert(kMnConv == 12, "six warps each");
-      load(0);
       for (int k = 0; cw + 6 * k < 4 * n_kt; ++k) {
         const int u = cw + 6 * k, t = u >> 2, w = u & 3, s = t & 1;
         const int j = u >> 1;  // page
@@ -1346,6 +1356,8 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
         __syncwarp();
         if (lane == 0) mbar_arrive(is_v ? &ms.v_full[s] : &ms.k_full[s]);
       }
+      __syncwarp();
+      if (lane == 0) mbar_inval(full);
       tc_fence_before();
       __syncthreads();
       tc_fence_after();
