@@ -987,6 +987,10 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
         mbar_init(&ms.mma_done, 1);
         fence_barrier_init();
       }
+      if (warp == 0) {  // the barriers are there: conversion begins
+        __syncwarp();
+        asm volatile("bar.arrive 8, 448;" ::: "memory");
+      }
       // ---- the query operand ----
       if (grp < 2) {
         const int h = grp;
@@ -1040,7 +1044,7 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
       }
       fence_proxy_async_smem();
       tc_fence_before();
-      __syncthreads();
+      asm volatile("bar.sync 9, 1024;" ::: "memory");
       tc_fence_after();
       const uint32_t tmem = ms.tmem;
       const uint32_t tl = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -1324,8 +1328,8 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
       }
       fence_proxy_async_smem();
       tc_fence_before();
-      __syncthreads();
-      tc_fence_after();
+      asm volatile("bar.arrive 9, 1024;" ::: "memory");  // the score rows are in place
+      asm volatile("bar.sync 8, 448;" ::: "memory");     // the barriers are
       for (int k = 0; cw + 6 * k < 4 * n_kt; ++k) {
         const int u = cw + 6 * k, t = u >> 2, w = u & 3, s = t & 1;
         const int j = u >> 1;  // page
@@ -1368,9 +1372,14 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
     MnTile c;
     for (int tile = tile0; tile < n_tiles && mn_tile(p, sq, tile, c); tile += p.chunks) {
       const int n_kt = c.n_kt;
-      tc_fence_before();
-      __syncthreads();
-      tc_fence_after();
+      if (warp == 29) {
+        asm volatile("bar.arrive 9, 1024;" ::: "memory");
+        asm volatile("bar.sync 8, 448;" ::: "memory");
+      } else {
+        tc_fence_before();
+        asm volatile("bar.sync 9, 1024;" ::: "memory");
+        tc_fence_after();
+      }
       const uint32_t tmem = ms.tmem;
       if (warp == 29) {
         // the exponents of V's pieces, ahead of their conversion: P needs
