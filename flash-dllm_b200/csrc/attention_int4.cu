@@ -2,15 +2,16 @@
 // as the bf16 cache attention: an item is up to 64 query rows of one sequence,
 // its masked rows first; keys [0, k_end) of the sequence.
 //
-// The dequantisation is folded out of the products.  With c = code - 8 (an
-// exact bf16 integer), step s and base b = low + 8 s of a (token, head) group,
+// Two kernels.  With few rows the cache's bytes and the conversion of its codes
+// are all the work, and the step s and base b of a (token, head) group are
+// folded out of the products:
 //   q . k_n = s_n (q . c_n) + b_n sum_d q_d
 //   o_d     = [ sum_n (p_n s_n) c_nd + sum_n p_n b_n ] / sum_n p_n
-// so the matrix instructions see small integers and bf16 queries or
-// probabilities, a key's step multiplies one logit or one probability instead
-// of 128 values, and the base costs one scalar per row.  p_n s_n is rounded
-// to bf16 once (it is the operand of the second product); sums, maxima and
-// logits stay in fp32.
+// so the matrix instructions see small integers, a key's step multiplies one
+// logit or one probability instead of 128 values, and the base costs one
+// scalar per row (mma.sync, keys in M).  With many rows the products are the
+// work, and the values themselves are formed as operands of the tensor cores
+// (tcgen05, 128 x 128 tiles).  Sums, maxima and logits stay in fp32.
 #include "common.cuh"
 #include "int4.cuh"
 #include "internal.h"
@@ -165,6 +166,15 @@ __device__ __forceinline__ void a4_convert_scores(const A4Params& p, int seq, in
 // running maximum, and are joined in shared memory.  Two CTAs share an SM.
 // Long key ranges are split over CTAs; the last one to finish joins the
 // partial results in split order, so the result does not depend on timing.
+//
+// Measured: 4 sequences of 65536 keys, 32 heads on 8 kv heads, one row each (285
+// MB): 57.7 us, 4.9 TB/s.  8 of 2176, 32 kv heads (76 MB): 22.4 us.  Some 920
+// instructions a page and warp, ALU 56 % busy, no unit more: what is left is
+// the latency of one page's chain (products, reductions, exponentials,
+// transposes, products), which sixteen warps an SM overlap only so far, and 4 us
+// of beginning and end a CTA.  Dividing pages evenly over a fixed grid (pieces
+// across sequences and heads) cost more in pieces than it gained in balance:
+// 8 of 2176 22.4 -> 29.6 us, 4 of 65536 57.9 -> 56.5.
 //
 // kE: logit columns of a lane that are used.  A fragment's lane holds columns
 // 2 t and 2 t + 1; with up to four rows they all go to the even columns, and
@@ -672,21 +682,27 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) attn_int4_few_kernel(co
 // column sums carry 22 bits and more.
 //
 // P goes from the registers to tensor memory and is the second product's A
-// operand there: the kernel's tightest resource is shared memory (per tile 72
-// KB of operands for S, 32 for P V, 72 written by the conversion, 34 of codes
-// in and out = 210 KB, 1640 clocks at 128 bytes a clock, against 1000 for the
-// tensor cores' 17 instructions of about 60 clocks, 1024 for the exponentials
-// at 16 a clock and about 900 issue slots of each scheduler).
+// operand there: of shared memory a tile takes 210 KB as it is (72 of operands
+// for S, 32 for P V, 72 written by the conversion, 34 of codes in and out).
 //
-// Warps (32): 0-15 softmax, 16-21 and 22-27 conversion of K and of V (the
-// 32-key pieces of the tiles in turn; a warp fetches its own), 28 the MMA
-// thread.  A tile's softmax is shared by two groups of four warps (thread =
-// tile row x 64 keys), two more work on the next tile; the reference R of a row
-// passes from tile to tile through shared memory right after a tile's maximum
-// is known, so the exponentials of consecutive tiles overlap.  Tensor memory:
-// O and three S tiles with P over them: S(t) is issued two tiles ahead of P
-// V(t).  Warp 29 works out V's exponents ahead of V's conversion.
-// Key ranges are split over CTAs as in the other kernel.
+// Warps (32): 0-15 softmax (thread = tile row x 32 keys; the four threads of a
+// row meet at a named barrier for the maximum, each keeps the row's reference),
+// 16-21 and 22-27 conversion of K and of V (the 32-key pieces of the tiles in
+// turn; a warp fetches its own), 28 the MMA thread, 29 V's exponents ahead of
+// V's conversion.  Tensor memory: O and three S tiles with P over them, S(t)
+// two tiles ahead of P V(t).  The first tiles are converted while the query
+// operand is laid out.  Key ranges are split over CTAs as in the other kernel.
+//
+// Measured: 2048 rows of one sequence of 2176, 32 heads: 142.7 us (512 CTAs of
+// 17 tiles in 3.5 waves), 0.26 of the fp16 rate; 96 rows of four of 8192, with
+// scores, 127 us; 64 of eight of 896, with scores, 47.5 us.  A tile takes about
+// 2900 clocks, of which the tensor cores' 17 instructions 1900 beside the rest
+// (1160 alone) and a softmax warp all: some 150 instructions issued at one in
+// 20 clocks, among 8500 a tile in all (0.62 of the issue slots).  What did not
+// help: packed or scalar arithmetic, fewer polls, other register splits, two
+// groups of softmax warps on alternate tiles, and one even division of the
+// tiles over a fixed grid (64 x 896 47.6 -> 50.8 us, 96 x 8192 128.5 -> 121.7,
+// 2048 x 2176 146.5 -> 149: a piece costs 3.5 us before and 3 after its tiles).
 // ---------------------------------------------------------------------------
 constexpr int kMnThreads = 1024;
 constexpr int kMnSoft = 16;        // softmax warps
@@ -1493,12 +1509,21 @@ struct A4Plan {
   int chunks, splits, split_pages;
 };
 
-// Query chunks and key splits of a launch, from what the host knows: the
-// plan's capacity (or the caller's estimate of its items), the rows of an
-// item, and the longest cache.  One CTA runs per SM and its eight warps take a
-// page each, so keys are split until the grid covers the SMs twice, and no
-// further than two pages per warp.
+// Rows x heads per kv head up to which the few-rows kernel runs.  Its time grows
+// with the chunks of eight, the other's not up to 128 (us, few | many):
+//   rows x heads                    16           32            64
+//   8 x 2176, 32 kv heads      42.6 | 75.9   73.7 | 76.9   142.8 | 77.7
+//   4 x 8192, 8 kv heads       25.0 | 43.5   38.6 | 43.6    63.0 | 44.7
+//   16 x 1024, 8 kv heads      14.5 | 23.1   26.2 | 23.5    43.9 | 23.8
+//   1 x 32768, 8 kv heads      26.8 | 56.3   39.2 | 56.9    66.1 | 58.1
 constexpr int kFewMaxRows = 32;
+
+// Query chunks and key splits of the few-rows kernel, from what the host knows:
+// the sequences, the rows of one, and the longest cache.  Two CTAs run per SM
+// and a CTA's eight warps take a page each in a round; beginning and end cost
+// about a round, joining splits another.  The count is the one whose waves of
+// CTAs take the fewest rounds (8 x 2176, 32 kv heads: 1 split 22.4 us, 2 splits
+// 30.6; 4 x 65536, 8 kv heads: 9 splits 58.0, 6 79.0, 14 72.4).
 
 A4Plan a4_plan_few(int items, int rows, int group, int n_kv, int seqlen_max, int kv_splits) {
   A4Plan pl{};

@@ -12,9 +12,10 @@
 // Memory-bound: every input is read once, every output written once.  Eight
 // lanes take a head (16 values each: 8 of either half, two 16-byte loads), so
 // the rotation needs no exchange and a 4-bit group's minimum and maximum take
-// three shuffles.  A CTA of 128 threads takes 32 heads of one row, two per
-// thread: the rotation's tables are read once for both, and both heads' loads
-// are in flight together.
+// three shuffles.  A CTA of 128 threads takes 16 heads a thread's turn of one
+// row.  To bf16 a thread takes four: the rotation's tables are read once for
+// them and their loads are in flight together.  To 4 bits it takes one: the
+// codes are half the work, and more threads hide them better.
 #include "common.cuh"
 #include "int4.cuh"
 #include "internal.h"
@@ -24,8 +25,7 @@ namespace fdllm {
 constexpr int kAppendKernelId = 8;
 constexpr int kReadKernelId = 9;
 constexpr int kApThreads = 128;
-constexpr int kApHeads = 2;                          // heads per thread
-constexpr int kApUnits = kApThreads / 8 * kApHeads;  // heads per CTA
+constexpr int kApHeadsBf16 = 4, kApHeadsInt4 = 1;  // heads per thread
 
 // Where a slot's token lives: slot = sequence * seqlen_max + position.
 struct PageMap {
@@ -36,16 +36,31 @@ struct PageMap {
   int64_t n_pages;
 };
 
+// A slot's sequence and position; 0 and 0 when the slot is out of range.
+struct SlotAt {
+  int64_t seq, pos;
+  bool ok;
+};
+__device__ __forceinline__ SlotAt slot_at(const PageMap& m, int64_t slot) {
+  SlotAt s{0, 0, slot >= 0 && slot < m.n_slots};
+  if (!s.ok) return s;
+  if (slot >> 32 == 0) {  // (64-bit division is a long subroutine)
+    s.seq = static_cast<uint32_t>(slot) / static_cast<uint32_t>(m.seqlen_max);
+  } else {
+    s.seq = slot / m.seqlen_max;
+  }
+  s.pos = slot - s.seq * m.seqlen_max;
+  return s;
+}
 // page * 64 + line of a slot; -1 (reported) when the slot or its page is out of range
-__device__ __forceinline__ int64_t page_line(const PageMap& m, int64_t slot, int32_t* status, int info,
+__device__ __forceinline__ int64_t page_line(const PageMap& m, int64_t slot, const SlotAt& s, int32_t* status, int info,
                                              int kernel_id) {
-  bool ok = slot >= 0 && slot < m.n_slots;
+  bool ok = s.ok;
   int64_t at = slot;
   if (ok && m.pages != nullptr) {
-    const int64_t seq = slot / m.seqlen_max, pos = slot - seq * m.seqlen_max;
-    const int64_t page = m.pages[seq * m.pages_per_seq + pos / kI4Page];
+    const int64_t page = m.pages[s.seq * m.pages_per_seq + s.pos / kI4Page];
     ok = page >= 0 && page < m.n_pages;
-    at = page * kI4Page + pos % kI4Page;
+    at = page * kI4Page + s.pos % kI4Page;
   }
   if (!ok) {
     report(status, FDLLM_ERR_INDEX, info, kernel_id);
@@ -89,15 +104,32 @@ __device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
   f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
 }
 
-// eight codes in a word's order (dim 2 i + j at bits 16 j + 4 i)
-__device__ __forceinline__ uint32_t codes8(const float (&x)[8], float low, float step) {
+// Eight codes in a word's order (dim 2 i + j at bits 16 j + 4 i).  The quotient
+// has to be the division's own, correctly rounded: ties are frequent between
+// bf16 values.  With y the correctly rounded reciprocal (one division a group),
+// q = x y, and the remainder x - q s exact by a fused multiply-add, q + r y is
+// it (Markstein, 1990; it was compared with the division for every mantissa of
+// a bf16 step and an fp32 numerator).  Four instructions on the multiply-add
+// pipe, where a division takes several on the unit of special functions, which
+// 16 codes a lane kept busy longer than the memory took.  The remainder is exact
+// while no operand nears the ends of fp32: beyond, the division itself.  The
+// sum with 1.5 * 2^23 rounds to the nearest integer (even on a tie), in its low
+// bits.
+template <bool EXACT>
+__device__ __forceinline__ uint32_t codes8(const float (&x)[8], float low, float step, float inv) {
   uint32_t w = 0;
 #pragma unroll
   for (int d = 0; d < 8; ++d) {
-    // true division: ties are frequent between bf16 values, and the quotient
-    // of a tie is exact only by the division itself
-    const float c = fminf(rintf(__fdiv_rn(__fsub_rn(x[d], low), step)), 15.f);
-    w |= static_cast<uint32_t>(static_cast<int>(c)) << (16 * (d & 1) + 4 * (d >> 1));
+    const float n = __fsub_rn(x[d], low);
+    float q;
+    if (EXACT) {
+      q = __fdiv_rn(n, step);
+    } else {
+      q = __fmul_rn(n, inv);
+      q = __fmaf_rn(__fmaf_rn(-q, step, n), inv, q);
+    }
+    const uint32_t c = __float_as_uint(__fadd_rn(fminf(q, 15.f), 12582912.f)) & 15u;
+    w |= c << (16 * (d & 1) + 4 * (d >> 1));
   }
   return w;
 }
@@ -131,9 +163,13 @@ __device__ __forceinline__ void store_group(uint8_t* block, int line, int sub, c
   if (mag >= 0x7f80u || s > 3.3e38f) {
     pair = 0x7fc07fc0u;  // an infinity or NaN in the group (or a range beyond fp32): the whole group reads as NaN
   } else {
-    if (s > 0.f) {
-      c0 = codes8(x, lo, s);
-      c1 = codes8(y, lo, s);
+    if (s >= 0x1p-90f && s <= 0x1p100f) {
+      const float inv = __frcp_rn(s);
+      c0 = codes8<false>(x, lo, s, inv);
+      c1 = codes8<false>(y, lo, s, inv);
+    } else if (s > 0.f) {
+      c0 = codes8<true>(x, lo, s, 0.f);
+      c1 = codes8<true>(y, lo, s, 0.f);
     }
     const __nv_bfloat16 low = __float2bfloat16_rn(lo);  // exact
     pair = static_cast<uint32_t>(__bfloat16_as_ushort(step)) | (static_cast<uint32_t>(__bfloat16_as_ushort(low)) << 16);
@@ -146,6 +182,8 @@ __device__ __forceinline__ void store_group(uint8_t* block, int line, int sub, c
 
 template <bool INT4>
 __global__ void __launch_bounds__(kApThreads) append_kernel(const AppendParams p) {
+  constexpr int kApHeads = INT4 ? kApHeadsInt4 : kApHeadsBf16;
+  constexpr int kApUnits = kApThreads / 8 * kApHeads;  // heads per CTA
   const int row = blockIdx.x;
   const int sub = threadIdx.x & 7;
   const int unit0 = blockIdx.y * kApUnits + (threadIdx.x >> 3);
@@ -167,17 +205,17 @@ __global__ void __launch_bounds__(kApThreads) append_kernel(const AppendParams p
       b[h] = *reinterpret_cast<const uint4*>(src + 64 + 8 * sub);
     }
   }
-  const int64_t at = page_line(p.map, slot, p.status, row, kAppendKernelId);
-  if (at < 0) return;  // the whole row is left as it was
+  const SlotAt where = slot_at(p.map, slot);
   float s1[8], s2[8], c1[8], c2[8];
   const bool turn = p.sin != nullptr;
-  if (turn) {
-    const int64_t pos = slot % p.map.seqlen_max;
-    load8(p.sin + pos * 128 + 8 * sub, s1);
-    load8(p.sin + pos * 128 + 64 + 8 * sub, s2);
-    load8(p.cos + pos * 128 + 8 * sub, c1);
-    load8(p.cos + pos * 128 + 64 + 8 * sub, c2);
+  if (turn) {  // (beside the page table's load)
+    load8(p.sin + where.pos * 128 + 8 * sub, s1);
+    load8(p.sin + where.pos * 128 + 64 + 8 * sub, s2);
+    load8(p.cos + where.pos * 128 + 8 * sub, c1);
+    load8(p.cos + where.pos * 128 + 64 + 8 * sub, c2);
   }
+  const int64_t at = page_line(p.map, slot, where, p.status, row, kAppendKernelId);
+  if (at < 0) return;  // the whole row is left as it was
 #pragma unroll
   for (int h = 0; h < kApHeads; ++h) {
     const int u = first + unit0 + h * (kApThreads / 8);
@@ -228,7 +266,8 @@ __global__ void __launch_bounds__(kRdThreads) read_int4_kernel(const uint8_t* __
   const int row = blockIdx.x;
   pdl_wait();
   pdl_launch_dependents();
-  const int64_t at = page_line(map, slots[row], status, row, kReadKernelId);
+  const int64_t slot = slots[row];
+  const int64_t at = page_line(map, slot, slot_at(map, slot), status, row, kReadKernelId);
   const uint8_t* cache = blockIdx.y == 0 ? kc : vc;
   __nv_bfloat16* out = (blockIdx.y == 0 ? k_out : v_out) + static_cast<int64_t>(row) * n_kv * 128;
   for (int i = threadIdx.x; i < n_kv * 16; i += kRdThreads) {
@@ -310,7 +349,8 @@ extern "C" int fdllm_rope_append(const void* q, const void* k, const void* v, in
   p.n_kv = n_kv_heads;
   p.status = status_ptr();
   const int units = (q_out != nullptr ? n_heads : 0) + 2 * n_kv_heads;
-  const dim3 grid(n_rows, (units + kApUnits - 1) / kApUnits);
+  const int per_cta = kApThreads / 8 * (kv_bits == 4 ? kApHeadsInt4 : kApHeadsBf16);
+  const dim3 grid(n_rows, (units + per_cta - 1) / per_cta);
   const cudaError_t e =
       kv_bits == 4 ? launch_ex(append_kernel<true>, grid, dim3(kApThreads), 0, stream, 1, pdl_enabled(), p)
                    : launch_ex(append_kernel<false>, grid, dim3(kApThreads), 0, stream, 1, pdl_enabled(), p);

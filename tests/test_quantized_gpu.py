@@ -378,6 +378,25 @@ def test_append_bad_slots_and_pages_leave_rows_out(bits):
             assert not k[(~good).cuda()].any() and not v[(~good).cuda()].any()
 
 
+@pytest.mark.parametrize("k", [-110, -95, -90, -85, -40, 40, 95, 100, 105, 118])
+def test_four_bit_codes_do_not_depend_on_the_scale(k):
+    """A power of two moves steps and lows, not the codes (the division has two
+    forms by the step's size)."""
+    from flash_dllm_b200 import ops
+    g = _gen(3)
+    x = _randn(g, 64, 4 * 128).bfloat16()
+    slots = torch.arange(64, device="cuda")
+    got = []
+    for y in (x, (x.double() * 2.0 ** k).bfloat16()):
+        kc, vc = ops.int4_cache(1, 4)
+        ops.rope_append(y, y, y, slots, None, None, kc, vc, 4, 4, 64)
+        assert torch.equal(kc, vc)
+        got.append(qr.int4_unpack(kc))
+    (c0, s0, l0), (c1, s1, l1) = got
+    assert torch.equal(c0, c1) and torch.equal(s0 * 2.0 ** k, s1) and torch.equal(l0 * 2.0 ** k, l1)
+    assert torch.equal(got[0][0].long(), qr.int4_group(x.reshape(64, 4, 128).transpose(0, 1))[0][None])
+
+
 # -------------------------------------------- attention over a 4-bit cache --
 
 def _attention_case(seed, seqs, h, hk, length, nan_past_end=False):
