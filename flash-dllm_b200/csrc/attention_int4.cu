@@ -1105,7 +1105,8 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
           if (lane == 0) mbar_arrive(&ms.p_full[slot]);  // S is read
           continue;
         }
-        const float mul = log_mul * k;
+        // (not 0, however small the query and the keys: a key past the end is -infinity times this)
+        const float mul = fmaxf(log_mul * k, 0x1p-126f);
         ms.mx[t & 1][r][grp] = fmaf(mn_max32(v), mul, static_cast<float>(ev));
         asm volatile("bar.sync %0, 128;" ::"r"(3 + (warp & 3)) : "memory");
         const float4 m4 = *reinterpret_cast<const float4*>(ms.mx[t & 1][r]);
@@ -1611,7 +1612,7 @@ A4Workspace a4_workspace(int32_t max_items, int32_t n_kv, int32_t seqlen_max, co
 bool a4_args_ok(int32_t n_rows, int32_t max_items, int32_t n_seqs, int32_t n_heads, int32_t n_kv, int32_t seqlen_max,
                 int32_t kv_splits, int32_t rows_hint) {
   return n_rows >= 0 && n_seqs > 0 && max_items >= n_seqs && n_kv > 0 && n_heads > 0 && n_heads % n_kv == 0 && n_kv <= 65535 &&
-         n_heads / n_kv <= 64 && seqlen_max > 0 && kv_splits >= 0 && rows_hint >= 0;
+         n_heads / n_kv <= 64 && seqlen_max > 0 && seqlen_max <= (1 << 30) && kv_splits >= 0 && rows_hint >= 0;
 }
 
 A4Plan a4_plan(int32_t n_rows, int32_t max_items, int32_t n_seqs, int32_t n_heads, int32_t n_kv, int32_t seqlen_max,

@@ -342,6 +342,10 @@ void attn_cache_int4(const Tensor& q, const Tensor& o, const Tensor& k_cache, co
                     "n_heads must be a multiple of n_kv_heads");
   TORCH_CHECK_VALUE(q.size(1) == n_heads * kHead && o.sizes() == q.sizes(), "q and o must be [rows, ",
                     n_heads * kHead, "], got ", q.sizes(), " and ", o.sizes());
+  // (scores sum all masked rows of q, rows that another CTA may have answered)
+  const auto* q0 = static_cast<const char*>(q.data_ptr());
+  const auto* o0 = static_cast<const char*>(o.data_ptr());
+  TORCH_CHECK_VALUE(q.numel() == 0 || q0 + q.nbytes() <= o0 || o0 + o.nbytes() <= q0, "o must not overlap q");
   const int64_t n_pages = int4_pages(c, k_cache, v_cache, n_kv_heads);
   c.plain(plan, "plan", at::kInt, 1);
   const Pages pt = page_table(c, table, seqlen_max);

@@ -171,6 +171,9 @@ def quantize_block_int8(block) -> None:
     if not isinstance(block.dropout, torch.nn.Identity) or not isinstance(block.act, torch.nn.SiLU):
         raise TypeError("8-bit projections need a block without dropout and with SiLU")
     wq, wk, wv, wo, wg, wu, wf = (m.weight.detach() for m in linears)
+    if wq.shape[1] % 128 or wg.shape[0] % 128 or wq.shape[1] > 16384:
+        raise ValueError(f"8-bit projections need widths that are multiples of 128 (d_model up to 16384), got d_model "
+                         f"{wq.shape[1]} and MLP width {wg.shape[0]}")
     block.int8_weights = Int8Weights(*ops.quantize_int8(torch.cat([wq, wk, wv], 0)), *ops.quantize_int8(wo),
                                      *ops.quantize_int8(torch.cat([wg, wu], 0)), *ops.quantize_int8(wf),
                                      next(_INT8_VERSIONS))
@@ -202,7 +205,8 @@ def flash_fused_elastic_cache(self, x: torch.Tensor, block_idx, positions, lengt
         k_cache, v_cache = self.k_cache, self.v_cache
         if four_bits:
             if key_pos_flat.numel() > 0:  # the gathered keys as bf16 rows of their own
-                k_cache, v_cache = ops.read_cache_int4(k_cache, v_cache, key_pos_flat, max_length)
+                k_cache, v_cache = ops.read_cache_int4(k_cache, v_cache, key_pos_flat.to(torch.int64).contiguous(),
+                                                       max_length)
                 key_pos_flat = torch.arange(key_pos_flat.numel(), device=x.device)
             else:
                 k_cache, v_cache = k1, v1  # (nothing is read)

@@ -277,7 +277,7 @@ def attn_cache_int4(q: torch.Tensor, o: torch.Tensor, k_cache: torch.Tensor, v_c
                     rows_hint: int = 0, page_table: Optional[torch.Tensor] = None) -> None:
     """:func:`attn_cache` over the 4-bit cache: the rows of ``plan`` (from
     :func:`plan_cache_attention`) attend to keys [0, k_end) of their sequence;
-    ``o`` rows outside the plan keep what they held.  Query head h reads kv
+    ``o`` (not overlapping ``q``) keeps what it held in rows outside the plan.  Query head h reads kv
     head h // (n_heads // n_kv_heads).  ``attn_scores`` fp32 [batch *
     seqlen_max] accumulates ``score_scale`` times the raw q.k sums of the
     masked rows over all heads.  ``rows_hint``: rows of one sequence to expect

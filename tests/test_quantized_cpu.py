@@ -159,6 +159,10 @@ def test_block_and_driver_refusals_on_cpu():
     cfg = LLaDAConfigB200(d_model=128, n_heads=2, n_layers=1, mlp_hidden_size=128, vocab_size=16)
     with pytest.raises(TypeError, match="bf16 Linear"):
         quantize_block_int8(LLaDABlockB200(cfg, 0, dtype=torch.float32))
+    blk = LLaDABlockB200(LLaDAConfigB200(d_model=128, n_heads=1, n_layers=1, mlp_hidden_size=192, vocab_size=16), 0,
+                         dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="multiples of 128"):
+        quantize_block_int8(blk)
     blk = LLaDABlockB200(cfg, 0, dtype=torch.bfloat16)
     blk.act = torch.nn.GELU()
     with pytest.raises(TypeError, match="SiLU"):

@@ -526,6 +526,47 @@ def test_attn_cache_int4_plan_of_another_shape_is_reported():
         check_device_status()
 
 
+@pytest.mark.parametrize("rows", [1, 6, 40])
+@pytest.mark.parametrize("k", [-100, -60, 60, 100])
+def test_attn_cache_int4_powers_of_two(rows, k):
+    """Both kernels normalise by powers of two: neither the size of the cache's
+    values nor of the query's costs precision.  (Not the same bits: an exponent
+    of 100 beside a logit in log2 units rounds it by up to 2^-18, some 3e-6 of a
+    weight, which moves single roundings of P.)"""
+    q, caches, pt, spans, mb, tb, B, L = _attention_case(21, [(200, rows, 0), (70, rows, 0)], 6, 2, 200)
+
+    def scaled(c, e):
+        c = c.clone()
+        p = c[..., qr.CODES:].contiguous().view(torch.bfloat16)
+        c[..., qr.CODES:] = (p.double() * 2.0 ** e).bfloat16().view(torch.uint8)
+        return c
+
+    for q2, c2 in ((q, (caches[0], scaled(caches[1], k))),
+                   ((q.double() * 2.0 ** -k).bfloat16(), (scaled(caches[0], k), caches[1]))):
+        out, sc = _run_attention(q2, c2, pt, mb, tb, B, L, 6, 2)
+        _check_attention(q2, c2, pt, spans, B, L, 6, 2, out, sc)
+
+
+@pytest.mark.parametrize("rows", [1, 6, 40])
+@pytest.mark.parametrize("size", [0.0, 2.0 ** -120, 2.0 ** -70])
+def test_attn_cache_int4_small_queries(rows, size):
+    """A query of zeros, or near them, weighs all keys alike, and keys past the
+    end (whole pieces and tiles of them) still not at all."""
+    q, caches, pt, spans, mb, tb, B, L = _attention_case(22, [(200, rows, 0), (70, rows, 0), (33, rows, 0)], 4, 2, 400)
+    q[::2] = (q[::2].double() * size).bfloat16()
+    caches[0][:, 1] = 0  # and keys of zeros in one head
+    out, sc = _run_attention(q, caches, pt, mb, tb, B, L, 4, 2)
+    _check_attention(q, caches, pt, spans, B, L, 4, 2, out, sc)
+
+
+def test_attn_cache_int4_refuses_its_query_as_output():
+    q, caches, pt, spans, mb, tb, B, L = _attention_case(9, [(200, 3, 0)], 2, 2, 200)
+    from flash_dllm_b200 import ops
+    plan, cap = ops.plan_cache_attention(mb, tb, q.shape[0], B, 64, L, q.device)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.attn_cache_int4(q, q, *caches, plan, cap, None, 1.0, 2, 2, L, 0.1, page_table=pt)
+
+
 @pytest.mark.parametrize("rows", [1, 40])
 def test_attn_cache_int4_rows_behind_the_last_sequence(rows):
     """More rows than the plan was made for: all its sequences are computed,
