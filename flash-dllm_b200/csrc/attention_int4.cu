@@ -663,9 +663,9 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) attn_int4_few_kernel(co
 // scores when those are wanted).  Both operands are fp16, normalised by powers
 // of two so that no cache or query can leave its range: a query row by its
 // largest value (2^-e_m), K and V by the largest value of each 32-key piece of
-// a tile (2^-ek, 2^-ev).  With 11 bits, fp16 holds (code - 8) * step exactly
+// a tile (2^(14 - ek), 2^(14 - ev)).  With 11 bits, fp16 holds (code - 8) * step exactly
 // (3 bits by 8), so
-//   K operand   (code - 8) * step * 2^-ek for 128 dims, and 16 more columns in
+//   K operand   (code - 8) * step * 2^(14 - ek) for 128 dims, and 16 more columns in
 //               which base_n * sum_d q_d is formed from two fp16 halves of the
 //               base and three of the sum (22 bits), and 0 or -infinity for a
 //               key past the end: the S tile is the whole logit, and a softmax
@@ -729,6 +729,8 @@ static_assert(kMnSmem <= 227 * 1024, "shared memory");
 constexpr int kMnRegsSoft = 72, kMnRegsConv = 56, kMnRegsMisc = 48;
 static_assert(32 * (kMnSoft * kMnRegsSoft + kMnConv * kMnRegsConv + 4 * kMnRegsMisc) <= kMnThreads * 64,
               "setmaxnreg split");
+constexpr int kMnUp = 14;        // a piece's largest K or V lies in [2^14, 2^15): fp16's normals reach 2^28 below it
+constexpr float kMnDown = 0x1p-28f;  // what V is raised by, and the sum of P lowered by
 constexpr float kMnLazy = 8.f;   // log2 units a contribution may pass the reference by before it moves
 constexpr float kMnRaise = 6.f;  // P is raised by 2^6: with the 8 above, below fp16's 2^16
 constexpr int kMnPartFloats = kMnRows * kA4HeadDim + 2 * kMnRows;
@@ -836,7 +838,7 @@ __device__ __forceinline__ MnParams mn_params(uint32_t pr) {
   MnParams r;
   r.e = mn_exponent(pr);
   const float step = __uint_as_float(pr << 16), low = __uint_as_float(pr & 0xffff0000u);
-  const float s = pow2i(-r.e);
+  const float s = pow2i(kMnUp - r.e);
   r.step = pack_f16x2(step * s, step * s);
   r.base = fmaf(8.f, step, low) * s;
   return r;
@@ -1082,7 +1084,7 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
         // logits in log2 units are v * mul (keys past the end -infinity)
         float v[32];
         tmem_ld_32x32b_x32(ts, v);
-        const float k = pow2i(ms.ek[t & 7][grp]);
+        const float k = pow2i(ms.ek[t & 7][grp] - kMnUp);
         const int ev = ms.ev[t & 7][grp];
         if (score_warp) {
           // lanes 24 .. 26 hold the three parts' logits
@@ -1150,7 +1152,7 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
         }
         float x, y;
         unpack_f32x2(add_f32x2(ps[0], ps[1]), x, y);
-        l = fmaf(x + y, pow2i(-ev), l);
+        l = fmaf((x + y) * 0x1p-14f, pow2i(-ev), l);  // (with ev = -100, of values of zero alone, still far from the end)
         // over the first half of the logits that this thread has read
         tmem_st_32x32b_x16(ts, pw);
         tmem_wait_st();
@@ -1171,6 +1173,8 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
         const float inv = direct ? (l_o > 0.f ? 1.f / l_o : (l_o == 0.f ? 0.f : l_o)) : 1.f;
         float ov[32];
         tmem_ld_32x32b_x32(to + 32 * grp, ov);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) ov[j] *= kMnDown;
         if (r < rows && direct) {
           __nv_bfloat16* dst = p.o + mn_row(p, sq, kvh, m0 + r) + 32 * grp;
 #pragma unroll

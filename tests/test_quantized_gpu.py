@@ -559,6 +559,24 @@ def test_attn_cache_int4_small_queries(rows, size):
     _check_attention(q, caches, pt, spans, B, L, 4, 2, out, sc)
 
 
+@pytest.mark.parametrize("rows", [1, 6, 40])
+@pytest.mark.parametrize("big", [2.0 ** 8, 2.0 ** 22])
+def test_attn_cache_int4_large_values_without_weight(rows, big):
+    """Keys that nothing attends to, with values far larger than their
+    neighbours': what is attended to keeps its precision."""
+    q, caches, pt, spans, mb, tb, B, L = _attention_case(23, [(200, rows, 0), (90, rows, 0)], 2, 2, 200)
+    g = _gen(4)
+    u = _randn(g, 1, 2, 128)
+    q = (u.reshape(1, 256) + 0.1 * _randn(g, q.shape[0], 256)).bfloat16()
+    n = caches[0].shape[0]
+    k, v = 0.3 * _randn(g, n, 2, 64, 128), _randn(g, n, 2, 64, 128)
+    k[:, :, 5::16] = -6 * u[:, :, None]  # a logit of about -6 * 128 / 128 ** 0.5 = -68
+    v[:, :, 5::16] *= big
+    caches = [qr.int4_pack(x.bfloat16()) for x in (k, v)]
+    out, sc = _run_attention(q, caches, pt, mb, tb, B, L, 2, 2)
+    _check_attention(q, caches, pt, spans, B, L, 2, 2, out, sc)
+
+
 def test_attn_cache_int4_refuses_its_query_as_output():
     q, caches, pt, spans, mb, tb, B, L = _attention_case(9, [(200, 3, 0)], 2, 2, 200)
     from flash_dllm_b200 import ops
