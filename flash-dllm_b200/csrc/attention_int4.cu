@@ -912,7 +912,6 @@ __device__ __forceinline__ int64_t mn_row(const A4Params& p, const MnSeq& s, int
 
 struct MnMisc {
   uint64_t raw_full[kMnConv];
-  uint64_t ev_full[8];             // [tile % 8]
   uint64_t k_full[2], v_full[2], s_full[3], p_full[3], pv_done[3], mma_done;
   uint32_t tmem;
   int32_t last, convert;
@@ -932,8 +931,8 @@ struct MnMisc {
   float l[4][kMnRows];              // the key quarters' sums
 };
 static_assert(sizeof(MnMisc) <= kMnMiscBytes, "misc");
-constexpr int kMnBars = 8 + 14;
-static_assert(offsetof(MnMisc, tmem) - offsetof(MnMisc, ev_full) == kMnBars * 8, "the barriers lie in a row");
+constexpr int kMnBars = 14;
+static_assert(offsetof(MnMisc, tmem) - offsetof(MnMisc, k_full) == kMnBars * 8, "the barriers lie in a row");
 
 // What one row tile of a CTA takes: every role computes the same.
 struct MnTile {
@@ -992,13 +991,12 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
       const int row_warps = (rows + 31) / 32;
       const int p_warps = 4 * (row_warps + (with_scores && row_warps < 4 ? 1 : 0));
       if (threadIdx.x == 0) {
-        for (int s = 0; s < 8; ++s) mbar_init(&ms.ev_full[s], 1);
         for (int s = 0; s < 2; ++s) {
           mbar_init(&ms.k_full[s], 4);
           mbar_init(&ms.v_full[s], 4);
         }
         for (int s = 0; s < 3; ++s) {
-          mbar_init(&ms.s_full[s], 1);
+          mbar_init(&ms.s_full[s], 2);  // S, and V's exponents
           mbar_init(&ms.p_full[s], p_warps);
           mbar_init(&ms.pv_done[s], 1);
         }
@@ -1079,7 +1077,7 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
       for (int t = soft || score_warp ? 0 : n_kt; t < n_kt; ++t) {
         const int slot = t % 3;
         const uint32_t ts = tmem + 128 + 128 * slot + 32 * grp + tl;
-        ok = ok && a4_wait(&ms.s_full[slot], (t / 3) & 1, p.status) && a4_wait(&ms.ev_full[t & 7], (t >> 3) & 1, p.status);
+        ok = ok && a4_wait(&ms.s_full[slot], (t / 3) & 1, p.status);
         tc_fence_after();
         // logits in log2 units are v * mul (keys past the end -infinity)
         float v[32];
@@ -1203,7 +1201,7 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
       __syncthreads();
       tc_fence_after();
       if (threadIdx.x == 0) {
-        uint64_t* b = ms.ev_full;  // every barrier but the conversion warps' own, in a row
+        uint64_t* b = ms.k_full;  // every barrier but the conversion warps' own, in a row
         for (int i = 0; i < kMnBars; ++i) mbar_inval(b + i);
       }
       if (n_splits > 1) {
@@ -1435,7 +1433,7 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
           if (t >= 3 && !a4_wait(&ms.pv_done[t % 3], (t / 3 - 1) & 1, p.status)) break;
           if (lane == 0) {
             *reinterpret_cast<int4*>(ms.ev[t & 7]) = make_int4(e[0], e[1], e[2], e[3]);
-            mbar_arrive(&ms.ev_full[t & 7]);
+            mbar_arrive(&ms.s_full[t % 3]);
           }
         }
       }
