@@ -693,16 +693,20 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) attn_int4_few_kernel(co
 // two tiles ahead of P V(t).  The first tiles are converted while the query
 // operand is laid out.  Key ranges are split over CTAs as in the other kernel.
 //
-// Measured: 2048 rows of one sequence of 2176, 32 heads: 142.7 us (512 CTAs of
-// 17 tiles in 3.5 waves), 0.26 of the fp16 rate; 96 rows of four of 8192, with
-// scores, 127 us; 64 of eight of 896, with scores, 47.5 us.  A tile takes about
-// 2900 clocks, of which the tensor cores' 17 instructions 1900 beside the rest
-// (1160 alone) and a softmax warp all: some 150 instructions issued at one in
-// 20 clocks, among 8500 a tile in all (0.62 of the issue slots).  What did not
-// help: packed or scalar arithmetic, fewer polls, other register splits, two
-// groups of softmax warps on alternate tiles, and one even division of the
-// tiles over a fixed grid (64 x 896 47.6 -> 50.8 us, 96 x 8192 128.5 -> 121.7,
-// 2048 x 2176 146.5 -> 149: a piece costs 3.5 us before and 3 after its tiles).
+// Measured: 2048 rows of one sequence of 2176, 32 heads: 141 us (512 CTAs of 17
+// tiles in 3.5 waves), 0.3 of the fp16 rate; 96 rows of four of 8192, with
+// scores, 127 us; 64 of eight of 896, with scores, 47 us.  A tile takes about
+// 2900 clocks.  The tensor cores need 1160 of them (17 instructions), and wait;
+// a softmax warp needs all: some 160 instructions, each issued about 18 clocks
+// after the last among 8 warps a scheduler, the four of a row quarter in step (a
+// scheduler owns a quarter of tensor memory's lanes), so the exponentials'
+// 1024 clocks and the rest do not overlap.  What did not help: the next tile's
+// maximum beside this one's exponentials (141 -> 154 us), two groups on
+// alternate tiles (157), the query operand in tensor memory (141), descriptors
+// in uniform registers (142), packed or scalar arithmetic, fewer polls, other
+// register splits; and one even division of the tiles over a fixed grid (64 x
+// 896 47.6 -> 50.8 us, 96 x 8192 128.5 -> 121.7, 2048 x 2176 146.5 -> 149: a
+// piece costs 3.5 us before and 3 after its tiles).
 // ---------------------------------------------------------------------------
 constexpr int kMnThreads = 1024;
 constexpr int kMnSoft = 16;        // softmax warps
