@@ -1217,34 +1217,46 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
         }
         asm volatile("bar.sync 1, 512;" ::: "memory");
         if (ms.last) {
-          // thread -> (row, 4 dims) units; splits joined in order
+          // thread -> row, the dims it has above; splits joined in order
           const float* all = p.part + cell * p.splits * kMnPartFloats;
-          const int r = threadIdx.x & 127;
+          const float* ml = all + kMnRows * kA4HeadDim;  // a split's references, its sums kMnRows further on
           if (r < rows) {
             float M = -INFINITY;
-            for (int k = 0; k < n_splits; ++k) M = fmaxf(M, __ldcg(all + k * kMnPartFloats + kMnRows * kA4HeadDim + r));
-            const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll 4
+            for (int k = 0; k < n_splits; ++k) M = fmaxf(M, __ldcg(ml + k * kMnPartFloats + r));
+            const float top = M == -INFINITY ? 0.f : M;
             float L = 0.f;
+#pragma unroll 4
             for (int k = 0; k < n_splits; ++k) {
-              const float* ml = all + k * kMnPartFloats + kMnRows * kA4HeadDim;
-              L = fmaf(ex2_approx(__ldcg(ml + r) - ref), __ldcg(ml + kMnRows + r), L);
+              const float* q = ml + k * kMnPartFloats + r;
+              L = fmaf(ex2_approx(__ldcg(q) - top), __ldcg(q + kMnRows), L);
             }
             const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
-            __nv_bfloat16* dst = p.o + mn_row(p, sq, kvh, m0 + r);
+            __nv_bfloat16* dst = p.o + mn_row(p, sq, kvh, m0 + r) + 32 * grp;
 #pragma unroll 1
-            for (int u = (threadIdx.x >> 7); u < kA4HeadDim / 4; u += 4) {
-              float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+            for (int half = 0; half < 2; ++half) {
+              float o[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = 0.f;
+#pragma unroll 2
               for (int k = 0; k < n_splits; ++k) {
-                const float f = ex2_approx(__ldcg(all + k * kMnPartFloats + kMnRows * kA4HeadDim + r) - ref);
-                const float4 x = __ldcg(reinterpret_cast<const float4*>(all + k * kMnPartFloats) + u * kMnRows + r);
-                o.x = fmaf(f, x.x, o.x);
-                o.y = fmaf(f, x.y, o.y);
-                o.z = fmaf(f, x.z, o.z);
-                o.w = fmaf(f, x.w, o.w);
+                const float* q = all + k * kMnPartFloats;
+                const float f = ex2_approx(__ldcg(q + kMnRows * kA4HeadDim + r) - top);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const float4 x = __ldcg(reinterpret_cast<const float4*>(q) + (8 * grp + 4 * half + i) * kMnRows + r);
+                  o[4 * i] = fmaf(f, x.x, o[4 * i]);
+                  o[4 * i + 1] = fmaf(f, x.y, o[4 * i + 1]);
+                  o[4 * i + 2] = fmaf(f, x.z, o[4 * i + 2]);
+                  o[4 * i + 3] = fmaf(f, x.w, o[4 * i + 3]);
+                }
               }
-              *reinterpret_cast<uint2*>(dst + 4 * u) =
-                  make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+#pragma unroll
+              for (int i = 0; i < 16; i += 8)
+                *reinterpret_cast<uint4*>(dst + 16 * half + i) =
+                    make_uint4(pack_bf16x2(o[i] * inv, o[i + 1] * inv), pack_bf16x2(o[i + 2] * inv, o[i + 3] * inv),
+                               pack_bf16x2(o[i + 4] * inv, o[i + 5] * inv),
+                               pack_bf16x2(o[i + 6] * inv, o[i + 7] * inv));
             }
           }
         }

@@ -1115,7 +1115,11 @@ int g2_max_pairs_for(int epi, int ksub) {
 //     eight k-blocks a CTA and more (16x24576x4096: 23.2 against 24.9), pairs
 //     with two tiles each and more or more than 512 rows (2048x4096x12288:
 //     74.3 against 81.4);
-//   - no piece is under four k-blocks (100x1024x1024: 11.3 against 17.1).
+//   - a tile is shared by sqrt(k-blocks / 3) CTAs at most: another one saves the
+//     others some of the k-blocks and costs the owner a partial result, the time
+//     of about three (55x296x11968, 94 k-blocks: 13.9 with 6 a tile, 16.0 with 12,
+//     19.5 with 2; 250x288x5168, 41: 13.3 with 4, 15.8 with 8, 19.4 with 1;
+//     64x1024x1024, 8: 7.1 with 1, 9.0 with 2).
 GemmPlan plan_gemm(int epi, int32_t n_rows, int32_t n_cols, int32_t k_dim, int32_t d_model, bool i8 = false) {
   GemmPlan pl{};
   const GemmOverride& ov = gemm_override();
@@ -1181,8 +1185,11 @@ GemmPlan plan_gemm(int epi, int32_t n_rows, int32_t n_cols, int32_t k_dim, int32
   // tiles fit the grid
   const int tiles_per_group = pl.groups > 1 ? pl.n_tiles : pl.m_tiles * pl.n_tiles;
   if (dp && tiles_per_group <= per_group) per_group = tiles_per_group;
-  // (pieces of at least four k-blocks: below that the join is all of the time)
-  if (i8_auto && !dp && iters < 4ll * per_group) per_group = static_cast<int>(std::max(1ll, iters / 4));
+  if (i8_auto && !dp) {
+    int s = 1;  // CTAs a tile: sqrt(k-blocks / 3)
+    while ((s + 1) * (s + 1) * 3 <= pl.kbt * pl.ksub) ++s;
+    if (per_group > static_cast<long long>(s) * tiles_per_group) per_group = s * tiles_per_group;
+  }
   bool even = false;  // CTAs' ranges meet at whole, half, ... tiles
   if (i8_auto && !dp &&
       (pl.pair ? pl.m_tiles <= 2 && tiles_per_group < 2 * per_group : pl.m_tiles > 1 || iters < 8ll * per_group)) {
