@@ -712,7 +712,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) attn_int4_few_kernel(co
 //
 // Measured: 2048 rows of one sequence of 2176, 32 heads: 141 us (512 CTAs of 17
 // tiles in 3.5 waves), 0.3 of the fp16 rate; 96 rows of four of 8192, with
-// scores, 127 us; 64 of eight of 896, with scores, 47 us.  A tile takes about
+// scores, 121.5 us (113.7 without); 64 of eight of 896, with scores, 46.5 us.  A tile takes about
 // 2900 clocks.  The tensor cores need 1160 of them (17 instructions), and wait;
 // a softmax warp needs all: some 160 instructions, each issued about 18 clocks
 // after the last among 8 warps a scheduler, the four of a row quarter in step (a
@@ -720,8 +720,9 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) attn_int4_few_kernel(co
 // 1024 clocks and the rest do not overlap.  What did not help: the next tile's
 // maximum beside this one's exponentials (141 -> 154 us), two groups on
 // alternate tiles (157), the query operand in tensor memory (141), descriptors
-// in uniform registers (142), packed or scalar arithmetic, fewer polls, other
-// register splits; and one even division of the tiles over a fixed grid (64 x
+// in uniform registers (142), a warp of their own for the scores (96 rows of
+// 8192: 121.9 -> 127), packed or scalar arithmetic, fewer polls, other register
+// splits; and one even division of the tiles over a fixed grid (64 x
 // 896 47.6 -> 50.8 us, 96 x 8192 128.5 -> 121.7, 2048 x 2176 146.5 -> 149: a
 // piece costs 3.5 us before and 3 after its tiles).
 // ---------------------------------------------------------------------------
