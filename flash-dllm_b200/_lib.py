@@ -108,7 +108,17 @@ def _load_torch_ops():
     return mod
 
 
-torch_ops = _load_torch_ops()
+class _TorchOps:
+    """That module, loaded at the first use of one of its functions: the rest of
+    the package works where it was not built."""
+
+    def __getattr__(self, name):
+        mod = _load_torch_ops()
+        self.__dict__.update({k: v for k, v in vars(mod).items() if not k.startswith("__")})
+        return getattr(mod, name)
+
+
+torch_ops = _TorchOps()
 
 
 def lib():

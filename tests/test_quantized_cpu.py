@@ -172,6 +172,23 @@ def test_block_and_driver_refusals_on_cpu():
         generate_with_Flash_dLLM(model, [], [4], 1, [], [], kv_bits=4)
 
 
+def test_binding_is_loaded_at_first_use(monkeypatch):
+    from flash_dllm_b200 import _lib
+    loads = []
+
+    def missing():
+        loads.append(1)
+        raise ImportError("not built")
+
+    ops = _lib._TorchOps()
+    monkeypatch.setattr(_lib, "_load_torch_ops", missing)
+    assert not loads
+    with pytest.raises(ImportError, match="not built"):
+        ops.quantize_int8
+    monkeypatch.undo()
+    assert ops.quantize_int8 is ops.quantize_int8 and "linear_int8" in vars(ops)
+
+
 def test_public_names():
     import flash_dllm_b200 as f
     from flash_dllm_b200 import api
