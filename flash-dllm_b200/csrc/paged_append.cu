@@ -12,10 +12,13 @@
 // Memory-bound: every input is read once, every output written once.  Eight
 // lanes take a head (16 values each: 8 of either half, two 16-byte loads), so
 // the rotation needs no exchange and a 4-bit group's minimum and maximum take
-// three shuffles.  A CTA of 128 threads takes 16 heads a thread's turn of one
-// row.  To bf16 a thread takes four: the rotation's tables are read once for
-// them and their loads are in flight together.  To 4 bits it takes one: the
-// codes are half the work, and more threads hide them better.
+// three shuffles.  A CTA of 128 threads works on 16 heads of one row at a time.
+// To bf16 a thread takes four of them: the rotation's tables are read once and
+// the loads are in flight together (6124 tokens of 32 + 16 heads: 29.3 us, 5.2
+// TB/s; with two 31.1, with one 33.2).  To 4 bits it takes one: the codes are
+// half the work, and more threads hide them better (512 tokens of 96 heads: 8.1
+// us; 6124 tokens 75, of which the memory takes 35; with two heads 112 and with
+// one 98.5 before the quotient below).
 #include "common.cuh"
 #include "int4.cuh"
 #include "internal.h"

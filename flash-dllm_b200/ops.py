@@ -47,7 +47,8 @@ class Workspace:
     def clear(cls) -> None:
         cls._bufs.clear()
         cls._retired.clear()
-        _T.workspace_clear()
+        if vars(_T):  # (loaded)
+            _T.workspace_clear()
 
     @classmethod
     def rezero(cls) -> None:
@@ -55,7 +56,8 @@ class Workspace:
         counters or flags set); addresses are kept."""
         for buf in cls._bufs.values():
             buf.zero_()
-        _T.workspace_rezero()
+        if vars(_T):
+            _T.workspace_rezero()
 
 
 _lib.on_device_error(Workspace.rezero)
