@@ -44,10 +44,12 @@ void check_status(const char* name, int rc) {
 // ------------------------------------------------------------- workspaces --
 // Scratch of one stream, its first `zero` bytes zero.  Eager calls keep a
 // buffer per (device, stream, tag).  A captured graph gets its own from its
-// memory pool, cleared by a node of the graph: two graphs that replay at the
-// same time, or a graph and an eager call, never share one, and nothing has
-// to run before the capture.  (Buffers that were outgrown stay allocated:
-// work of their stream may still use them.)
+// memory pool, cleared by a node of the graph, and so does every stream of one
+// capture (its branches replay at the same time): two graphs, two branches of
+// one, or a graph and an eager call never share one, and nothing has to run
+// before the capture.  The clearing node is on the branch that uses the
+// buffer.  (Buffers that were outgrown stay allocated: work of their stream
+// may still use them.)
 class Workspaces {
  public:
   void* get(const at::Device& dev, cudaStream_t stream, const char* tag, size_t bytes, size_t zero, size_t* size) {
@@ -69,16 +71,17 @@ class Workspaces {
         *buf = at::zeros({static_cast<int64_t>(n)}, opts);
       }
     } else {
-      auto& held = captured_[{capture, dev.index(), tag}];
-      if (held.empty() || static_cast<size_t>(held.back().numel()) < bytes) {
+      const Captured key{capture, dev.index(), stream, tag};
+      const auto held = captured_.find(key);
+      if (held == captured_.end() || static_cast<size_t>(held->second.back().numel()) < bytes) {
         // captures long ended: their memory belongs to their graphs' pools
         while (captured_.size() > 64 && std::get<0>(captured_.begin()->first) < capture)
           captured_.erase(captured_.begin());
         Tensor t = at::empty({static_cast<int64_t>(std::max<size_t>(bytes, 256))}, opts);
         if (zero > 0) t.narrow(0, 0, static_cast<int64_t>(zero)).zero_();
-        captured_[{capture, dev.index(), tag}].push_back(t);
+        captured_[key].push_back(t);
       }
-      buf = &captured_[{capture, dev.index(), tag}].back();
+      buf = &captured_[key].back();
     }
     *size = static_cast<size_t>(buf->numel());
     return buf->data_ptr();
@@ -98,7 +101,8 @@ class Workspaces {
  private:
   std::mutex mu_;
   std::map<std::tuple<int, cudaStream_t, std::string>, Tensor> eager_;
-  std::map<std::tuple<uint64_t, int, std::string>, std::vector<Tensor>> captured_;
+  using Captured = std::tuple<uint64_t, int, cudaStream_t, std::string>;  // (ordered by capture first)
+  std::map<Captured, std::vector<Tensor>> captured_;
   std::vector<Tensor> retired_;
 };
 
