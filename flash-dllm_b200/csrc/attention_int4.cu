@@ -50,7 +50,7 @@ struct A4Params {
   int32_t n_heads, n_kv, group;    // group = n_heads / n_kv
   int32_t seqlen_max, pages_per_seq;
   int32_t max_items, n_rows;
-  int32_t batch;                   // sequences the page table (or the cache) holds
+  int32_t batch;                   // sequences that the page table (or the cache) holds and the plan was made for
   int32_t n_seqs;                  // sequences the plan was made for
   int32_t chunks;                  // query chunks of an item that have CTAs of their own
   int32_t splits, split_pages;     // key splits of split_pages pages each
@@ -1630,13 +1630,14 @@ struct A4Workspace {
   size_t scratch;                                // bytes of partial results, never cleared
 };
 
-A4Workspace a4_workspace(int32_t max_items, int32_t n_kv, int32_t seqlen_max, const A4Plan& pl, bool scores) {
+A4Workspace a4_workspace(int32_t max_items, int32_t n_seqs, int32_t n_kv, int32_t seqlen_max, const A4Plan& pl,
+                         bool scores) {
   A4Workspace w{};
   size_t at = 0;
-  w.score_acc = at;
-  if (scores) at += align_up(static_cast<size_t>(max_items) * seqlen_max * sizeof(unsigned long long), 256);
+  w.score_acc = at;  // (a row and a counter a sequence: the plan's are below n_seqs)
+  if (scores) at += align_up(static_cast<size_t>(n_seqs) * seqlen_max * sizeof(unsigned long long), 256);
   w.score_cnt = at;
-  if (scores) at += align_up(static_cast<size_t>(max_items) * sizeof(int32_t), 256);
+  if (scores) at += align_up(static_cast<size_t>(n_seqs) * sizeof(int32_t), 256);
   const size_t cells = pl.splits > 1 ? static_cast<size_t>(pl.many ? pl.batch : max_items) * n_kv * pl.chunks : 0;
   w.part_cnt = at;
   at += align_up(cells * sizeof(int32_t), 256);
@@ -1677,7 +1678,7 @@ extern "C" size_t fdllm_attn_int4_workspace_bytes(int32_t n_rows, int32_t max_it
   if (scratch_bytes != nullptr) *scratch_bytes = 0;
   if (!a4_args_ok(n_rows, max_items, n_seqs, n_heads, n_kv_heads, seqlen_max, kv_splits, rows_hint)) return 0;
   const A4Plan pl = a4_plan(n_rows, max_items, n_seqs, n_heads, n_kv_heads, seqlen_max, kv_splits, rows_hint, scores != 0);
-  const A4Workspace w = a4_workspace(max_items, n_kv_heads, seqlen_max, pl, scores != 0);
+  const A4Workspace w = a4_workspace(max_items, n_seqs, n_kv_heads, seqlen_max, pl, scores != 0);
   if (scratch_bytes != nullptr) *scratch_bytes = w.scratch;
   return w.total;
 }
@@ -1704,7 +1705,7 @@ extern "C" int fdllm_attn_cache_int4(const void* q, void* o, const void* k_cache
     if (x == nullptr || !aligned16(x)) return FDLLM_ERR_ARG;
   const A4Plan pl = a4_plan(n_rows, max_items, n_seqs, n_heads, n_kv_heads, seqlen_max, kv_splits, rows_hint,
                             attn_scores != nullptr);
-  const A4Workspace w = a4_workspace(max_items, n_kv_heads, seqlen_max, pl, attn_scores != nullptr);
+  const A4Workspace w = a4_workspace(max_items, n_seqs, n_kv_heads, seqlen_max, pl, attn_scores != nullptr);
   if (w.total > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < w.total))
     return FDLLM_ERR_WORKSPACE;
   if (w.scratch > 0 && (scratch == nullptr || !aligned16(scratch) || scratch_bytes < w.scratch))
@@ -1737,6 +1738,7 @@ extern "C" int fdllm_attn_cache_int4(const void* q, void* o, const void* k_cache
   p.n_rows = n_rows;
   p.n_seqs = n_seqs;
   p.batch = page_table != nullptr ? batch : static_cast<int32_t>(std::min<int64_t>(n_pages / p.pages_per_seq, 1 << 20));
+  p.batch = std::min(p.batch, n_seqs);  // (a sequence past it is reported)
   p.chunks = pl.chunks;
   p.splits = pl.splits;
   p.split_pages = pl.split_pages;
