@@ -47,6 +47,7 @@ struct A4Params {
   int64_t n_pages;
   float scale_log2;                // softmax_scale * log2(e)
   float score_scale;
+  float score_limit;               // of a term of the column sums (many rows: one a kv head)
   int32_t n_heads, n_kv, group;    // group = n_heads / n_kv
   int32_t seqlen_max, pages_per_seq;
   int32_t max_items, n_rows;
@@ -119,9 +120,16 @@ __device__ __forceinline__ int64_t a4_page(const A4Params& p, int seq, int n) {
   return page;
 }
 
-__device__ __forceinline__ void a4_add_score(unsigned long long* acc, float x, bool& ok) {
-  // |x| < 2^24: x * 2^32 is exact in fp32 and 128 such terms stay inside int64
-  const bool in = fabsf(x) < 16777216.f;  // false for NaN and infinities
+// The largest term of a key's column sum, of `terms` of them: their sum stays
+// below 2^31 (2^63 as fixed point), and a term below 2^24.
+__host__ __device__ inline float a4_score_limit(long long terms) {
+  int bits = 7;
+  while (bits < 62 && (1ll << bits) < terms) ++bits;
+  return bits <= 31 ? static_cast<float>(1u << (31 - bits)) : 0.f;
+}
+__device__ __forceinline__ void a4_add_score(unsigned long long* acc, float x, float limit, bool& ok) {
+  // (|x| < 2^24: x * 2^32 is exact in fp32)
+  const bool in = fabsf(x) < limit;  // false for NaN and infinities
   ok &= in;
   atomicAdd(acc, static_cast<unsigned long long>(in ? __float2ll_rn(x * 4294967296.f) : 0ll));
 }
@@ -237,6 +245,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) attn_int4_few_kernel(co
   constexpr int kRows = 4 * kE;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int s_last, s_convert;
+  __shared__ float s_limit;  // of a term of the column sums
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + kFewRing) + warp * kFewStages;
@@ -258,6 +267,12 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) attn_int4_few_kernel(co
   int n_splits = (seq_pages + p.split_pages - 1) / p.split_pages;
   const int cta_splits = n_splits;
   const bool scores_on = p.scores != nullptr && it.m_len > 0 && it.mchunk >= 0;
+  if (scores_on && threadIdx.x == 0) {
+    // a term a chunk and kv head: a sequence's chunks of kRows masked rows x
+    // heads (an item's 64 rows are whole chunks)
+    const int64_t masked = p.plan[p.plan[3] + kA4PlanSeq * it.seq + 4];
+    s_limit = a4_score_limit((masked * p.group + kRows - 1) / kRows * p.n_kv);
+  }
   __syncthreads();
 
   const int m_all = it.rows * p.group;
@@ -440,7 +455,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) attn_int4_few_kernel(co
             v += __shfl_xor_sync(0xffffffffu, v, 1);
             v += __shfl_xor_sync(0xffffffffu, v, 2);
             const int key = mt * 16 + 8 * hh + g;
-            if (t == mt && n0 + key < it.k_end) a4_add_score(sacc + key, v, range_ok);
+            if (t == mt && n0 + key < it.k_end) a4_add_score(sacc + key, v, s_limit, range_ok);
           }
       }
       live = mbar_wait(&bar[slot], parity, p.status, kA4KernelId);
@@ -1119,7 +1134,7 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
           const int n = first * kI4Page + t * kMnKeys + 32 * grp + lane;
           if (n < sq.k_end)
             a4_add_score(p.score_acc + static_cast<int64_t>(seq) * p.seqlen_max + n,
-                         ms.score[grp][0][lane] + ms.score[grp][1][lane] + ms.score[grp][2][lane], range_ok);
+                         ms.score[grp][0][lane] + ms.score[grp][1][lane] + ms.score[grp][2][lane], p.score_limit, range_ok);
           __syncwarp();
         }
         if (!soft) {
@@ -1730,6 +1745,7 @@ extern "C" int fdllm_attn_cache_int4(const void* q, void* o, const void* k_cache
   p.n_pages = n_pages;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.score_scale = score_scale;
+  p.score_limit = a4_score_limit(n_kv_heads);
   p.n_heads = n_heads;
   p.n_kv = n_kv_heads;
   p.group = n_heads / n_kv_heads;

@@ -284,7 +284,9 @@ int fdllm_read_cache_int4(const void* k_cache, const void* v_cache, const int64_
  * max_items as for fdllm_attn_cache, n_seqs the plan's batch_size (a plan of another one is reported as
  * FDLLM_ERR_TABLE and nothing is computed); page_table int32 [batch, pages_per_seq] or NULL (sequence b owns
  * pages [b * seqlen_max / 64, ...), seqlen_max a multiple of 64); a page outside the cache is reported as
- * FDLLM_ERR_INDEX and read as page 0.  attn_scores and score_scale as there.
+ * FDLLM_ERR_INDEX and read as page 0.  attn_scores and score_scale as there; a term of a column sum (the
+ * masked rows of a kv head, or four or eight rows x heads of them) is left out, and reported as
+ * FDLLM_ERR_RANGE, when it is non-finite or reaches 2^24, or 2^31 / T for T > 128 terms a key (T a power of two).
  *   rows_hint  rows of one sequence the caller expects at most (0: unknown): chooses the kernel and the
  *              split; results are right whatever it says
  *   kv_splits  key ranges per item (0: automatic)
