@@ -5,7 +5,7 @@
 // Two kernels.  With few rows the cache's bytes and the conversion of its codes
 // are all the work, and the step s and base b of a (token, head) group are
 // folded out of the products:
-//   q . k_n = s_n (q . c_n) + b_n sum_d q_d
+//   q . k_n = s_n (q . c_n) + b_n sum_d q_d      (or of c_n - 8 and b_n + 8 s_n)
 //   o_d     = [ sum_n (p_n s_n) c_nd + sum_n p_n b_n ] / sum_n p_n
 // so the matrix instructions see small integers, a key's step multiplies one
 // logit or one probability instead of 128 values, and the base costs one
@@ -179,10 +179,19 @@ __device__ __forceinline__ void a4_convert_scores(const A4Params& p, int seq, in
 // The codes are operands as they lie: a masked nibble at the foot of a half
 // word is the fp16 subnormal code * 2^-24, one nibble higher it is code *
 // 2^-20, and products with subnormals are exact.  Eight codes cost five
-// instructions (a shift, four masks).  The other operands are fp16 then: a
-// query row is divided by a power of two (and every second pair of dims by 16
-// more) so that its largest value lies in [2^13, 2^14), which drops what is
-// 2^-37 of it; p_n s_n is taken relative to the largest p_n v_n so far, v being
+// instructions (a shift, four masks).  Their sums lose bits, though: a logit is
+// off by 6e-7 of its size (it seems that a subnormal's product is aligned as if
+// its operand had the least normal exponent, up to 2^10 above it, and cut at
+// the accumulator's end).  That is nothing beside P's rounding, but the
+// importance scores are such sums themselves, and where rows' logits cancel it
+// shows (of one-key cases, one in twenty was off by 1e-5 of its score).  With
+// scores (kScores) K's operand is code - 8 as a normal fp16, four instructions
+// more: 6e-8, and 17.1 -> 17.8 us for 8 sequences of 2176 keys, 4 rows, 8 kv
+// heads.  (Starting the sums of codes at -8 sum_d q_d left 6e-7; adding each
+// instruction's sums in fp32, 4.5e-7.)
+// The other operands are fp16 then: a query row is divided by a power of two
+// (and, beside subnormal codes, every second pair of dims by 16 more) so that
+// its largest value lies in [2^13, 2^14), which drops what is 2^-37 of it; p_n s_n is taken relative to the largest p_n v_n so far, v being
 // the power of two at the largest value of a page (so 2^-39 of it is dropped,
 // and the rest is rounded by 2^-12).
 //
@@ -240,9 +249,25 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-template <int kE>
+// code - 8 of the pairs at bits 0 (even) or 4 (odd) of each half: 1024 + code
+// and 1024 + 16 code are fp16 values whose mantissas hold the code
+__device__ __forceinline__ uint32_t i4_even_f16(uint32_t w) {
+  uint32_t m, r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(m) : "r"(w), "n"(0x000f000f), "r"(0x64006400u));
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(m), "r"(0xE408E408u));  // - 1032
+  return r;
+}
+__device__ __forceinline__ uint32_t i4_odd_f16(uint32_t w) {
+  uint32_t m, r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(m) : "r"(w), "n"(0x00f000f0), "r"(0x64006400u));
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(m), "r"(0x2C002C00u), "r"(0xD480D480u));  // / 16 - 72
+  return r;
+}
+
+template <int kE, bool kScores>
 __global__ void __launch_bounds__(kFewThreads, kFewCtas) attn_int4_few_kernel(const A4Params p) {
   constexpr int kRows = 4 * kE;
+  constexpr int kLift = kScores ? 0 : 24;  // K's operand is this many powers of two below the codes
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int s_last, s_convert;
   __shared__ float s_limit;  // of a term of the column sums
@@ -266,7 +291,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) attn_int4_few_kernel(co
   if (first >= seq_pages) return;
   int n_splits = (seq_pages + p.split_pages - 1) / p.split_pages;
   const int cta_splits = n_splits;
-  const bool scores_on = p.scores != nullptr && it.m_len > 0 && it.mchunk >= 0;
+  const bool scores_on = kScores && it.m_len > 0 && it.mchunk >= 0;
   if (scores_on && threadIdx.x == 0) {
     // a term a chunk and kv head: a sequence's chunks of kRows masked rows x
     // heads (an item's 64 rows are whole chunks)
@@ -354,17 +379,17 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) attn_int4_few_kernel(co
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&qf[j]));
-        const float d = (j & 1) ? down16 : down;
+        const float d = (j & 1) && !kScores ? down16 : down;
         qf[j] = pack_half2(f.x * d, f.y * d);
       }
     }
-    // logits are kept divided by 2^(24 + eq)
-    const float qsn = qs * pow2i(-max(min(eq + 24, 126), -126));
+    // logits are kept divided by 2^(kLift + eq)
+    const float qsn = qs * pow2i(-max(min(eq + kLift, 126), -126));
     float qsum[kE], up[kE], mul[kE];
 #pragma unroll
     for (int e = 0; e < kE; ++e) {
       qsum[e] = __shfl_sync(0xffffffffu, qsn, 8 * t + 4 * e);
-      up[e] = pow2i(24 + __shfl_sync(0xffffffffu, eq, 8 * t + 4 * e));
+      up[e] = pow2i(kLift + __shfl_sync(0xffffffffu, eq, 8 * t + 4 * e));
       mul[e] = up[e] * p.scale_log2;
     }
     // this lane's rows of the chunk; masked ones count into the scores
@@ -413,7 +438,8 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) attn_int4_few_kernel(co
           for (int h = 0; h < 4; ++h) {
             const uint32_t x = (ks & 1) ? w[2 * h][ks >> 1] >> 8 : w[2 * h][ks >> 1];
             const uint32_t y = (ks & 1) ? w[2 * h + 1][ks >> 1] >> 8 : w[2 * h + 1][ks >> 1];
-            const uint32_t a[4] = {x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u};
+            const uint32_t a[4] = {kScores ? i4_even_f16(x) : x & 0x000f000fu, kScores ? i4_even_f16(y) : y & 0x000f000fu,
+                                   kScores ? i4_odd_f16(x) : x & 0x00f000f0u, kScores ? i4_odd_f16(y) : y & 0x00f000f0u};
             mma_f16(sc[h], a, qf[2 * ks], qf[2 * ks + 1]);
           }
       }
@@ -429,10 +455,11 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) attn_int4_few_kernel(co
           const int key = mt * 16 + 8 * hh + g;
           const uint32_t pr = kp[key];
           const float st = __uint_as_float(pr << 16), low = __uint_as_float(pr & 0xffff0000u);
+          const float base = kScores ? fmaf(8.f, st, low) : low;  // of code - 8, or of the code
           const bool in = whole || n0 + key < it.k_end;
 #pragma unroll
           for (int e = 0; e < kE; ++e) {
-            const float raw = fmaf(st, sc[mt][2 * hh + e], low * qsum[e]);
+            const float raw = fmaf(st, sc[mt][2 * hh + e], base * qsum[e]);
             sc[mt][2 * hh + e] = in ? raw : -INFINITY;  // (a select: what lies past the end may be NaN)
             pm[e] = fmaxf(pm[e], sc[mt][2 * hh + e]);
           }
@@ -837,20 +864,6 @@ __device__ __forceinline__ uint8_t* ext_chunk(uint8_t* base, int row, int chunk)
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
-}
-// code - 8 of the pairs at bits 0 (even) or 4 (odd) of each half: 1024 + code
-// and 1024 + 16 code are fp16 values whose mantissas hold the code
-__device__ __forceinline__ uint32_t i4_even_f16(uint32_t w) {
-  uint32_t m, r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(m) : "r"(w), "n"(0x000f000f), "r"(0x64006400u));
-  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(m), "r"(0xE408E408u));  // - 1032
-  return r;
-}
-__device__ __forceinline__ uint32_t i4_odd_f16(uint32_t w) {
-  uint32_t m, r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(m) : "r"(w), "n"(0x00f000f0), "r"(0x64006400u));
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(m), "r"(0x2C002C00u), "r"(0xD480D480u));  // / 16 - 72
-  return r;
 }
 __device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t r;
@@ -1671,13 +1684,7 @@ A4Plan a4_plan(int32_t n_rows, int32_t max_items, int32_t n_seqs, int32_t n_head
                int32_t kv_splits, int32_t rows_hint, bool scores) {
   const int items = std::max(n_seqs, max_items - n_seqs);  // (the capacity: an item per 64 rows and one a sequence)
   const int seq_rows = rows_hint > 0 && rows_hint < n_rows ? rows_hint : n_rows;
-  // Scores of a page's keys at most: a few sums over rows and heads, which may
-  // cancel to little.  The few-rows kernel's products are of codes 0 .. 15, four
-  // times the logits, and their sums' errors with them: of 300 random cases of
-  // one key, 5 were off by more than 1e-5 of the scores' norm (median 6e-7), of
-  // the other kernel none (1.2e-7).  From 4 keys on neither was.  (8 sequences of
-  // 64 keys, 4 rows, 8 kv heads: 10.4 us against 12.5.)
-  if (static_cast<long long>(seq_rows) * (n_heads / n_kv) > kFewMaxRows || (scores && seqlen_max <= kI4Page))
+  if (static_cast<long long>(seq_rows) * (n_heads / n_kv) > kFewMaxRows)
     return a4_plan_many(n_seqs, seq_rows, n_heads / n_kv, n_kv, seqlen_max, kv_splits, scores);
   const int rows = seq_rows < kA4ItemRows ? seq_rows : kA4ItemRows;
   return a4_plan_few(items, rows, n_heads / n_kv, n_kv, seqlen_max, kv_splits);
@@ -1762,12 +1769,11 @@ extern "C" int fdllm_attn_cache_int4(const void* q, void* o, const void* k_cache
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return FDLLM_ERR_CUDA;
   if (!attr[dev]) {
-    if (cudaFuncSetAttribute(attn_int4_few_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem) !=
-            cudaSuccess ||
-        cudaFuncSetAttribute(attn_int4_few_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem) !=
-            cudaSuccess ||
-        cudaFuncSetAttribute(attn_int4_many_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMnSmem) !=
-            cudaSuccess)
+    for (const auto f : {attn_int4_few_kernel<1, false>, attn_int4_few_kernel<1, true>, attn_int4_few_kernel<2, false>,
+                         attn_int4_few_kernel<2, true>})
+      if (cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem) != cudaSuccess)
+        return FDLLM_ERR_CUDA;
+    if (cudaFuncSetAttribute(attn_int4_many_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMnSmem) != cudaSuccess)
       return FDLLM_ERR_CUDA;
     attr[dev] = true;
   }
@@ -1780,8 +1786,10 @@ extern "C" int fdllm_attn_cache_int4(const void* q, void* o, const void* k_cache
   }
   const dim3 grid(static_cast<unsigned>(max_items) * pl.chunks, static_cast<unsigned>(n_kv_heads),
                   static_cast<unsigned>(pl.splits));
-  if (launch_ex(pl.narrow ? attn_int4_few_kernel<1> : attn_int4_few_kernel<2>, grid, dim3(kFewThreads), kFewSmem, stream,
-                1, pdl_enabled(), p) != cudaSuccess)
+  const auto few = attn_scores != nullptr
+                       ? (pl.narrow ? attn_int4_few_kernel<1, true> : attn_int4_few_kernel<2, true>)
+                       : (pl.narrow ? attn_int4_few_kernel<1, false> : attn_int4_few_kernel<2, false>);
+  if (launch_ex(few, grid, dim3(kFewThreads), kFewSmem, stream, 1, pdl_enabled(), p) != cudaSuccess)
     return FDLLM_ERR_CUDA;
   return cudaPeekAtLastError() == cudaSuccess ? FDLLM_OK : FDLLM_ERR_CUDA;
 }

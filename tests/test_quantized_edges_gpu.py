@@ -39,3 +39,49 @@ def test_column_sums_of_many_large_terms(hint, rows):
             assert e.value.code == RANGE
             assert not sc.any()
         assert (out == 1).all()
+
+
+def _score_error(seed, seqs, h, hk, length, cancel, hint):
+    """(|error|^2, the bound's square) of a case's scores, each key's summed.
+
+    What 32-bit sums have to cost a logit sum_d q_d (c_d - 8) s + b sum_d q_d: 128
+    products added 16 at a time, 8 sums whose last places are half cut, half a
+    unit 2^-24 each, of partial sums that grow as a random walk to A = the root
+    of the products' squares: 2^-24 A sum_j sqrt(j / 8) = 5.6 2^-24 A; then two
+    roundings of it and of the base's part, B.  Errors of different rows and heads
+    are independent (squares add)."""
+    from flash_dllm_b200 import ops
+    q, caches, pt, spans, mb, tb, B, L = tq._attention_case(seed, seqs, h, hk, length)
+    if cancel:  # the second half of a sequence's masked rows against the first
+        for _, _, masked, _ in spans:
+            m = len(masked) // 2
+            a = q[masked[0]:masked[0] + m].float()
+            q[masked[0] + m:masked[0] + 2 * m] = (0.015625 * torch.randn_like(a) - a).bfloat16()
+    sc, out = torch.zeros(B * L, device="cuda"), torch.empty_like(q)
+    plan, cap = ops.plan_cache_attention(mb, tb, q.shape[0], B, 64, L, q.device)
+    ops.attn_cache_int4(q, out, *caches, plan, cap, sc, 1.0, h, hk, L, 128 ** -0.5, rows_hint=hint, page_table=pt)
+    _, _, ref, _ = qr.attention(q, *caches, pt, spans, h, hk, 128 ** -0.5, 1.0, B, L)
+    u, err2, bound2 = 2.0 ** -24, (sc.double() - ref) ** 2, torch.zeros_like(ref)
+    for b, k_end, masked, _ in spans:
+        c, s, low = (t.transpose(0, 1).flatten(1, 2)[:, :k_end] for t in qr.int4_unpack(caches[0][pt[b, :-(-k_end // 64)].long()]))
+        x = q[list(masked)].double().reshape(len(masked), hk, h // hk, 128).permute(1, 0, 2, 3).flatten(1, 2)
+        a2 = (x ** 2) @ (((c - 8) * s[..., None]) ** 2).transpose(1, 2)
+        b2 = x.sum(-1, keepdim=True) ** 2 * ((low + 8 * s) ** 2)[:, None]
+        bound2[b * L:b * L + k_end] = (u * u * (7.6 ** 2 * a2 + 4 * b2)).sum((0, 1))
+    bound2 += (2.0 ** -33 * h * 64) ** 2 + (2 * u * ref) ** 2  # fixed point, and the sum as fp32
+    assert (err2[ref == 0] == 0).all()
+    keep = ref != 0
+    return err2[keep], bound2[keep]
+
+
+@pytest.mark.parametrize("length", [64, 128, 2176])
+@pytest.mark.parametrize("cancel", [False, True])
+@pytest.mark.parametrize("keys,rows,h,hk", [(1, 1, 8, 8), (1, 4, 8, 2), (2, 8, 4, 4), (3, 4, 8, 8), (1, 32, 4, 4), (1, 40, 4, 4)])
+def test_scores_of_few_keys(keys, rows, h, hk, cancel, length):
+    """A slot's capacity says nothing about its keys: with one to three of them
+    the column sums cancel to little, and are right to 32 bits all the same."""
+    err2, bound2 = zip(*[_score_error(seed, [(keys, rows, 0), (max(1, keys - 1), rows, 0)], h, hk, length, cancel, rows)
+                         for seed in range(700, 720)])
+    err2, bound2 = torch.cat(err2), torch.cat(bound2)
+    assert err2.sum() <= bound2.sum(), (err2.sum() / bound2.sum()) ** 0.5
+    assert (err2 <= 16 * bound2).all()  # four deviations
