@@ -37,6 +37,10 @@ Two options, each on its own or together:
 - a 4-bit cache (``k_cache`` / ``v_cache`` from ``ops.int4_cache``): Q and K are
   rotated and K and V quantised on the way into the pages, attention reads the
   4-bit pages, and the verify attention the keys and values they stand for.
+  ``lengths[10]`` (None in the reference) may hold the most rows that a sequence
+  of the forward has, by which that attention divides its work; without it the
+  mean is taken, which is right and, where one sequence has many more rows than
+  the others, slower (1 x 2000 and 7 x 64 rows: 246 against 202 us).
 """
 from __future__ import annotations
 
@@ -182,7 +186,7 @@ def quantize_block_int8(block) -> None:
 def flash_fused_elastic_cache(self, x: torch.Tensor, block_idx, positions, lengths, softmax_scale: float = None):
     query_pos_flat, key_pos_flat, rotary_emb_pos, _info, attn_scores, attn_mask = positions
     (_start_layer, query_verify_blocks, query_masked_blocks, query_tracked_blocks, _query_blocks, active_batch,
-     _num_active, max_length, block_m, _block_n, _elastic, verify) = lengths
+     _num_active, max_length, block_m, _block_n, max_rows, verify) = lengths
     d_model = self.config.d_model
     n_heads = self.config.n_heads
     head_dim = d_model // n_heads
@@ -232,7 +236,7 @@ def flash_fused_elastic_cache(self, x: torch.Tensor, block_idx, positions, lengt
             if four_bits:
                 ops.attn_cache_int4(q, att, self.k_cache, self.v_cache, plan, cap, scores, 1.0 / (block_m * n_heads),
                                     n_heads, n_heads, max_length, softmax_scale,
-                                    rows_hint=-(-n_rows // max(1, len(active_batch))))
+                                    rows_hint=max_rows if max_rows else -(-n_rows // max(1, len(active_batch))))
             else:
                 ops.attn_cache(q, att, self.k_cache, self.v_cache, plan, cap, scores, 1.0 / (block_m * n_heads),
                                n_heads, max_length, softmax_scale, items_hint=-(-n_rows // 64))

@@ -377,19 +377,22 @@ def generate_with_Flash_dLLM(model, prompts, prompt_lengths, batch_size, respons
         pk.add(seqtab[:, 2])
         pk.add(seqtab[:, 3])
         seq_d, eos_known, act_d, nd_d, pred_d = pk.send(h2d)
-        ckey = ("cache", r_m + int(t_n.sum()), n_m, n_t, r_m)
+        # (the 4-bit attention's grid follows the most rows of a sequence, so a
+        # captured forward serves those of its multiple of 32)
+        max_rows = -(-int((m_n + t_n).max()) // 32) * 32 if kv_bits == 4 else None
+        ckey = ("cache", r_m + int(t_n.sum()), n_m, n_t, r_m, max_rows)
         st_in = forward.static_inputs(ckey)
         tables, query_pos_flat, x_query, seq_info = ops.cache_build(
             seq_d.view(-1, 16), r_m + int(t_n.sum()), n_m + n_t, bm, full_pos, x,
             out=None if st_in is None else (st_in["tables"], st_in["qpos"], st_in["x"]))
         eos_known = eos_known.to(torch.int32)
 
-        def cache_forward(t, hook, n_m=n_m, r_m=r_m, has_t=n_t > 0):
+        def cache_forward(t, hook, n_m=n_m, r_m=r_m, has_t=n_t > 0, max_rows=max_rows):
             masked_blocks = t["tables"][:n_m] if n_m else empty_i32
             tracked_blocks = t["tables"][n_m:] if has_t else empty_i32
             positions = [t["qpos"], empty_i64, rotary_emb_pos, [], attn_scores, []]
             lengths = [start_layer, None, masked_blocks, tracked_blocks, t["tables"], st.active, n_m, L, bm, bn,
-                       None, False]
+                       max_rows, False]
             return _call_model(model, t["x"].unsqueeze(0), lengths, positions, r_m, hook)
 
         logits = forward(ckey,

@@ -85,3 +85,43 @@ def test_scores_of_few_keys(keys, rows, h, hk, cancel, length):
     err2, bound2 = torch.cat(err2), torch.cat(bound2)
     assert err2.sum() <= bound2.sum(), (err2.sum() / bound2.sum()) ** 0.5
     assert (err2 <= 16 * bound2).all()  # four deviations
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+def test_driver_hints_at_the_most_rows_of_a_sequence(graphs, monkeypatch):
+    """Prompts of unequal length: what the 4-bit attention is told covers every
+    sequence of the forward, also where a captured one is replayed."""
+    import cases
+    import test_generate_gpu as tg
+    from flash_dllm_b200 import generate as gen, ops
+    model = tg._model()
+    calls, forwards = [], []
+    attn, call = ops.attn_cache_int4, gen._Forwarder.__call__
+
+    def spy(q, o, kc, vc, plan, capacity, *a, rows_hint=0, **kw):
+        calls.append((plan, rows_hint))
+        return attn(q, o, kc, vc, plan, capacity, *a, rows_hint=rows_hint, **kw)
+
+    def forward(self, key, inputs, build):
+        if key[0] == "cache":
+            t = inputs["tables"].cpu()
+            rows = [int((t[t[:, 0] == b, 3] - t[t[:, 0] == b, 2]).sum()) for b in t[:, 0].unique()]
+            forwards.append((key, max(rows), len(rows)))
+        return call(self, key, inputs, build)
+
+    monkeypatch.setattr(ops, "attn_cache_int4", spy)
+    monkeypatch.setattr(gen._Forwarder, "__call__", forward)
+    resp, steps = [None] * 3, [0] * 3
+    lens = [20, 150, 24]
+    g = torch.Generator().manual_seed(3)
+    prompts = [torch.randint(0, 500, (n,), generator=g).cuda() for n in lens]
+    gen.generate_with_Flash_dLLM(model, prompts, lens, 2, resp, steps, gen_length=32, kv_bits=4, use_graphs=graphs,
+                                 **cases.GEN_KW)
+    assert len(forwards) > 3 and any(k[1] < n * m for k, m, n in forwards)  # (unequal)
+    for key, most, _ in forwards:
+        assert most <= key[-1] < most + 32
+    if not graphs:
+        assert {h for _, h in calls} == {k[-1] for k, _, _ in forwards}
+        for plan, hint in calls:
+            seq = plan[int(plan[3]):].view(-1, 8).cpu()
+            assert int((seq[:, 4] + seq[:, 6]).max()) <= hint
