@@ -72,6 +72,16 @@ __device__ __forceinline__ bool a4_wait(uint64_t* bar, uint32_t parity, int32_t*
   return a4_timeout(status);
 }
 
+// Both kernels' references follow the largest contribution, weight times the
+// size of the values, and the sum of weights is kept relative to it.  Beside
+// pages of values near 2^-100 (zeros count as that) or far above 1 the sum is
+// itself a number of that size: it is scaled by 2^x in two halves, which
+// cannot vanish on the way, and a page's own part of it is summed from the
+// weights where the values are below 2^-60 (their P, which fp32 may not hold
+// there, contributes nothing then).
+constexpr int kA4LowV = -60;
+__device__ __forceinline__ float a4_half(float x) { return ex2_approx(0.5f * x); }
+
 struct A4Item {
   int seq, k_end, m_start, m_len, t_start, rows, mchunk;
 };
@@ -513,8 +523,9 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) attn_int4_few_kernel(co
         float al[2] = {0.f, 0.f};
 #pragma unroll
         for (int e = 0; e < kE; ++e) {
-          al[e] = ex2_approx(mx[e] - ref[e]);
-          l[e] *= al[e];
+          const float h = a4_half(mx[e] - ref[e]);
+          al[e] = h * h;
+          l[e] = l[e] * h * h;
           pb[e] *= al[e];
           mx[e] = pm[e];
         }
@@ -525,6 +536,14 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) attn_int4_few_kernel(co
             acc[jj][e] *= al[e];
             acc[jj][2 + e] *= al[e];
           }
+      }
+      float ln = vn;
+      if (ev < kA4LowV) {  // (uniform)
+        ln = 0.f;
+#pragma unroll
+        for (int e = 0; e < kE; ++e)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) l[e] += ex2_approx(fmaf(sc[k >> 1][2 * (k & 1) + e], mul[e], -ref[e]));
       }
       uint32_t bf[4][2];
       float lp[kE];
@@ -552,7 +571,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) attn_int4_few_kernel(co
           bf[mt][hh] = transpose8x8(pack_half2(w[0], w[1]));
         }
 #pragma unroll
-      for (int e = 0; e < kE; ++e) l[e] = fmaf(lp[e], vn, l[e]);
+      for (int e = 0; e < kE; ++e) l[e] = fmaf(lp[e], ln, l[e]);
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
         const uint8_t* vr = vb + (mt * 16 + 2 * t) * kI4Row + 8 * g;
@@ -630,9 +649,9 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) attn_int4_few_kernel(co
 #pragma unroll
     for (int w = 0; w < kFewWarps; ++w) {
       const float* pw = reinterpret_cast<const float*>(smem) + w * kFewPartFloats;
-      const float f = ex2_approx(pw[r] - Mr);
+      const float h = a4_half(pw[r] - Mr), f = h * h;
       const float4 v = *reinterpret_cast<const float4*>(pw + 2 * kFewRows + r * kA4HeadDim + 4 * c);
-      L = fmaf(f, pw[kFewRows + r], L);
+      L = fmaf(h, h * pw[kFewRows + r], L);
       O.x = fmaf(f, v.x, O.x);
       O.y = fmaf(f, v.y, O.y);
       O.z = fmaf(f, v.z, O.z);
@@ -668,9 +687,9 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) attn_int4_few_kernel(co
 #pragma unroll 4
         for (int k = 0; k < n_splits; ++k) {
           const float* ps = all + k * kFewPartFloats;
-          const float f = ex2_approx(__ldcg(ps + r) - ref);
+          const float h = a4_half(__ldcg(ps + r) - ref), f = h * h;
           const float4 v = __ldcg(reinterpret_cast<const float4*>(ps + 2 * kFewRows + r * kA4HeadDim) + c);
-          L = fmaf(f, __ldcg(ps + kFewRows + r), L);
+          L = fmaf(h, h * __ldcg(ps + kFewRows + r), L);
           O.x = fmaf(f, v.x, O.x);
           O.y = fmaf(f, v.y, O.y);
           O.z = fmaf(f, v.z, O.z);
@@ -968,7 +987,7 @@ struct MnMisc {
   // [tile % 8][32-key piece]: who writes tile t's has seen S(t - 2), so P V(t - 5),
   // so the softmax of every tile up to t - 5
   alignas(16) int32_t ek[8][4];
-  alignas(16) int32_t ev[8][4];
+  alignas(16) float2 ev[8][4];  // the exponent, and 2^-ev (0 below kA4LowV)
   float red[4][8];                  // score rows: warp partials
   float q_amax[2][kMnRows], q_sum[2][kMnRows];
   float q_mul[kMnRows];             // 2^e of the rows
@@ -1133,7 +1152,7 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
         float v[32];
         tmem_ld_32x32b_x32(ts, v);
         const float k = pow2i(ms.ek[t & 7][grp] - kMnUp);
-        const int ev = ms.ev[t & 7][grp];
+        const float2 ev = ms.ev[t & 7][grp];
         if (score_warp) {
           // lanes 24 .. 26 hold the three parts' logits
           if (lane >= 24 && lane < 27) {
@@ -1157,15 +1176,15 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
         }
         // (not 0, however small the query and the keys: a key past the end is -infinity times this)
         const float mul = fmaxf(log_mul * k, 0x1p-126f);
-        ms.mx[t & 1][r][grp] = fmaf(mn_max32(v), mul, static_cast<float>(ev));
+        ms.mx[t & 1][r][grp] = fmaf(mn_max32(v), mul, ev.x);
         asm volatile("bar.sync %0, 128;" ::"r"(3 + (warp & 3)) : "memory");
         const float4 m4 = *reinterpret_cast<const float4*>(ms.mx[t & 1][r]);
         const float mt = fmaxf(max3(m4.x, m4.y, m4.z), m4.w);
         // the reference moves if this tile passes it (a row's four threads
         // decide the same)
         const bool need = mt > ref + kMnLazy;
-        if (__any_sync(0xffffffffu, need)) {
-          const float a = need ? ex2_approx(ref - mt) : 1.f;
+        if (__any_sync(0xffffffffu, need || ev.y == 0.f)) {
+          const float h = need ? a4_half(ref - mt) : 1.f, a = h * h;
           if (t > 0) {
             // O holds P V of the tiles before; each key quarter scales a quarter of its dims
             ok = ok && a4_wait(&ms.pv_done[(t - 1) % 3], ((t - 1) / 3) & 1, p.status);
@@ -1181,11 +1200,21 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
           }
           if (need) {
             ref = mt;
-            l *= a;
+            l = l * h * h;
+          }
+          if (ev.y == 0.f) {  // (uniform) the weights' own sum, of S once more
+            const float s0 = kMnRaise - (ref == -INFINITY ? 0.f : ref);
+#pragma unroll 1
+            for (int c = 0; c < 2; ++c) {
+              float w[16];
+              tmem_ld_32x32b_x16(ts + 16 * c, w);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) l = fmaf(ex2_approx(fmaf(w[j], mul, s0)), 0x1p-14f, l);
+            }
           }
         }
         // P = 2^(logit + ev - R + kMnRaise)
-        const float shift = kMnRaise - (ref == -INFINITY ? 0.f : ref) + static_cast<float>(ev);
+        const float shift = kMnRaise - (ref == -INFINITY ? 0.f : ref) + ev.x;
         const uint64_t shift2 = pack_f32x2(shift, shift), mul2 = pack_f32x2(mul, mul);
         uint64_t ps[2] = {0ull, 0ull};  // (zero pairs)
         uint32_t pw[16];
@@ -1200,7 +1229,7 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
         }
         float x, y;
         unpack_f32x2(add_f32x2(ps[0], ps[1]), x, y);
-        l = fmaf((x + y) * 0x1p-14f, pow2i(-ev), l);  // (with ev = -100, of values of zero alone, still far from the end)
+        l = fmaf((x + y) * 0x1p-14f, ev.y, l);
         // over the first half of the logits that this thread has read
         tmem_st_32x32b_x16(ts, pw);
         tmem_wait_st();
@@ -1275,7 +1304,8 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
 #pragma unroll 4
             for (int k = 0; k < n_splits; ++k) {
               const float* q = ml + k * kMnPartFloats + r;
-              L = fmaf(ex2_approx(__ldcg(q) - top), __ldcg(q + kMnRows), L);
+              const float h = a4_half(__ldcg(q) - top);
+              L = fmaf(h, h * __ldcg(q + kMnRows), L);
             }
             const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
             __nv_bfloat16* dst = p.o + mn_row(p, sq, kvh, m0 + r) + 32 * grp;
@@ -1494,7 +1524,9 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
           // before this wait sees it, as P V(t) needs what follows)
           if (t >= 3 && !a4_wait(&ms.pv_done[t % 3], (t / 3 - 1) & 1, p.status)) break;
           if (lane == 0) {
-            *reinterpret_cast<int4*>(ms.ev[t & 7]) = make_int4(e[0], e[1], e[2], e[3]);
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+              ms.ev[t & 7][g] = make_float2(static_cast<float>(e[g]), e[g] < kA4LowV ? 0.f : pow2i(-e[g]));
             mbar_arrive(&ms.s_full[t % 3]);
           }
         }

@@ -279,7 +279,9 @@ int fdllm_read_cache_int4(const void* k_cache, const void* v_cache, const int64_
                           const int32_t* page_table, int32_t batch, int32_t pages_per_seq, cudaStream_t stream);
 
 /* fdllm_attn_cache over the 4-bit cache.  q, o bf16 [n_rows, n_heads * 128], not overlapping, |q| below
- * 2^117 (a row with an infinity or NaN answers NaN); seqlen_max at most 2^30; n_heads a multiple of
+ * 2^117 (a row with an infinity or NaN answers NaN); |v| below 2^48, or a
+ * sequence and head's pages' largest values within 2^100 of one another (the sum of weights is kept in
+ * units of the largest contribution); seqlen_max at most 2^30; n_heads a multiple of
  * n_kv_heads (query head h reads kv head h / (n_heads / n_kv_heads); at most 64 per kv head); plan and
  * max_items as for fdllm_attn_cache, n_seqs the plan's batch_size (a plan of another one is reported as
  * FDLLM_ERR_TABLE and nothing is computed); page_table int32 [batch, pages_per_seq] or NULL (sequence b owns

@@ -125,3 +125,23 @@ def test_driver_hints_at_the_most_rows_of_a_sequence(graphs, monkeypatch):
         for plan, hint in calls:
             seq = plan[int(plan[3]):].view(-1, 8).cpu()
             assert int((seq[:, 4] + seq[:, 6]).max()) <= hint
+
+
+@pytest.mark.parametrize("rows", [1, 6, 40])
+@pytest.mark.parametrize("zeros", ["first", "last", "between"])
+@pytest.mark.parametrize("small", [0.0, 2.0 ** -96])
+def test_attention_beside_pages_of_zero_values(rows, zeros, small):
+    """Pages whose values are zero, or far below their neighbours' 2^23, have
+    their share of the weights in any order."""
+    length, h = 384, 2
+    q, caches, pt, spans, mb, tb, B, L = tq._attention_case(24, [(length, rows, 0), (320, rows, 0)], h, h, length)
+    g = tq._gen(5)
+    big = {"first": [2, 3, 4, 5], "last": [0, 1], "between": [1, 4]}[zeros]
+    v = tq._randn(g, caches[1].shape[0], h, 64, 128).bfloat16() * small
+    for b in range(B):
+        for p in big:
+            v[pt[b, p].long()] = (2.0 ** 22 * tq._randn(g, h, 64, 128)).clamp(-2.0 ** 23.9, 2.0 ** 23.9).bfloat16()
+    q[::2] = 0  # equal weights; the others' logits differ
+    caches = [caches[0], qr.int4_pack(v)]
+    out, sc = tq._run_attention(q, caches, pt, mb, tb, B, L, h, h)
+    tq._check_attention(q, caches, pt, spans, B, L, h, h, out, sc)
