@@ -146,6 +146,36 @@ struct Call {
   }
 };
 
+// Bytes of `rows` rows of `width` at a stride; a contiguous tensor is one row.
+struct Span {
+  int64_t at, rows, stride, width;
+};
+Span span(const Tensor& t) { return {reinterpret_cast<int64_t>(t.data_ptr()), 1, 0, static_cast<int64_t>(t.nbytes())}; }
+Span span(const Tensor& t, int64_t ld) {
+  const int64_t size = t.element_size(), width = t.size(1) * size;
+  if (ld == t.size(1)) return span(t);
+  return {reinterpret_cast<int64_t>(t.data_ptr()), t.size(0), ld * size, width};
+}
+// Whether two of them share a byte (with different strides: whether their
+// ranges meet).  Rows of one tensor do not overlap.
+bool meet(const Span& a, const Span& b) {
+  if (a.rows == 0 || b.rows == 0 || a.width == 0 || b.width == 0) return false;
+  const auto end = [](const Span& s) { return s.at + (s.rows - 1) * s.stride + s.width; };
+  if (end(a) <= b.at || end(b) <= a.at) return false;
+  if (a.rows > 1 && b.rows == 1) return meet(b, a);
+  if (a.rows > 1 && a.stride != b.stride) return true;
+  if (b.rows == 1) return true;
+  const auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y != 0 && x < 0); };
+  if (a.rows == 1) {  // the first row of b that ends behind a's begin
+    const int64_t i = std::max<int64_t>(0, floor_div(a.at - b.at - b.width, b.stride) + 1);
+    return i < b.rows && b.at + i * b.stride < a.at + a.width;
+  }
+  // b's row j begins `off` behind the begin of a's row k + j
+  const int64_t k = floor_div(b.at - a.at, a.stride), off = b.at - a.at - k * a.stride;
+  const auto any = [&](int64_t k0) { return std::max<int64_t>(0, -k0) <= std::min(b.rows - 1, a.rows - 1 - k0); };
+  return (off < a.width && any(k)) || (off + b.width > a.stride && any(k + 1));
+}
+
 // (the allocator itself: at::empty's way through the dispatcher costs as much
 // again as the allocation, at up to three outputs a call)
 Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
@@ -208,6 +238,15 @@ Tensor linear_int8(const Tensor& a, const Tensor& a_scale, const Tensor& w, cons
   const int64_t ld_res = residual.has_value() ? c.rows(*residual, "residual", s.rows, s.n) : 0;
   Tensor y = out.has_value() ? *out : empty({s.rows, s.n}, at::kBFloat16, a);
   const int64_t ld_out = out.has_value() ? c.rows(y, "out", s.rows, s.n) : s.n;
+  if (out.has_value()) {
+    const Span o = span(y, ld_out);
+    for (const Tensor* t : {&a, &a_scale, &w, &w_scale})
+      TORCH_CHECK_VALUE(!meet(o, span(*t)), "out must not overlap the operands");
+    if (residual.has_value()) {  // (the residual itself: a value is read by the thread that writes it)
+      const bool itself = y.data_ptr() == residual->data_ptr() && ld_out == ld_res;
+      TORCH_CHECK_VALUE(itself || !meet(o, span(*residual, ld_res)), "out must not overlap the residual, unless it is it");
+    }
+  }
   size_t size = 0;
   void* ws = workspaces().get(a.device(), c.stream, "int8", fdllm_gemm_int8_workspace_bytes(s.rows, s.n, s.k, 0),
                               kGemmFlagBytes, &size);
@@ -305,6 +344,17 @@ Tensor rope_append(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
                       n_heads * kHead, "], got ", out.sizes());
   } else if (sin.has_value()) {
     out = empty({rows, n_heads * kHead}, at::kBFloat16, q);
+  }
+  // what is written overlaps nothing else, but for q_out, which may be q
+  const Span ks = span(k_cache), vs = span(v_cache), in[] = {span(q, ldq), span(k, ldk), span(v, ldv)};
+  TORCH_CHECK_VALUE(!meet(ks, vs), "k_cache and v_cache must not overlap");
+  for (const Span& x : in)
+    TORCH_CHECK_VALUE(!meet(ks, x) && !meet(vs, x), "q, k and v must not overlap the caches");
+  if (out.defined() && q_out.has_value()) {
+    const Span o = span(out);
+    const bool itself = out.data_ptr() == q.data_ptr() && ldq == n_heads * kHead;
+    TORCH_CHECK_VALUE((itself || !meet(o, in[0])) && !meet(o, in[1]) && !meet(o, in[2]) && !meet(o, ks) && !meet(o, vs),
+                      "q_out must not overlap k, v or the caches, nor q, unless it is q");
   }
   check_status("fdllm_rope_append",
                fdllm_rope_append(q.data_ptr(), k.data_ptr(), v.data_ptr(), ldq, ldk, ldv,

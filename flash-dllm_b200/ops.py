@@ -232,7 +232,8 @@ def linear_int8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale
                 residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """bf16((a @ w.T) * a_scale[:, None] * w_scale (+ residual)) of int8 a
     [rows, k] and w [n, k]: an exact integer sum, scaled in fp32, rounded once.
-    k a multiple of 16, n of 8.  ``residual`` and ``out`` may be row-strided."""
+    k a multiple of 16, n of 8.  ``residual`` and ``out`` may be row-strided, and
+    ``out`` the residual itself; otherwise it may not overlap what is read."""
     return _T.linear_int8(a, a_scale, w, w_scale, residual, out)
 
 
@@ -263,7 +264,8 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.
     n_kv_heads * 128] or 4-bit (:func:`int4_cache`); ``page_table`` int32 [batch,
     pages]: position p of sequence b is line p % 64 of page
     ``page_table[b, p // 64]`` (None: page slot // 64).  Returns the rotated Q
-    [rows, n_heads * 128]; ``q_out`` may be ``q`` itself."""
+    [rows, n_heads * 128]; ``q_out`` may be ``q`` itself.  Nothing else that is
+    written may overlap what is read."""
     return _T.rope_append(q, k, v, slots, sin, cos, k_cache, v_cache, n_heads, n_kv_heads, seqlen_max, page_table, q_out)
 
 

@@ -137,7 +137,7 @@ int fdllm_rmsnorm_int8(const void* x, const void* weight, void* codes, float* sc
 /* 8-bit integer product with a scale per token and per output channel:
  *   out[r, c] = bf16(float(sum_k a[r, k] * w[c, k]) * a_scale[r] * w_scale[c] (+ residual[r, c]))
  * a int8 [n_rows, k_dim], w int8 [n_cols, k_dim] (both contiguous), scales fp32, out / residual bf16 with
- * row strides ld_out / ld_res elements (residual may be NULL).  The sum is an exact 32-bit integer,
+ * row strides ld_out / ld_res elements (residual may be NULL, or out itself; no other overlap).  The sum is an exact 32-bit integer,
  * rounded to fp32 once.  n_cols a multiple of 8, k_dim a multiple of 16 and at most 131056.  Up to eight
  * rows a dp4a kernel without a workspace (the size is 0), above the stream-K tcgen05 GEMM of
  * fdllm_gemm_bf16 with kind::i8 instructions; workspace as there, its first 4096 bytes (the flags) zero
@@ -259,7 +259,8 @@ int fdllm_attn_cache(const void* q, void* o, const void* k_cache, const void* v_
  *   q, k, v   bf16, row strides ldq / ldk / ldv elements (e.g. parts of one stacked projection), n_heads /
  *             n_kv_heads / n_kv_heads heads of 128
  *   rope_sin, rope_cos  fp32 [>= seqlen_max, 128] by position, or both NULL: no rotation
- *   q_out     bf16 [n_rows, n_heads * 128]: the rotated Q (NULL: q is not read); may be q itself
+ *   q_out     bf16 [n_rows, n_heads * 128]: the rotated Q (NULL: q is not read); may be q itself, and
+ *             overlaps nothing else
  *   kv_bits   16: k_cache, v_cache bf16 [n_pages * 64, n_kv_heads * 128];  4: the 4-bit cache above
  * Rotated K and V go to their token's line; everything else in the caches stays as it was.  A slot or
  * page out of range is reported as FDLLM_ERR_INDEX and its row left out entirely.  Slots of one call must

@@ -145,3 +145,63 @@ def test_attention_beside_pages_of_zero_values(rows, zeros, small):
     caches = [caches[0], qr.int4_pack(v)]
     out, sc = tq._run_attention(q, caches, pt, mb, tb, B, L, h, h)
     tq._check_attention(q, caches, pt, spans, B, L, h, h, out, sc)
+
+
+def test_products_refuse_outputs_that_overlap():
+    """Views of one buffer: beside one another they pass, shifted they are
+    refused; the residual itself is an output."""
+    from flash_dllm_b200 import ops
+    g = tq._gen(1)
+    rows, n, k = 20, 64, 128
+    a, w = tq._int8(g, rows, k), tq._int8(g, n, k)
+    sa, sw = torch.rand(rows, device="cuda", generator=g), torch.rand(n, device="cuda", generator=g) * 1e-2
+    buf = tq._randn(g, rows + 4, 4 * n).bfloat16()
+    res = buf[:rows, n:2 * n]
+    before = buf.clone()
+    want = ops.linear_int8(a, sa, w, sw, residual=res)
+    for out in (buf[:rows, :n], buf[:rows, 2 * n:3 * n], buf[4:, 3 * n:], res):
+        got = ops.linear_int8(a, sa, w, sw, residual=res, out=out)
+        assert torch.equal(got, want) and got.data_ptr() == out.data_ptr()
+        buf.copy_(before)
+    for out in (buf[:rows, n - 8:2 * n - 8], buf[:rows, 2 * n - 8:3 * n - 8], buf[1:rows + 1, n:2 * n],
+                buf.view(-1)[n:n + rows * n].view(rows, n)):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.linear_int8(a, sa, w, sw, residual=res, out=out)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.linear_int8(a, sa, w, sw, out=a.view(torch.bfloat16)[:, :n])
+    assert torch.equal(buf, before)
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+def test_append_refuses_what_overlaps(bits):
+    from flash_dllm_b200 import ops
+    h, rows = 2, 3
+    qkv = torch.randn(rows + 1, 3 * h * 128, device="cuda").bfloat16()
+    q, k, v = (qkv[:rows, i * 256:(i + 1) * 256] for i in range(3))
+    slots = torch.arange(rows, device="cuda")
+    sin, cos = qr.rope_tables(64, "cuda")
+
+    def caches():
+        return ops.int4_cache(1, h) if bits == 4 else [torch.zeros(64, 256, device="cuda", dtype=torch.bfloat16) for _ in "kv"]
+
+    def run(kc, vc, q=q, k=k, v=v, **kw):
+        return ops.rope_append(q, k, v, slots, sin, cos, kc, vc, h, h, 64, **kw)
+
+    kc, vc = caches()
+    want = run(kc, vc)
+    flat = qkv.view(-1)
+    for bad in (flat[:rows * 256].view(rows, 256), flat[128:128 + rows * 256].view(rows, 256), k[:1].expand(rows, 256)):
+        with pytest.raises(ValueError):
+            run(kc, vc, q_out=bad)
+    own = q.contiguous()
+    with pytest.raises(ValueError, match="overlap"):
+        ops.rope_append(own[:2], k[:2], v[:2], slots[:2], sin, cos, kc, vc, h, h, 64, q_out=own[1:])
+    with pytest.raises(ValueError, match="overlap"):
+        run(kc, kc)
+    if bits == 16:
+        with pytest.raises(ValueError, match="overlap"):
+            run(kc, vc, k=kc[:rows])
+    # a lone row between the others of a buffer, and q itself, are fine
+    one = ops.rope_append(q[1:2], k[1:2], v[1:2], slots[1:2], sin, cos, kc, vc, h, h, 64, q_out=qkv[3:4, :256])
+    assert torch.equal(one, want[1:2])
+    assert torch.equal(run(kc, vc, q=own, q_out=own), want)
