@@ -148,12 +148,18 @@ int launch_quant(const void* x, int64_t ld, const void* w, float eps, void* code
   const auto* xb = static_cast<const __nv_bfloat16*>(x);
   const auto* wb = static_cast<const __nv_bfloat16*>(w);
   auto* c = static_cast<uint8_t*>(codes);
-  // four 16-byte loads a thread up to 4096 values, eight above
+  // Four 16-byte loads a thread up to 4096 values, eight of twice the threads
+  // above.  Behind a norm the threads are norm.cu's 128 up to its 8192 values:
+  // the squares are summed in its order, and the codes are those of its rows.
+  // (512 rows of 8192: 4.6 us, with 256 threads 7.1.)
   const cudaError_t e =
       dim <= 4096 ? launch_ex(quant_rows_kernel<128, 4, NORM>, dim3(rows), dim3(128), 0, stream, 1, pdl_enabled(), xb,
                               ld, wb, eps, c, scale, static_cast<int>(dim))
-                  : launch_ex(quant_rows_kernel<256, 8, NORM>, dim3(rows), dim3(256), 0, stream, 1, pdl_enabled(), xb,
-                              ld, wb, eps, c, scale, static_cast<int>(dim));
+      : NORM && dim <= 8192
+          ? launch_ex(quant_rows_kernel<128, 8, NORM>, dim3(rows), dim3(128), 0, stream, 1, pdl_enabled(), xb, ld, wb,
+                      eps, c, scale, static_cast<int>(dim))
+          : launch_ex(quant_rows_kernel<256, 8, NORM>, dim3(rows), dim3(256), 0, stream, 1, pdl_enabled(), xb, ld, wb,
+                      eps, c, scale, static_cast<int>(dim));
   return e == cudaSuccess && cudaPeekAtLastError() == cudaSuccess ? FDLLM_OK : FDLLM_ERR_CUDA;
 }
 

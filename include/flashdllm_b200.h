@@ -129,8 +129,8 @@ int fdllm_gemm_swiglu(const void* a, const void* w_gate_up, void* out, int32_t n
 int fdllm_quantize_int8(const void* x, int64_t ld, void* codes, float* scale, int32_t rows, int32_t dim,
                         cudaStream_t stream);
 
-/* fdllm_rmsnorm followed by fdllm_quantize_int8 in one pass (the same codes and scales); dim a multiple
- * of 8, at most 16384. */
+/* fdllm_rmsnorm followed by fdllm_quantize_int8 in one pass: the same codes and scales, bit for bit, up to
+ * the 8192 values of a row that fdllm_rmsnorm takes.  dim a multiple of 8, at most 16384. */
 int fdllm_rmsnorm_int8(const void* x, const void* weight, void* codes, float* scale, int32_t rows, int32_t dim,
                        float eps, cudaStream_t stream);
 
