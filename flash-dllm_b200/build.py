@@ -7,7 +7,8 @@ arch=compute_100a,code=sm_100a -lineinfo -O3``) into ``_build/`` at the repo
 root and linked into ``flash-dllm_b200/libflashdllm_b200.so`` next to this
 file.  ``csrc/torch_ops.cpp`` (the torch binding of the quantised operators)
 is compiled with g++ against the installed torch and linked to that library
-as ``_torch_ops.so``.  Objects are rebuilt when a source or header is newer.
+as ``_torch_ops.so``.  Objects are rebuilt when a source or header is newer,
+the binding also when another torch or Python or other flags built it.
 """
 from __future__ import annotations
 
@@ -27,6 +28,7 @@ BUILD = os.path.join(ROOT, "_build")
 LIB = os.path.join(PKG, "libflashdllm_b200.so")
 BINDING_SRC = os.path.join(CSRC, "torch_ops.cpp")
 BINDING = os.path.join(PKG, "_torch_ops.so")
+BINDING_STAMP = os.path.join(BUILD, "_torch_ops.stamp")  # what the binding was built with
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr", "-I", INCLUDE,
          "-I", CSRC]
@@ -57,6 +59,23 @@ def _binding_cmd() -> list:
             f"-L{PKG}", f"-l:{os.path.basename(LIB)}", "-Wl,-rpath,$ORIGIN"]
 
 
+def _binding_stamp(cmd: list) -> str:
+    import torch
+    return "\n".join([sys.version, torch.__version__, str(torch.version.git_version), *cmd])
+
+
+def _binding_stale(stamp: str, dep_t: float) -> bool:
+    """Whether the binding is missing, older than its source or a header, or
+    built for another torch (its C++ interface is not stable), Python or path."""
+    if not os.path.exists(BINDING) or os.path.getmtime(BINDING) < max(os.path.getmtime(BINDING_SRC), dep_t):
+        return True
+    try:
+        with open(BINDING_STAMP) as f:
+            return f.read() != stamp
+    except FileNotFoundError:
+        return True
+
+
 def build(verbose: bool = False, force: bool = False) -> str:
     nvcc = _nvcc()
     os.makedirs(BUILD, exist_ok=True)
@@ -81,8 +100,12 @@ def build(verbose: bool = False, force: bool = False) -> str:
         list(ex.map(run, jobs))
     if jobs or not os.path.exists(LIB) or any(os.path.getmtime(o) > os.path.getmtime(LIB) for o in objs):
         run([nvcc, *ARCH, "-shared", "-o", LIB, *objs, "-lcudart_static", "-lrt", "-ldl", "-lpthread"])
-    if force or not os.path.exists(BINDING) or os.path.getmtime(BINDING) < max(os.path.getmtime(BINDING_SRC), dep_t):
-        run(_binding_cmd())
+    cmd = _binding_cmd()
+    stamp = _binding_stamp(cmd)
+    if force or _binding_stale(stamp, dep_t):
+        run(cmd)
+        with open(BINDING_STAMP, "w") as f:
+            f.write(stamp)
     return LIB
 
 
