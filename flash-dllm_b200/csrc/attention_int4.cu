@@ -254,13 +254,14 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 // code - 8 of the pairs at bits 0 (even) or 4 (odd) of each half: 1024 + code
-// and 1024 + 16 code are fp16 values whose mantissas hold the code
+// and 1024 + 16 code are fp16 values whose mantissas hold the code (the widely
+// published way to turn small integers into floating-point numbers)
 __device__ __forceinline__ uint32_t i4_even_f16(uint32_t w) {
   uint32_t m, r;
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(m) : "r"(w), "n"(0x000f000f), "r"(0x64006400u));
@@ -390,7 +391,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) attn_int4_few_kernel(co
       for (int j = 0; j < 16; ++j) {
         const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&qf[j]));
         const float d = (j & 1) && !kScores ? down16 : down;
-        qf[j] = pack_half2(f.x * d, f.y * d);
+        qf[j] = pack_f16x2(f.x * d, f.y * d);
       }
     }
     // logits are kept divided by 2^(kLift + eq)
@@ -568,7 +569,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) attn_int4_few_kernel(co
             pb[e] = fmaf(x, low, pb[e]);
             w[e] = x * (st * static_cast<float>(1 << kFewRaise));
           }
-          bf[mt][hh] = transpose8x8(pack_half2(w[0], w[1]));
+          bf[mt][hh] = transpose8x8(pack_f16x2(w[0], w[1]));
         }
 #pragma unroll
       for (int e = 0; e < kE; ++e) l[e] = fmaf(lp[e], ln, l[e]);
@@ -880,10 +881,6 @@ __device__ __forceinline__ uint8_t* ext_chunk(uint8_t* base, int row, int chunk)
   return base + row * 32 + ((chunk ^ ((row >> 2) & 1)) << 4);
 }
 
-__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 __device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t r;
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));

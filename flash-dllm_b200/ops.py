@@ -218,13 +218,14 @@ INT4_BLOCK = PAGE * HEAD_DIM // 2 + PAGE * 4  # bytes of one page of one head: c
 
 def quantize_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """(codes int8, scale fp32 [rows]) of a bf16 [rows, dim]: scale = max|x| / 127
-    of the row, codes = round(x / scale) in [-127, 127].  ``x`` may be a
-    row-strided view.  A row with an infinity or NaN gets a NaN scale."""
+    of the row, codes = round(x * (127 / max|x|)) in [-127, 127] (half to even;
+    the factor rounded to fp32).  ``x`` may be a row-strided view.  A row with an infinity or NaN gets a NaN scale."""
     return _T.quantize_int8(x)
 
 
 def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float) -> Tuple[torch.Tensor, torch.Tensor]:
-    """``quantize_int8(rmsnorm(x, weight, eps))`` in one pass."""
+    """``quantize_int8(rmsnorm(x, weight, eps))`` in one pass (the same bits, for
+    the rows of up to 8192 that :func:`rmsnorm` takes; here up to 16384)."""
     return _T.rmsnorm_int8(x, weight, eps)
 
 
