@@ -38,3 +38,33 @@ def test_binding_is_rebuilt_for_another_torch(tmp_path, monkeypatch):
     assert build._binding_stale(build._binding_stamp(["g++", "-O3"]), 0)
     monkeypatch.setattr(torch, "__version__", "0.0.1")
     assert build._binding_stale(build._binding_stamp(["g++"]), 0)
+
+
+def test_bound_of_the_attention_sees_lost_bits_and_keys():
+    """Answers with P in fp16 are within the mean square that the attention is
+    tested with; with P in bf16, or without one key of 2176, they are not."""
+    import torch
+
+    import quantized_reference as qr
+    import test_quantized_attention_gpu as ta
+    g = torch.Generator().manual_seed(0)
+    k_end, rows, h = 2176, 4, 4
+    pt = torch.arange(k_end // 64).reshape(1, -1).int()
+    caches = [qr.int4_pack(torch.randn(k_end // 64, h, 64, 128, generator=g).bfloat16()) for _ in range(2)]
+    q = torch.randn(rows, h * 128, generator=g).bfloat16()
+    ref, ms = ta._mean_square(q, caches, pt, [(0, k_end, range(rows), range(0))], h, h, 128 ** -0.5)
+    k, v = ((c * s[..., None] + low[..., None]).transpose(0, 1).flatten(1, 2) for c, s, low in map(qr.int4_unpack, caches))
+    x = q.double().reshape(rows, h, 128).transpose(0, 1)
+    logits = x @ k.transpose(1, 2) * 128 ** -0.5
+
+    def ratio(held, without=None):
+        z = logits.clone()
+        if without is not None:
+            z[..., without] = -float("inf")
+        p = (z - z.amax(-1, keepdim=True)).exp()
+        o = (p.to(held).double() @ v / p.sum(-1, keepdim=True)).transpose(0, 1).flatten(1).bfloat16().double()
+        return float((o - ref).square().sum() / ms.sum() / (1 + 5 * (0.8 / ref.numel()) ** 0.5))
+
+    assert ratio(torch.float16) <= 1
+    assert ratio(torch.bfloat16) > 1.3
+    assert ratio(torch.float16, without=k_end - 1) > 10
