@@ -1604,13 +1604,23 @@ struct A4Plan {
 };
 
 // Rows x heads per kv head up to which the few-rows kernel runs.  Its time grows
-// with the chunks of eight, the other's not up to 128 (us, few | many):
-//   rows x heads                    16           32            64
-//   8 x 2176, 32 kv heads      42.6 | 75.9   73.7 | 76.9   142.8 | 77.7
-//   4 x 8192, 8 kv heads       25.0 | 43.5   38.6 | 43.6    63.0 | 44.7
-//   16 x 1024, 8 kv heads      14.5 | 23.1   26.2 | 23.5    43.9 | 23.8
-//   1 x 32768, 8 kv heads      26.8 | 56.3   39.2 | 56.9    66.1 | 58.1
-constexpr int kFewMaxRows = 32;
+// with the chunks of eight, and with scores each adds its own sums to every key;
+// the other's hardly grows up to 128 (us, few | many; a row is sequences x keys):
+//   without scores: rows x heads     16            24            32
+//   8 x 2176, 32 kv heads      41.9 | 67.5   60.5 | 67.8   71.0 | 68.0
+//   4 x 8192, 8 kv heads       23.3 | 38.5   28.8 | 38.6   36.9 | 38.6
+//   16 x 1024, 8 kv heads      14.1 | 20.2   19.7 | 20.3   24.5 | 20.3
+//   1 x 2176, 32 kv heads      16.8 | 20.7   21.3 | 20.9   21.5 | 20.7
+//   1 x 32768, 8 kv heads      36.6 | 48.6   46.8 | 49.0   63.2 | 48.8
+//   64 x 512, 8 kv heads       29.2 | 51.4   43.7 | 51.6   56.6 | 52.0
+//   with scores
+//   8 x 2176, 32 kv heads      57.6 | 73.9   83.8 | 74.7   99.0 | 75.2
+//   4 x 8192, 8 kv heads       33.1 | 43.1   40.6 | 43.3   51.0 | 43.6
+//   16 x 1024, 8 kv heads      19.4 | 23.3   28.5 | 23.8   33.8 | 24.1
+//   1 x 2176, 32 kv heads      22.8 | 24.0   30.1 | 24.3   30.1 | 24.1
+//   1 x 32768, 8 kv heads      57.9 | 58.8   71.6 | 60.2   93.6 | 60.2
+//   64 x 512, 8 kv heads       41.5 | 61.1   60.8 | 62.6   77.7 | 63.4
+constexpr int kFewMaxRows = 24, kFewMaxRowsScores = 16;
 
 // Query chunks and key splits of the few-rows kernel, from what the host knows:
 // the sequences, the rows of one, and the longest cache.  Two CTAs run per SM
@@ -1713,7 +1723,7 @@ A4Plan a4_plan(int32_t n_rows, int32_t max_items, int32_t n_seqs, int32_t n_head
                int32_t kv_splits, int32_t rows_hint, bool scores) {
   const int items = std::max(n_seqs, max_items - n_seqs);  // (the capacity: an item per 64 rows and one a sequence)
   const int seq_rows = rows_hint > 0 && rows_hint < n_rows ? rows_hint : n_rows;
-  if (static_cast<long long>(seq_rows) * (n_heads / n_kv) > kFewMaxRows)
+  if (static_cast<long long>(seq_rows) * (n_heads / n_kv) > (scores ? kFewMaxRowsScores : kFewMaxRows))
     return a4_plan_many(n_seqs, seq_rows, n_heads / n_kv, n_kv, seqlen_max, kv_splits, scores);
   const int rows = seq_rows < kA4ItemRows ? seq_rows : kA4ItemRows;
   return a4_plan_few(items, rows, n_heads / n_kv, n_kv, seqlen_max, kv_splits);

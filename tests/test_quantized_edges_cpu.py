@@ -68,3 +68,19 @@ def test_bound_of_the_attention_sees_lost_bits_and_keys():
     assert ratio(torch.float16) <= 1
     assert ratio(torch.bfloat16) > 1.3
     assert ratio(torch.float16, without=k_end - 1) > 10
+
+
+def test_rows_that_choose_the_attention_kernel(L):
+    """Up to 24 rows x heads of a kv head, 16 with scores, the kernel of few rows
+    (parts of eight rows a split), above the other (parts of 128)."""
+    def part(rows, group, scores):
+        n = ctypes.c_size_t(0)
+        cap = L.fdllm_attn_plan_capacity(rows, 1)
+        L.fdllm_attn_int4_workspace_bytes(rows, cap, 1, 8 * group, 8, 8192, 2, rows, scores, ctypes.byref(n))
+        return n.value // (2 * 8)  # two splits, eight kv heads
+
+    few, many = (8 * 128 + 16) * 4, (128 * 128 + 256) * 4
+    for rows, group, scores, chunks in ((24, 1, 0, 3), (3, 8, 0, 3), (16, 1, 1, 2), (2, 8, 1, 2)):
+        assert part(rows, group, scores) % (chunks * few) == 0 and part(rows, group, scores) < many
+    for rows, group, scores in ((25, 1, 0), (4, 8, 0), (17, 1, 1), (3, 8, 1)):
+        assert part(rows, group, scores) == many
