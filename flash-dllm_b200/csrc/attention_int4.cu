@@ -1182,7 +1182,7 @@ __global__ void __launch_bounds__(kMnThreads, 1) attn_int4_many_kernel(const A4P
         const bool need = mt > ref + kMnLazy;
         if (__any_sync(0xffffffffu, need || ev.y == 0.f)) {
           const float h = need ? a4_half(ref - mt) : 1.f, a = h * h;
-          if (t > 0) {
+          if (t > 0 && __any_sync(0xffffffffu, need)) {
             // O holds P V of the tiles before; each key quarter scales a quarter of its dims
             ok = ok && a4_wait(&ms.pv_done[(t - 1) % 3], ((t - 1) / 3) & 1, p.status);
             tc_fence_after();
