@@ -212,7 +212,7 @@ __device__ __forceinline__ void a4_convert_scores(const A4Params& p, int seq, in
 // partial results in split order, so the result does not depend on timing.
 //
 // Measured: 4 sequences of 65536 keys, 32 heads on 8 kv heads, one row each (285
-// MB): 57.7 us, 4.9 TB/s.  8 of 2176, 32 kv heads (76 MB): 22.4 us.  Some 920
+// MB): 57.4 us, 5.0 TB/s.  8 of 2176, 32 kv heads (76 MB): 19.6 us.  Some 920
 // instructions a page and warp, ALU 56 % busy, no unit more: what is left is
 // the latency of one page's chain (products, reductions, exponentials,
 // transposes, products), which sixteen warps an SM overlap only so far, and 4 us
@@ -772,9 +772,10 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) attn_int4_few_kernel(co
 // two tiles ahead of P V(t).  The first tiles are converted while the query
 // operand is laid out.  Key ranges are split over CTAs as in the other kernel.
 //
-// Measured: 2048 rows of one sequence of 2176, 32 heads: 141 us (512 CTAs of 17
+// Measured: 2048 rows of one sequence of 2176, 32 heads: 143 us (512 CTAs of 17
 // tiles in 3.5 waves), 0.3 of the fp16 rate; 96 rows of four of 8192, with
-// scores, 121.5 us (113.7 without); 64 of eight of 896, with scores, 46.5 us.  A tile takes about
+// scores, 118.5 us; 64 of eight of 896, with scores, 43.6 us (the bf16 cache's
+// kernel: 28.3).  A tile takes about
 // 2900 clocks.  The tensor cores need 1160 of them (17 instructions), and wait;
 // a softmax warp needs all: some 160 instructions, each issued about 18 clocks
 // after the last among 8 warps a scheduler, the four of a row quarter in step (a

@@ -504,7 +504,7 @@ __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepc
 
 // ------------------------------------------------------------------ misc ----
 // The PTX ex2.approx.ftz.f32 instruction (2^x; -inf -> +0, tiny results flush
-// to zero), as flash-attention softmax kernels use it.
+// to zero), whose error is far below a probability's rounding to 16 bits.
 __device__ __forceinline__ float ex2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -29,7 +29,9 @@ environment variable ``FDLLM_OWN_GEMMS`` (a comma list of ``attn_out``,
 ``mlp``, ``ff_out``, ``lm_head``, ``all`` or ``none``) forces the choice for
 comparisons (``lm_head``: the model's LM head, in ``model.py``).
 
-Two options, each on its own or together:
+Two options, each on its own or together (with either, Q and K are rounded to
+bf16 before the rotation as well as after it, where the QKV kernel rotates its
+fp32 sums):
 - 8-bit projections (``quantize_block_int8``): QKV, ``attn_out``, the MLP and
   ``ff_out`` as int8 products with a scale per token and per output channel,
   the tokens quantised behind the norms.  The verify forward, whose task is to
@@ -37,6 +39,7 @@ Two options, each on its own or together:
 - a 4-bit cache (``k_cache`` / ``v_cache`` from ``ops.int4_cache``): Q and K are
   rotated and K and V quantised on the way into the pages, attention reads the
   4-bit pages, and the verify attention the keys and values they stand for.
+  (With bf16 weights its Q, K and V are three library products.)
   ``lengths[10]`` (None in the reference) may hold the most rows that a sequence
   of the forward has, by which that attention divides its work; without it the
   mean is taken, which is right and, where one sequence has many more rows than
