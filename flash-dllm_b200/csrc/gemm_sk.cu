@@ -592,7 +592,10 @@ __global__ void __launch_bounds__(kGThreads, 1)
   constexpr uint32_t kTx = static_cast<uint32_t>(C::kStageBytes);
   // B (weights: never written by the kernel before) of the stages that need
   // no free slot, requested before the programmatic-launch wait so its
-  // latency overlaps the tail of the kernel before; A comes from that kernel
+  // latency overlaps the tail of the kernel before; A comes from that kernel.
+  // Not with I8: there either operand may be codes that the kernel before
+  // makes (a product of activations), and what that one wrote is only sure to
+  // be seen behind the wait.
   auto load_b = [&](int n_tile, int kb, int s) {
     int b_row = 0;
     const CUtensorMap* map_b = g_b_coord<EPI>(p, n_tile, BN, 0, BN, &map_b0, &map_b1, &map_b2, b_row);
@@ -606,7 +609,7 @@ __global__ void __launch_bounds__(kGThreads, 1)
     }
   };
   uint32_t n_pre = 0;
-  if (warp == 0 && lane == 0) {
+  if (!I8 && warp == 0 && lane == 0) {
     GIter it{lo, hi, p.sk_tiles + idx};
     GSeg sg;
     while (n_pre < static_cast<uint32_t>(C::kStages) && g_step<false>(it, p, per_group, sg))
@@ -861,7 +864,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   // B (weights) of the stages that need no free slot, requested before the
-  // programmatic-launch wait (see the single-CTA kernel); A after it
+  // programmatic-launch wait (see the single-CTA kernel; not with I8); A after it
   auto load_b = [&](int n_tile, int kb, int s) {
     int b_row = 0;
     const CUtensorMap* map_b =
@@ -873,7 +876,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGThreads, 1)
                        bar);
   };
   uint32_t n_pre = 0;
-  if (warp == 0 && lane == 0) {
+  if (!I8 && warp == 0 && lane == 0) {
     GIter it{lo, hi, p.sk_tiles + idx};
     GSeg sg;
     while (n_pre < static_cast<uint32_t>(C::kStages) && g_step<WAVES>(it, p, per_group, sg))

@@ -77,11 +77,10 @@ __global__ void __launch_bounds__(kGvThreads, kR <= 2 ? 5 : kR == 4 ? 4 : 3) gem
   const int4 zero = make_int4(0, 0, 0, 0);
   int i = threadIdx.x;
   int4 b[kGvCols];
-  // the first weights are requested before the kernel ahead is waited for
+  pdl_wait();  // (the weights too may be codes that the kernel ahead makes)
+  pdl_launch_dependents();
 #pragma unroll
   for (int c = 0; c < kGvCols; ++c) b[c] = i < vecs ? load_weights(w[c] + i) : zero;
-  pdl_wait();
-  pdl_launch_dependents();
   while (i - lane < vecs) {  // uniform over the warp
     const int next = i + kGvThreads;
 #pragma unroll

@@ -74,9 +74,7 @@ __global__ void __launch_bounds__(THREADS) quant_rows_kernel(const __nv_bfloat16
   __shared__ float red_f[THREADS / 32];
   const int nvec = dim / 8;
   pdl_wait();
-  // (No early start for the next kernel: the integer product requests its
-  // weights before it waits for the kernel ahead of it, and these codes may be
-  // those weights.)
+  pdl_launch_dependents();
   const uint4* xr = reinterpret_cast<const uint4*>(x + static_cast<int64_t>(blockIdx.x) * ld);
   uint2* out = reinterpret_cast<uint2*>(codes + static_cast<int64_t>(blockIdx.x) * dim);
   uint4 v[VEC];
