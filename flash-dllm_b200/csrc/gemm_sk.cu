@@ -1123,6 +1123,8 @@ int g2_max_pairs_for(int epi, int ksub) {
 //     of about three (55x296x11968, 94 k-blocks: 13.9 with 6 a tile, 16.0 with 12,
 //     19.5 with 2; 250x288x5168, 41: 13.3 with 4, 15.8 with 8, 19.4 with 1;
 //     64x1024x1024, 8: 7.1 with 1, 9.0 with 2).
+// (Figures from back-to-back products whose weights were still requested ahead
+// of the wait; behind it, either side of each takes about half a us more.)
 GemmPlan plan_gemm(int epi, int32_t n_rows, int32_t n_cols, int32_t k_dim, int32_t d_model, bool i8 = false) {
   GemmPlan pl{};
   const GemmOverride& ov = gemm_override();

@@ -17,9 +17,9 @@
 // order changes nothing.
 //
 // us at 1, 2, 4, 8 rows, against the tensor-core kernel at 9 rows:
-//   4096 x 4096    4.9  4.7   4.9   6.6   (12.4)
-//   12288 x 4096  10.1  9.5  12.3  16.9   (18.3)
-//   24576 x 4096  17.3 16.6  21.5  31.2   (28.6)   6.1 TB/s at 2 rows
+//   4096 x 4096    4.5  4.6   5.8   7.2   (11.2)
+//   12288 x 4096   9.5  9.7  12.1  17.0   (18.4)
+//   24576 x 4096  17.1 17.1  21.9  31.2   (29.6)   5.9 TB/s at 2 rows
 #include "common.cuh"
 #include "internal.h"
 

@@ -76,7 +76,7 @@ size_t qkv_sk_ws_bytes(int32_t n_rows, int32_t d_model);
 // int8 products of a few rows (gemv_int8.cu); n: output columns.  Up to four
 // rows it is ahead of the tensor cores at every size but the largest (126464 x
 // 4096 at four rows: 107 us against 101); up to eight while the weights are few
-// (50 M: 16.9 us against 18.3; 100 M: 31.2 against 28.6).
+// (50 M: 17.0 us against 18.4; 100 M: 31.2 against 28.8).
 inline bool gemv_int8_rows(int32_t rows, int64_t weights) {
   return rows <= 4 || (rows <= 8 && weights <= (int64_t(1) << 26));
 }
