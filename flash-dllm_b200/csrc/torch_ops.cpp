@@ -12,6 +12,7 @@
 // Every call runs on the device of its tensors, on torch's current stream
 // there.
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -86,10 +87,16 @@ class Workspaces {
     *size = static_cast<size_t>(buf->numel());
     return buf->data_ptr();
   }
-  // after a device error left flags or counters set
+  // After a device error left flags or counters set: zeros, once nothing that
+  // runs on any stream uses them, and before anything else does.
   void rezero() {
     std::lock_guard<std::mutex> lock(mu_);
-    for (auto& kv : eager_) kv.second.zero_();
+    for (auto& kv : eager_) {
+      const c10::cuda::CUDAGuard guard(kv.second.device());
+      C10_CUDA_CHECK(cudaDeviceSynchronize());
+      kv.second.zero_();
+      C10_CUDA_CHECK(cudaDeviceSynchronize());
+    }
   }
   void clear() {
     std::lock_guard<std::mutex> lock(mu_);

@@ -53,9 +53,12 @@ class Workspace:
     @classmethod
     def rezero(cls) -> None:
         """Zero every live buffer in place (after a device error left
-        counters or flags set); addresses are kept."""
+        counters or flags set); addresses are kept.  Work of any stream that
+        still uses them is waited for first."""
         for buf in cls._bufs.values():
+            torch.cuda.synchronize(buf.device)
             buf.zero_()
+            torch.cuda.synchronize(buf.device)
         if vars(_T):
             _T.workspace_rezero()
 
