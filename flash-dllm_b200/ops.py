@@ -262,7 +262,7 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.
 
     ``q`` / ``k`` / ``v`` bf16 [rows, heads * 128] may be row-strided parts of one
     stacked projection.  ``slots`` int64 [rows]: sequence * seqlen_max +
-    position, all distinct.  ``sin`` / ``cos`` fp32 [>= seqlen_max, 128] by
+    position, all distinct (the line of one named twice may hold a mix of both rows).  ``sin`` / ``cos`` fp32 [>= seqlen_max, 128] by
     position; both None when q and k are rotated already (q is then returned
     as it is, unless ``q_out`` is given).  The caches are bf16 [pages * 64,
     n_kv_heads * 128] or 4-bit (:func:`int4_cache`); ``page_table`` int32 [batch,

@@ -264,7 +264,8 @@ int fdllm_attn_cache(const void* q, void* o, const void* k_cache, const void* v_
  *   kv_bits   16: k_cache, v_cache bf16 [n_pages * 64, n_kv_heads * 128];  4: the 4-bit cache above
  * Rotated K and V go to their token's line; everything else in the caches stays as it was.  A slot or
  * page out of range is reported as FDLLM_ERR_INDEX and its row left out entirely.  Slots of one call must
- * be distinct (of two rows with the same slot, either may be kept, value by value).  batch and
+ * be distinct: of two rows with the same slot either may be kept, in pieces (bf16: eight values; 4 bits: a
+ * group's words and its step and low, which then need not belong together).  batch and
  * pages_per_seq are page_table's sizes.  ref llada/flash_cache_triton.py:78-100 (the rotation and the
  * cache store, into contiguous bf16 regions). */
 int fdllm_rope_append(const void* q, const void* k, const void* v, int64_t ldq, int64_t ldk, int64_t ldv,
