@@ -40,12 +40,12 @@ fp32 sums):
   rotated and K and V quantised on the way into the pages, attention reads the
   4-bit pages, and the verify attention the keys and values they stand for.
   (With bf16 weights its Q, K and V are three library products.)
-
-Either option appends to pages of 64 tokens: ``max_length`` is a multiple of 64.
   ``lengths[10]`` (None in the reference) may hold the most rows that a sequence
   of the forward has, by which that attention divides its work; without it the
   mean is taken, which is right and, where one sequence has many more rows than
   the others, slower (1 x 2000 and 7 x 64 rows: 246 against 202 us).
+
+Either option appends to pages of 64 tokens: ``max_length`` is a multiple of 64.
 """
 from __future__ import annotations
 
