@@ -1606,22 +1606,29 @@ struct A4Plan {
 
 // Rows x heads per kv head up to which the few-rows kernel runs.  Its time grows
 // with the chunks of eight, and with scores each adds its own sums to every key;
-// the other's hardly grows up to 128 (us, few | many; a row is sequences x keys):
-//   without scores: rows x heads     16            24            32
-//   8 x 2176, 32 kv heads      41.9 | 67.5   60.5 | 67.8   71.0 | 68.0
-//   4 x 8192, 8 kv heads       23.3 | 38.5   28.8 | 38.6   36.9 | 38.6
-//   16 x 1024, 8 kv heads      14.1 | 20.2   19.7 | 20.3   24.5 | 20.3
-//   1 x 2176, 32 kv heads      16.8 | 20.7   21.3 | 20.9   21.5 | 20.7
-//   1 x 32768, 8 kv heads      36.6 | 48.6   46.8 | 49.0   63.2 | 48.8
-//   64 x 512, 8 kv heads       29.2 | 51.4   43.7 | 51.6   56.6 | 52.0
-//   with scores
-//   8 x 2176, 32 kv heads      57.6 | 73.9   83.8 | 74.7   99.0 | 75.2
-//   4 x 8192, 8 kv heads       33.1 | 43.1   40.6 | 43.3   51.0 | 43.6
-//   16 x 1024, 8 kv heads      19.4 | 23.3   28.5 | 23.8   33.8 | 24.1
-//   1 x 2176, 32 kv heads      22.8 | 24.0   30.1 | 24.3   30.1 | 24.1
-//   1 x 32768, 8 kv heads      57.9 | 58.8   71.6 | 60.2   93.6 | 60.2
-//   64 x 512, 8 kv heads       41.5 | 61.1   60.8 | 62.6   77.7 | 63.4
-constexpr int kFewMaxRows = 24, kFewMaxRowsScores = 16;
+// the other's hardly grows up to 128.  Where the sequences' kv heads leave half
+// of the SMs without a CTA of it, the other kernel has its fixed costs and few
+// CTAs to hide them, and the limit is eight rows higher (us, few | many):
+//                                  16            24            32            48
+//   8 x 2176, 32 kv heads    42.5 | 67.6   61.6 | 67.8   72.2 | 68.3  110.6 | 68.4
+//   16 x 1024, 8 kv heads    13.8 | 20.2   19.8 | 20.3   24.7 | 20.2   35.5 | 20.4
+//   64 x 512, 8 kv heads     29.5 | 51.1   44.1 | 51.1   56.9 | 51.1   86.0 | 51.7
+//   8 x 896, 8 kv heads      12.5 | 17.7   12.9 | 17.9   13.4 | 17.7   19.9 | 17.9
+//   4 x 8192, 8 kv heads     23.3 | 38.3   29.3 | 38.6   37.5 | 38.4   53.8 | 38.5
+//   1 x 32768, 8 kv heads    25.0 | 48.8   32.2 | 49.0   38.3 | 48.8   48.8 | 49.0
+//   1 x 2176, 32 kv heads    14.2 | 20.7   15.2 | 20.9   17.6 | 20.7   22.3 | 21.0
+//  with scores
+//   8 x 2176, 32 kv heads    58.5 | 73.8   85.2 | 74.5  100.5 | 75.2
+//   16 x 1024, 8 kv heads    19.3 | 23.4   28.5 | 23.7   34.1 | 24.0
+//   64 x 512, 8 kv heads     41.5 | 61.5   60.7 | 62.3   78.2 | 63.5
+//   8 x 896, 8 kv heads      17.9 | 20.4   18.2 | 20.7   18.7 | 21.1   27.9 | 21.7
+//   4 x 8192, 8 kv heads     33.3 | 43.1   41.0 | 43.4   51.8 | 43.8
+//   1 x 32768, 8 kv heads    42.0 | 59.2   51.4 | 60.1   59.6 | 60.2   73.5 | 60.9
+//   1 x 2176, 32 kv heads    19.1 | 23.7   20.3 | 23.9   24.1 | 24.1   30.7 | 24.9
+int few_max_rows(int n_seqs, int n_kv, bool scores) {
+  const bool spare = static_cast<long long>(n_seqs) * n_kv <= sm_count() / 2;
+  return (scores ? 16 : 24) + (spare ? 8 : 0);
+}
 
 // Query chunks and key splits of the few-rows kernel, from what the host knows:
 // the sequences, the rows of one, and the longest cache.  Two CTAs run per SM
@@ -1724,7 +1731,7 @@ A4Plan a4_plan(int32_t n_rows, int32_t max_items, int32_t n_seqs, int32_t n_head
                int32_t kv_splits, int32_t rows_hint, bool scores) {
   const int items = std::max(n_seqs, max_items - n_seqs);  // (the capacity: an item per 64 rows and one a sequence)
   const int seq_rows = rows_hint > 0 && rows_hint < n_rows ? rows_hint : n_rows;
-  if (static_cast<long long>(seq_rows) * (n_heads / n_kv) > (scores ? kFewMaxRowsScores : kFewMaxRows))
+  if (static_cast<long long>(seq_rows) * (n_heads / n_kv) > few_max_rows(n_seqs, n_kv, scores))
     return a4_plan_many(n_seqs, seq_rows, n_heads / n_kv, n_kv, seqlen_max, kv_splits, scores);
   const int rows = seq_rows < kA4ItemRows ? seq_rows : kA4ItemRows;
   return a4_plan_few(items, rows, n_heads / n_kv, n_kv, seqlen_max, kv_splits);

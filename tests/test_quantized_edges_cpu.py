@@ -72,15 +72,16 @@ def test_bound_of_the_attention_sees_lost_bits_and_keys():
 
 def test_rows_that_choose_the_attention_kernel(L):
     """Up to 24 rows x heads of a kv head, 16 with scores, the kernel of few rows
-    (parts of eight rows a split), above the other (parts of 128)."""
-    def part(rows, group, scores):
+    (parts of eight rows a split), above the other (parts of 128); eight more
+    where a few sequences' kv heads leave most SMs to split keys over."""
+    def kernel(seqs, rows, group, scores):
         n = ctypes.c_size_t(0)
-        cap = L.fdllm_attn_plan_capacity(rows, 1)
-        L.fdllm_attn_int4_workspace_bytes(rows, cap, 1, 8 * group, 8, 8192, 2, rows, scores, ctypes.byref(n))
-        return n.value // (2 * 8)  # two splits, eight kv heads
+        cap = L.fdllm_attn_plan_capacity(seqs * rows, seqs)
+        L.fdllm_attn_int4_workspace_bytes(seqs * rows, cap, seqs, 8 * group, 8, 8192, 2, rows, scores, ctypes.byref(n))
+        chunks = -(-rows * group // 8)
+        return {cap * 2 * 8 * chunks * (8 * 128 + 16) * 4: "few", seqs * 2 * 8 * (128 * 128 + 256) * 4: "many"}[n.value]
 
-    few, many = (8 * 128 + 16) * 4, (128 * 128 + 256) * 4
-    for rows, group, scores, chunks in ((24, 1, 0, 3), (3, 8, 0, 3), (16, 1, 1, 2), (2, 8, 1, 2)):
-        assert part(rows, group, scores) % (chunks * few) == 0 and part(rows, group, scores) < many
-    for rows, group, scores in ((25, 1, 0), (4, 8, 0), (17, 1, 1), (3, 8, 1)):
-        assert part(rows, group, scores) == many
+    for seqs, extra in ((64, 0), (1, 8)):
+        for scores, limit in ((0, 24 + extra), (1, 16 + extra)):
+            assert kernel(seqs, limit, 1, scores) == "few" and kernel(seqs, limit // 8, 8, scores) == "few"
+            assert kernel(seqs, limit + 1, 1, scores) == "many" and kernel(seqs, limit // 8 + 1, 8, scores) == "many"
