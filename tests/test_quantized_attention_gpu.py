@@ -128,3 +128,27 @@ def test_error_is_that_of_16_bit_operands(seqs, h, hk, length, sharp):
         err = (out.double() - ref)[have].square()
         n = err.numel()
         assert err.sum() <= ms[have].sum() * (1 + 5 * (0.8 / n) ** 0.5), (err.sum() / ms[have].sum(), n)
+
+
+@pytest.mark.parametrize("seqs,h,hk", [
+    ([(3, 16, 0), (2, 16, 0), (5, 4, 0)], 4, 4), ([(9, 8, 0), (17, 16, 0), (33, 2, 0)], 4, 4), ([(3, 1, 0)] * 40, 8, 2),
+    ([(6, 2, 0), (7, 2, 0), (63, 2, 0)], 14, 2), ([(200, 1, 0)] * 16, 8, 8),
+])
+@pytest.mark.parametrize("sharp", [0.01, 0.3, 1.0])
+def test_error_of_few_keys_and_rows(seqs, h, hk, sharp):
+    """The same bound where a few keys' roundings add up: they count by a value's
+    distance from its group's middle, not from its lowest."""
+    total, allowed, n = 0.0, 0.0, 0
+    for seed in range(8):
+        length = max(s[0] for s in seqs)
+        q, caches, pt, spans, mb, tb, B, L = tq._attention_case(50 + seed, seqs, h, hk, length)
+        q = (q * sharp).bfloat16()
+        v = tq._randn(tq._gen(seed), caches[1].shape[0], hk, 64, 128)
+        caches = [caches[0], qr.int4_pack(v.bfloat16())]  # (without a mean: sums cancel)
+        out, _ = tq._run_attention(q, caches, pt, mb, tb, B, L, h, hk, scores=False)
+        ref, ms = _mean_square(q, caches, pt, spans, h, hk, 128 ** -0.5)
+        have = ~torch.isnan(ref)
+        total += (out.double() - ref)[have].square().sum().item()
+        allowed += ms[have].sum().item()
+        n += int(have.sum())
+    assert total <= allowed * (1 + 5 * (0.8 / n) ** 0.5), (total / allowed, n)
