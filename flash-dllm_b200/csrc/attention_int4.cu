@@ -217,7 +217,7 @@ __device__ __forceinline__ void a4_convert_scores(const A4Params& p, int seq, in
 // partial results in split order, so the result does not depend on timing.
 //
 // Measured: 4 sequences of 65536 keys, 32 heads on 8 kv heads, one row each (285
-// MB): 57.4 us, 5.0 TB/s.  8 of 2176, 32 kv heads (76 MB): 19.6 us.  Some 920
+// MB): 58.1 us, 4.9 TB/s.  8 of 2176, 32 kv heads (76 MB): 19.7 us.  Some 920
 // instructions a page and warp, ALU 56 % busy, no unit more: what is left is
 // the latency of one page's chain (products, reductions, exponentials,
 // transposes, products), which sixteen warps an SM overlap only so far, and 4 us
@@ -1618,7 +1618,7 @@ struct A4Plan {
 // with the chunks of eight, and with scores each adds its own sums to every key;
 // the other's hardly grows up to 128.  Where the sequences' kv heads leave half
 // of the SMs without a CTA of it, the other kernel has its fixed costs and few
-// CTAs to hide them, and the limit is eight rows higher (us, few | many):
+// CTAs to hide them, and the limit is higher (us, few | many):
 //                                  16            24            32            48
 //   8 x 2176, 32 kv heads    42.5 | 67.6   61.6 | 67.8   72.2 | 68.3  110.6 | 68.4
 //   16 x 1024, 8 kv heads    13.8 | 20.2   19.8 | 20.3   24.7 | 20.2   35.5 | 20.4
@@ -1635,9 +1635,10 @@ struct A4Plan {
 //   4 x 8192, 8 kv heads     33.3 | 43.1   41.0 | 43.4   51.8 | 43.8
 //   1 x 32768, 8 kv heads    42.0 | 59.2   51.4 | 60.1   59.6 | 60.2   73.5 | 60.9
 //   1 x 2176, 32 kv heads    19.1 | 23.7   20.3 | 23.9   24.1 | 24.1   30.7 | 24.9
+//   1 x 896, 8 kv heads      13.1 | 19.4   13.2 | 19.2   13.2 | 19.5   14.1 | 19.9
 int few_max_rows(int n_seqs, int n_kv, bool scores) {
   const bool spare = static_cast<long long>(n_seqs) * n_kv <= sm_count() / 2;
-  return (scores ? 16 : 24) + (spare ? 8 : 0);
+  return spare ? 32 : scores ? 16 : 24;
 }
 
 // Query chunks and key splits of the few-rows kernel, from what the host knows:

@@ -72,8 +72,8 @@ def test_bound_of_the_attention_sees_lost_bits_and_keys():
 
 def test_rows_that_choose_the_attention_kernel(L):
     """Up to 24 rows x heads of a kv head, 16 with scores, the kernel of few rows
-    (parts of eight rows a split), above the other (parts of 128); eight more
-    where a few sequences' kv heads leave most SMs to split keys over."""
+    (parts of eight rows a split), above the other (parts of 128); up to 32 where
+    a few sequences' kv heads leave most SMs to split keys over."""
     def kernel(seqs, rows, group, scores):
         n = ctypes.c_size_t(0)
         cap = L.fdllm_attn_plan_capacity(seqs * rows, seqs)
@@ -81,7 +81,6 @@ def test_rows_that_choose_the_attention_kernel(L):
         chunks = -(-rows * group // 8)
         return {cap * 2 * 8 * chunks * (8 * 128 + 16) * 4: "few", seqs * 2 * 8 * (128 * 128 + 256) * 4: "many"}[n.value]
 
-    for seqs, extra in ((64, 0), (1, 8)):
-        for scores, limit in ((0, 24 + extra), (1, 16 + extra)):
-            assert kernel(seqs, limit, 1, scores) == "few" and kernel(seqs, limit // 8, 8, scores) == "few"
-            assert kernel(seqs, limit + 1, 1, scores) == "many" and kernel(seqs, limit // 8 + 1, 8, scores) == "many"
+    for seqs, scores, limit in ((64, 0, 24), (64, 1, 16), (1, 0, 32), (1, 1, 32)):
+        assert kernel(seqs, limit, 1, scores) == "few" and kernel(seqs, limit // 8, 8, scores) == "few"
+        assert kernel(seqs, limit + 1, 1, scores) == "many" and kernel(seqs, limit // 8 + 1, 8, scores) == "many"
