@@ -241,7 +241,8 @@ def flash_fused_elastic_cache(self, x: torch.Tensor, block_idx, positions, lengt
             if four_bits:
                 ops.attn_cache_int4(q, att, self.k_cache, self.v_cache, plan, cap, scores, 1.0 / (block_m * n_heads),
                                     n_heads, n_heads, max_length, softmax_scale,
-                                    rows_hint=max_rows if max_rows else -(-n_rows // max(1, len(active_batch))))
+                                    rows_hint=max_rows if isinstance(max_rows, int) and max_rows > 0
+                                    else -(-n_rows // max(1, len(active_batch))))
             else:
                 ops.attn_cache(q, att, self.k_cache, self.v_cache, plan, cap, scores, 1.0 / (block_m * n_heads),
                                n_heads, max_length, softmax_scale, items_hint=-(-n_rows // 64))
