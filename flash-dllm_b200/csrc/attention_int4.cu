@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) attn_int4_few_kernel(co
     for (int e = 0; e < kE; ++e) {
       qsum[e] = __shfl_sync(0xffffffffu, qsn, 8 * t + 4 * e);
       up[e] = pow2i(kLift + __shfl_sync(0xffffffffu, eq, 8 * t + 4 * e));
-      mul[e] = up[e] * p.scale_log2;
+      mul[e] = fmaxf(up[e] * p.scale_log2, 0x1p-126f);  // (not 0: a key past the end is -infinity times this)
     }
     // this lane's rows of the chunk; masked ones count into the scores
     bool is_m[kE];
@@ -785,12 +785,12 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) attn_int4_few_kernel(co
 // Measured: 2048 rows of one sequence of 2176, 32 heads: 143 us (512 CTAs of 17
 // tiles in 3.5 waves), 0.3 of the fp16 rate; 96 rows of four of 8192, with
 // scores, 118.5 us; 64 of eight of 896, with scores, 43.6 us (the bf16 cache's
-// kernel: 28.3).  A tile takes about
-// 2900 clocks.  The tensor cores need 1160 of them (17 instructions), and wait;
-// a softmax warp needs all: some 160 instructions, each issued about 18 clocks
-// after the last among 8 warps a scheduler, the four of a row quarter in step (a
-// scheduler owns a quarter of tensor memory's lanes), so the exponentials'
-// 1024 clocks and the rest do not overlap.  What did not help: the next tile's
+// kernel: 28.3).  A tile takes about 2900 clocks.  The tensor cores need 1160 of
+// them (17 instructions), and wait; a softmax warp needs all: some 160
+// instructions, each issued about 18 clocks after the last among 8 warps a
+// scheduler, the four of a row quarter in step (a scheduler owns a quarter of
+// tensor memory's lanes), so the exponentials' 1024 clocks and the rest do not
+// overlap.  What did not help: the next tile's
 // maximum beside this one's exponentials (141 -> 154 us), two groups on
 // alternate tiles (157), the query operand in tensor memory (141), descriptors
 // in uniform registers (142), a warp of their own for the scores (96 rows of

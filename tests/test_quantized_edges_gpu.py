@@ -205,3 +205,20 @@ def test_append_refuses_what_overlaps(bits):
     one = ops.rope_append(q[1:2], k[1:2], v[1:2], slots[1:2], sin, cos, kc, vc, h, h, 64, q_out=qkv[3:4, :256])
     assert torch.equal(one, want[1:2])
     assert torch.equal(run(kc, vc, q=own, q_out=own), want)
+
+
+@pytest.mark.parametrize("rows", [1, 6, 40])
+@pytest.mark.parametrize("scores", [False, True])
+def test_attention_at_a_scale_near_zero(rows, scores):
+    """Queries of zeros at a softmax scale of 2^-100: all keys alike, those past the
+    end not at all."""
+    from flash_dllm_b200 import ops
+    q, caches, pt, spans, mb, tb, B, L = tq._attention_case(22, [(200, rows, 0), (70, rows, 0), (33, rows, 0)], 4, 2, 400,
+                                                            nan_past_end=True)
+    q[::2] = 0
+    out, sc = torch.full_like(q, 5.0), torch.zeros(B * L, device="cuda") if scores else None
+    plan, cap = ops.plan_cache_attention(mb, tb, q.shape[0], B, 64, L, q.device)
+    ops.attn_cache_int4(q, out, *caches, plan, cap, sc, 1.0, 4, 2, L, 2.0 ** -100, page_table=pt)
+    ref, err, _, _ = qr.attention(q, *caches, pt, spans, 4, 2, 2.0 ** -100, 1.0, B, L)
+    have = ~torch.isnan(ref[:, 0])
+    assert ((out.double() - ref).abs() <= err)[have].all()
